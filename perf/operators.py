@@ -268,7 +268,8 @@ class _Call:
 
         types = {torch.float32: G.DType.F32, torch.float16: G.DType.F16, torch.bfloat16: G.DType.BF16,
                  torch.int32: G.DType.U32}
-        space = {n: (types[t.dtype], tuple(t.shape)) for n, t in tensors.items()}
+        space = {n: (types[t.dtype], tuple(t.shape[:3]) + (t.shape[3:].numel(),) if t.dim() > 4 else tuple(t.shape))
+                 for n, t in tensors.items()}  # a table row holds four dims
         if op == "attention":
             space["workspace"] = (G.DType.U32, (G.attention_paged_workspace_words(
                 scalars["requests"], scalars["tokens"], scalars["q_heads"], scalars["kv_heads"], scalars["head_dim"]),))
@@ -283,7 +284,7 @@ class _Call:
         table = G.TensorTable(layout)
         token = {n: table.add_placed(n, place[n], d, s) for n, (d, s) in space.items()}
         heap.write_table(table.seal())
-        views = {n: torch.as_tensor(_Shared(heap.view(token[n]), self.device), device="cuda").view(t.dtype)
+        views = {n: torch.as_tensor(_Shared(heap.view(token[n]), self.device), device="cuda").view(t.dtype).view(t.shape)
                  for n, t in tensors.items()}
         for n, t in tensors.items():
             views[n].copy_(t)
