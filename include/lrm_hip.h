@@ -38,7 +38,8 @@ int lrm_abi_version(void);
  * exact rules the device enforces. */
 
 /* Kernels.all / catalog.json (src/Lrm.Gpu.Core/Kernels.g.fs:27-285): ids 0..13 are the reference catalog, 14..40
- * this backend's appended fast-path kernels, 41..46 appended fp32 kernels that do several of ids 0..13 in one launch.
+ * this backend's appended fast-path kernels, 41..46 appended fp32 kernels that do several of ids 0..13 in one launch,
+ * 47..49 the paged key/value cache of the fast set.
  * kind: 1 token, 2 u32, 3 i32, 4 f32; access: 1 read, 2 write, 3 readwrite, 4 meta; dtype_mask: bit (1 << DType code). */
 int lrm_catalog_count(void);
 int lrm_catalog_find(const char *name); /* id, or -1 */
@@ -105,6 +106,11 @@ int lrm_hip_create_heap(lrm_hip_device *d, const uint32_t *arenas, const uint64_
 int lrm_hip_write_table(lrm_hip_device *d, const void *image, uint64_t bytes);
 int lrm_hip_upload(lrm_hip_device *d, int slot, uint64_t offset, const void *src, uint64_t bytes);
 int lrm_hip_download(lrm_hip_device *d, int slot, uint64_t offset, void *dst, uint64_t bytes);
+/* An extension: the device address of `bytes` bytes of a page, for other libraries that use this GPU in the same process
+ * (their results go into a heap tensor, or a heap tensor to them, without a copy). It is valid until lrm_hip_destroy.
+ * Nothing orders their work with this device's stream: a caller waits for a submission before others read what it wrote,
+ * and for others' work before it submits what reads theirs. LRM_E_CONTRACT for slot 0 or a range past the page. */
+int lrm_hip_address(lrm_hip_device *d, int slot, uint64_t offset, uint64_t bytes, uint64_t *address);
 
 /* IGpuBackend.LoadKernels / IKernelSet (Backend.fs:104-108,144-147): the gfx950 code objects are part of this
  * library. Loads the reference kernel set (catalog ids 0-13, Kernels.g.fs:27-285, and ids 41-46, which give the same
@@ -113,7 +119,7 @@ int lrm_hip_download(lrm_hip_device *d, int slot, uint64_t offset, void *dst, ui
  * (ExecutionClass.fs:58), is the SHA-256 of the set's name and the library file's SHA-256. Runs the fp32 denormal
  * probe (Backend.fs:457-547): mode 1 preserve, 2 flush, 3 mixed. */
 int lrm_hip_load_kernels(lrm_hip_device *d, uint8_t shader_set_hash[32]);
-/* An extension of LoadKernels: the set to load, once per backend. LRM_HIP_KERNELS_FAST is every id (0-46, the
+/* An extension of LoadKernels: the set to load, once per backend. LRM_HIP_KERNELS_FAST is every id (0-49, the
  * appended fast path included) under its own shader-set hash, so its results form their own ExecutionClass: it only
  * claims that the same work on the same inputs gives the same bits (the row count chooses its k-split and attention
  * splits; its prefill and decode kernels sum in different orders), and no bit-identity claim crosses the two sets. */
@@ -128,6 +134,13 @@ int lrm_hip_contains(lrm_hip_device *d, uint32_t kernel); /* 1 or 0 */
  * epilogue end, in 100 MHz constant-clock ticks. The shipped build records nothing and returns LRM_E_ARG. */
 int lrm_hip_debug_gemm_stamps(lrm_hip_device *d, uint32_t kind, uint64_t *dst, uint64_t words);
 int lrm_hip_denormal_probe(lrm_hip_device *d, int *mode, uint32_t results[7]);
+
+/* The paged key/value cache (ids 47 paged_plan, 48 qk_norm_rope_append_paged, 49 attention_paged; no counterpart in the
+ * reference, whose cache is one sequence's rows): u32 words of attention_paged's workspace for dispatches of up to that many
+ * requests and tokens. The workspace's words must be zero before the first launch (a new heap's are); every launch leaves
+ * the ones that it counts in at zero. Dispatches that may overlap need a workspace each. */
+int lrm_attention_paged_workspace(uint32_t requests, uint32_t tokens, uint32_t q_heads, uint32_t kv_heads,
+                                  uint32_t head_dim, uint64_t *words);
 
 /* ICommandList (Backend.fs:125-136) and IGpuBackend.Begin/Submit/Wait (Backend.fs:148-153). A list created with
  * reusable = 1 is an extension for replay: it is captured into a HIP graph at its first submission and every

@@ -117,6 +117,8 @@ PROTOTYPES = {
     "lrm_hip_write_table": (C.c_int, [P, P, C.c_uint64]),
     "lrm_hip_upload": (C.c_int, [P, C.c_int, C.c_uint64, P, C.c_uint64]),
     "lrm_hip_download": (C.c_int, [P, C.c_int, C.c_uint64, P, C.c_uint64]),
+    "lrm_hip_address": (C.c_int, [P, C.c_int, C.c_uint64, C.c_uint64, U64P]),
+    "lrm_attention_paged_workspace": (C.c_int, [C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, U64P]),
     "lrm_hip_load_kernels": (C.c_int, [P, P]),
     "lrm_hip_load_kernel_set": (C.c_int, [P, C.c_uint32, P]),
     "lrm_hip_debug_gemm_stamps": (C.c_int, [P, C.c_uint32, P, C.c_uint64]),

@@ -10,6 +10,7 @@
 #include "../../include/lrm_hip.h"
 #include "contract.hpp"
 #include "device.hpp"
+#include "paged.hpp"
 #include "qwen_exec.hpp"
 #include "safetensors.hpp"
 #include "tokenizer.hpp"
@@ -316,6 +317,22 @@ int lrm_hip_download(lrm_hip_device* d, int slot, uint64_t off, void* dst, uint6
         need_ptr(d, "device");
         need_ptr(dst, "dst");
         d->d.download(slot, off, dst, bytes);
+    });
+}
+
+int lrm_hip_address(lrm_hip_device* d, int slot, uint64_t off, uint64_t bytes, uint64_t* address) {
+    return guard([&] {
+        need_ptr(d, "device");
+        need_ptr(address, "address");
+        *address = reinterpret_cast<uint64_t>(d->d.address(slot, off, bytes));
+    });
+}
+
+int lrm_attention_paged_workspace(uint32_t requests, uint32_t tokens, uint32_t q_heads, uint32_t kv_heads,
+                                  uint32_t head_dim, uint64_t* words) {
+    return guard([&] {
+        need_ptr(words, "words");
+        *words = paged::workspace_words(requests, tokens, q_heads, kv_heads, head_dim);
     });
 }
 

@@ -450,6 +450,8 @@ static std::vector<KernelSpec> base_catalog() {
 // The appended entries of this backend: the fast path (ids 14..40), defined next to its kernels' host code, then fusions
 // of the reference's own kernels (ids 41..46), whose results equal the dispatches they stand for bit for bit.
 std::vector<KernelSpec> fast_catalog();
+// The paged key/value cache (ids 47..49), part of the fast set.
+std::vector<KernelSpec> paged_catalog();
 
 // The checks of 43 and 45. w: rows, q_heads, kv_heads, head_dim, pos0; norms: q_norm's field, with k_norm and the tables after
 // it; caches: k_cache's, with v_cache after it.
@@ -568,6 +570,8 @@ const std::vector<KernelSpec>& catalog() {
         c.insert(c.end(), f.begin(), f.end());
         auto u = fused_catalog();
         c.insert(c.end(), u.begin(), u.end());
+        auto p = paged_catalog();
+        c.insert(c.end(), p.begin(), p.end());
         return c;
     }();
     return all;
@@ -667,6 +671,7 @@ static PreparedDispatch prepare_impl(const SealedTableView& table, int kernel, c
     pd.grid = k.grid(words);
     pd.physical = grid_physical(k.linear, pd.grid);
     if (k.check_counts) k.check_counts(words, counts);
+    if (k.check_tokens) k.check_tokens(pd.tokens);
     std::memcpy(pd.words.data(), words, 128);
     pd.words[0] = pd.physical.x;
     return pd;

@@ -2,7 +2,7 @@
 //   - heap constants, arenas and HeapLayout / HeapPlanner   (src/Lrm.Gpu.Core/HeapLayout.fs:149-525)
 //   - the 64-byte TensorRow and the sealed TensorTable image (src/Lrm.Gpu.Core/TensorTable.fs:46-474)
 //   - the 128-byte ArgBlock, catalog grids and folding        (src/Lrm.Gpu.Core/ArgBlock.fs:240-393)
-//   - the kernel catalog (ids 0..13 as catalog.json, plus this backend's appended fast and fused fp32 kernels)
+//   - the kernel catalog (ids 0..13 as catalog.json, plus this backend's appended fast, fused fp32 and paged-cache kernels)
 //   - Dispatch.prepare: word rules, token rules, aliasing     (src/Lrm.Gpu.Core/Dispatch.fs:48-173)
 // Violations throw ContractError, the counterpart of GpuContractException (src/Lrm.Gpu.Core/Errors.fs:7-13).
 #pragma once
@@ -150,6 +150,14 @@ struct Grid3 {
     int64_t x, y, z;
 };
 
+struct TokenUse {
+    int field;
+    Access access;
+    uint32_t token;
+    TensorRow row;
+    uint64_t start, end;  // byte range inside row.slot()
+};
+
 struct KernelSpec {
     const char* name;
     const char* family;
@@ -158,6 +166,8 @@ struct KernelSpec {
     Grid3 (*grid)(const uint32_t* w);                 // the logical grid from the argument words
     std::vector<FieldSpec> fields;                    // field i is word i + 1
     void (*check_counts)(const uint32_t* w, const uint32_t* counts);  // minimum element counts; counts[i] for field i
+    // rules between the tensors of a dispatch (tokens that must share a dtype), or nullptr
+    void (*check_tokens)(const std::vector<TokenUse>& tokens) = nullptr;
 };
 
 const std::vector<KernelSpec>& catalog();
@@ -169,14 +179,6 @@ struct Physical {
     uint32_t x, y, z;
 };
 Physical grid_physical(bool linear, const Grid3& g);
-
-struct TokenUse {
-    int field;
-    Access access;
-    uint32_t token;
-    TensorRow row;
-    uint64_t start, end;  // byte range inside row.slot()
-};
 
 struct PreparedDispatch {
     int kernel;

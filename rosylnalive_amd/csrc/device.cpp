@@ -198,6 +198,14 @@ void* Device::resolve(uint32_t token) const {
     return static_cast<uint8_t*>(slot_ptr(int(r.slot()))) + r.offset();
 }
 
+void* Device::address(int slot, uint64_t offset, uint64_t bytes) const {
+    if (!heap_created_) contract_fail("a device address needs the heap");
+    if (slot == kTableSlot) contract_fail("slot 0 is the table, written only by WriteTable");
+    const Page& p = layout_.page(slot);
+    if (offset > p.bytes || bytes > p.bytes - offset) contract_fail("the range ends past the page in slot %d", slot);
+    return static_cast<uint8_t*>(slot_ptr(slot)) + offset;
+}
+
 // ---------------------------------------------------------------- kernels
 
 // (of the file this library was loaded from: once per process)
@@ -227,6 +235,7 @@ std::array<uint8_t, 32> Device::load_kernels(KernelSet set) {
 
 bool Device::contains(int kernel) const {
     if (kernel < 0 || kernel >= catalog_size()) return false;
+    if (kernel >= kPagedFirstId) return set_ == KernelSet::Fast;
     if (kernel >= kFusedFirstId) return true;  // both sets: the bits of the reference kernels they stand for
     if (set_ == KernelSet::Reference && kernel >= fast_first_id()) return false;
     if (kernel < fast_first_id()) return catalog_launchers()[kernel] != nullptr;
@@ -234,6 +243,7 @@ bool Device::contains(int kernel) const {
 }
 
 static LaunchFn launcher_of(int kernel) {
+    if (kernel >= kPagedFirstId) return paged_launchers()[kernel - kPagedFirstId];
     if (kernel >= kFusedFirstId) return fused_launchers()[kernel - kFusedFirstId];
     return kernel < fast_first_id() ? catalog_launchers()[kernel] : fast_launchers()[kernel - fast_first_id()];
 }

@@ -44,8 +44,10 @@ using LaunchFn = void (*)(const PreparedDispatch& pd, void* const* ptr, hipStrea
 const LaunchFn* catalog_launchers();  // ids 0..13
 const LaunchFn* fast_launchers();     // ids 14..40
 int fast_first_id();
-const LaunchFn* fused_launchers();    // ids 41.. (kFusedFirstId)
+const LaunchFn* fused_launchers();    // ids 41..46 (kFusedFirstId)
+const LaunchFn* paged_launchers();    // ids 47.. (kPagedFirstId)
 constexpr int kFusedFirstId = 41;
+constexpr int kPagedFirstId = 47;
 
 class Device;
 class CommandList;
@@ -164,8 +166,8 @@ class Device {
 
     // IKernelSet. Two kernel sets, each its own ExecutionClass (its own shader-set hash), since they make different
     // bit-identity claims:
-    //   Reference: the reference's catalog, ids 0 .. fast_first_id() - 1, and the fused fp32 kernels, ids kFusedFirstId and
-    //     up, which keeps the BatchInvariance contract (a row alone equals the row in any batch; prefill equals decode and
+    //   Reference: the reference's catalog, ids 0 .. fast_first_id() - 1, and the fused fp32 kernels, ids kFusedFirstId ..
+    //     kPagedFirstId - 1, which keeps the BatchInvariance contract (a row alone equals the row in any batch; prefill equals decode and
     //     any chunked prefill);
     //   Fast: every id (the reference's catalog and the fast path), which only claims that the same work on the same
     //     inputs gives the same bits: its k-split and attention-split choices depend on the row count, and its
@@ -205,6 +207,8 @@ class Device {
     uint32_t collected_f16_range() const { return host_words()[kHostRange] | host_words()[kHostRange + 1]; }
     void* slot_ptr(int slot) const;
     void* resolve(uint32_t token) const;  // device pointer of a token's first byte
+    // The device address of a range of a page, for other users of this GPU in the process.
+    void* address(int slot, uint64_t offset, uint64_t bytes) const;
 
   private:
     friend class CommandList;

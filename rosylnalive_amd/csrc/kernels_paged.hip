@@ -1,0 +1,499 @@
+// A key/value cache in pages for batches of requests of any lengths (ids 47..49, the fast set): the step's page tables and
+// slots from the request lengths, the append of new keys and values to their slots, and the attention of the new tokens
+// over their requests' pages. Lengths, tables and slots are device memory, so a recorded list replays for new ones; every
+// index that comes from device memory is checked against its tensor before it is used.
+#include <hip/hip_runtime.h>
+
+#include <cmath>
+#include <cstdint>
+#include <cstring>
+#include <vector>
+
+#include "contract.hpp"
+#include "device.hpp"
+#include "fast_common.hpp"
+#include "paged.hpp"
+
+namespace lrm {
+
+using namespace fast;
+
+namespace {
+
+// a + b, at most 2^32 - 1 (still associative, so a scan in any order gives the same)
+__device__ __forceinline__ uint32_t add_sat(uint32_t a, uint32_t b) {
+    const uint32_t s = a + b;
+    return s < a ? 0xFFFFFFFFu : s;
+}
+
+// The inclusive scan of v over the workgroup's 256 threads; red: 4 words of LDS, free again after the next barrier.
+__device__ __forceinline__ uint32_t scan_sat(uint32_t v, uint32_t* red) {
+    const int t = threadIdx.x, lane = t & 63, wv = t >> 6;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const uint32_t o = __shfl_up(v, d, 64);
+        if (lane >= d) v = add_sat(v, o);
+    }
+    if (lane == 63) red[wv] = v;
+    __syncthreads();
+    for (int i = 0; i < wv; ++i) v = add_sat(v, red[i]);
+    return v;
+}
+
+// the first r with ends[r] > x (x < ends[n - 1])
+__device__ __forceinline__ int first_above(const uint32_t* ends, int n, uint32_t x) {
+    int lo = 0, hi = n - 1;
+    while (lo < hi) {
+        const int m = (lo + hi) >> 1;
+        if (ends[m] > x)
+            hi = m;
+        else
+            lo = m + 1;
+    }
+    return lo;
+}
+
+// ---------------------------------------------------------------- 47 paged_plan
+// begin = min(past, blocks page), end = min(past + fresh, blocks page); request r takes ceil(end / page) - ceil(begin /
+// page) pages off the free list, after those of the requests before it; row j of its fresh ones has position past + j and
+// the slot of that position. Every workgroup scans the R lengths itself (two scans in LDS, at most 16 requests a thread)
+// and then finds its rows' requests by bisection, so one launch does it: what bounds it is the latency of the lengths'
+// load, the scans and the table's load one after the other.
+__global__ __launch_bounds__(256) void k_paged_plan(const uint32_t* past, const uint32_t* fresh, const uint32_t* free,
+                                                    uint32_t* table, uint32_t* starts, uint32_t* context,
+                                                    uint32_t* positions, uint32_t* slots, uint32_t* counts, uint32_t R,
+                                                    uint32_t blocks, uint32_t page_log2, uint32_t pages, uint32_t free_count,
+                                                    uint32_t tokens) {
+    __shared__ uint32_t row_end[paged::kMaxRequests];
+    __shared__ uint32_t new_end[paged::kMaxRequests];
+    __shared__ uint32_t red[8];
+    __shared__ uint32_t over;
+    const uint32_t t = threadIdx.x, page = 1u << page_log2, most = blocks * page;
+    auto pages_of = [&](uint32_t n) { return (n >> page_log2) + uint32_t((n & (page - 1)) != 0); };
+    auto need_of = [&](uint32_t p, uint32_t f) {
+        return pages_of(min(add_sat(p, f), most)) - pages_of(min(p, most));
+    };
+    if (t == 0) over = 0;
+    __syncthreads();
+    // thread t's requests per_thread t ..
+    const uint32_t per = (R + 255) / 256, r0 = min(t * per, R), r1 = min(r0 + per, R);
+    uint32_t rows = 0, fills = 0, past_most = 0;
+    for (uint32_t r = r0; r < r1; ++r) {
+        const uint32_t p = past[r], f = fresh[r];
+        rows = add_sat(rows, f);
+        fills = add_sat(fills, need_of(p, f));
+        past_most |= add_sat(p, f) > most;
+        row_end[r] = rows;
+        new_end[r] = fills;
+    }
+    if (past_most) over = 1;
+    const uint32_t rows_end = scan_sat(rows, red), fills_end = scan_sat(fills, red + 4);
+    // what the threads before this one hold (a saturated sum says nothing of its parts)
+    const uint32_t rows_before = __shfl_up(rows_end, 1, 64), fills_before = __shfl_up(fills_end, 1, 64);
+    uint32_t rb = rows_before, fb = fills_before;
+    if ((t & 63) == 0) {
+        rb = fb = 0;
+        for (uint32_t i = 0; i < (t >> 6); ++i) {
+            rb = add_sat(rb, red[i]);
+            fb = add_sat(fb, red[4 + i]);
+        }
+    }
+    for (uint32_t r = r0; r < r1; ++r) {
+        row_end[r] = add_sat(row_end[r], rb);
+        new_end[r] = add_sat(new_end[r], fb);
+    }
+    __syncthreads();
+    const uint32_t total = row_end[R - 1], fill = new_end[R - 1];
+    if (blockIdx.x == 0) {
+        for (uint32_t r = t; r < R; r += 256) {
+            starts[r + 1] = min(row_end[r], tokens);
+            context[r] = min(add_sat(past[r], fresh[r]), most);
+        }
+        if (t == 0) {
+            starts[0] = 0;
+            counts[0] = total;
+            counts[1] = fill;
+            counts[2] = uint32_t(total > tokens) | over << 1 | uint32_t(fill > free_count) << 2;
+        }
+    }
+    const uint32_t at = blockIdx.x * 256 + t, stride = gridDim.x * 256;
+    for (uint32_t e = at; e < fill; e = add_sat(e, stride)) {
+        const int r = first_above(new_end, int(R), e);
+        const uint32_t j = e - (r ? new_end[r - 1] : 0);
+        table[size_t(r) * blocks + pages_of(min(past[r], most)) + j] = e < free_count ? free[e] : paged::kNone;
+    }
+    const uint32_t valid = min(total, tokens);
+    for (uint32_t i = at; i < valid; i = add_sat(i, stride)) {
+        const int r = first_above(row_end, int(R), i);
+        const uint64_t pos = uint64_t(past[r]) + (i - (r ? row_end[r - 1] : 0));
+        uint32_t slot = paged::kNone;
+        if (pos < most) {
+            const uint32_t b = uint32_t(pos) >> page_log2, have = pages_of(min(past[r], most));
+            uint32_t id = paged::kNone;
+            if (b < have) {
+                id = table[size_t(r) * blocks + b];
+            } else {
+                const uint32_t e = (r ? new_end[r - 1] : 0) + (b - have);
+                if (e < free_count) id = free[e];
+            }
+            if (id < pages) slot = (id << page_log2) + (uint32_t(pos) & (page - 1));
+        }
+        positions[i] = uint32_t(pos);
+        slots[i] = slot;
+    }
+}
+
+// ---------------------------------------------------------------- element types
+
+template <typename T>
+__device__ __forceinline__ float widen(T v);
+template <>
+__device__ __forceinline__ float widen<float>(float v) {
+    return v;
+}
+template <>
+__device__ __forceinline__ float widen<_Float16>(_Float16 v) {
+    return static_cast<float>(v);
+}
+template <>
+__device__ __forceinline__ float widen<__bf16>(__bf16 v) {
+    return bf2f(__builtin_bit_cast(uint16_t, v));
+}
+template <typename T>
+__device__ __forceinline__ T narrow(float v);
+template <>
+__device__ __forceinline__ _Float16 narrow<_Float16>(float v) {
+    return static_cast<_Float16>(v);
+}
+template <>
+__device__ __forceinline__ __bf16 narrow<__bf16>(float v) {
+    return __builtin_bit_cast(__bf16, f2bf(v));
+}
+
+// ---------------------------------------------------------------- 48 qk_norm_rope_append_paged
+// One wave per (row, head): the head's sum of squares over the wave, its norm and rotation, one store. The values' eight
+// positions of a tile come from eight rows, so their stores are two bytes each.
+template <typename IN, typename T, int HD>
+__global__ __launch_bounds__(256) void k_paged_append(const IN* qkv, const uint16_t* qn, const uint16_t* kn,
+                                                      const float* cos_t, const float* sin_t, const uint32_t* starts,
+                                                      const uint32_t* positions, const uint32_t* slots, T* q, T* kc, T* vc,
+                                                      uint32_t requests, uint32_t tokens, uint32_t qh, uint32_t kvh,
+                                                      uint32_t max_pos, uint32_t page_log2, uint32_t pages, float eps) {
+    constexpr int H = HD / 2;
+    const uint32_t row = blockIdx.x, lane = threadIdx.x & 63, head = blockIdx.y * 4 + (threadIdx.x >> 6);
+    if (row >= min(starts[requests], tokens) || head >= qh + 2 * kvh) return;
+    const uint32_t pos = positions[row], slot = slots[row], id = slot >> page_log2, off = slot & ((1u << page_log2) - 1);
+    const bool in = lane < H;
+    const IN* x = qkv + (size_t(row) * (qh + 2 * kvh) + head) * HD;
+    const float a = in ? widen(x[lane]) : 0.f, b = in ? widen(x[lane + H]) : 0.f;
+    if (head >= qh + kvh) {
+        if (id >= pages || pos >= max_pos || !in) return;
+        T* v = vc + ((size_t(id) * kvh + (head - qh - kvh)) << page_log2) * HD + size_t(off >> 3) * (8 * HD) + (off & 7);
+        v[lane * 8] = narrow<T>(a);
+        v[(lane + H) * 8] = narrow<T>(b);
+        return;
+    }
+    const float r = 1.0f / sqrtf(wave_sum(a * a + b * b) / float(HD) + eps);
+    if (!in) return;
+    const uint16_t* w = head < qh ? qn : kn;
+    const float an = bf2f(w[lane]) * (a * r), bn = bf2f(w[lane + H]) * (b * r);
+    float lo = 0.f, hi = 0.f;
+    if (pos < max_pos) {
+        const float c = cos_t[size_t(pos) * H + lane], s = sin_t[size_t(pos) * H + lane];
+        lo = an * c - bn * s;
+        hi = bn * c + an * s;
+    }
+    if (head < qh) {
+        T* y = q + (size_t(row) * qh + head) * HD;
+        y[lane] = narrow<T>(lo);
+        y[lane + H] = narrow<T>(hi);
+    } else if (id < pages && pos < max_pos) {
+        T* k = kc + (((size_t(id) * kvh + (head - qh)) << page_log2) + off) * HD;
+        k[lane] = narrow<T>(lo);
+        k[lane + H] = narrow<T>(hi);
+    }
+}
+
+// ---------------------------------------------------------------- 49 attention_paged
+// One wave per (row, query head): a key per lane for the scores, a dim (or two) per lane for the products.
+template <typename T, int HD>
+__global__ __launch_bounds__(64) void k_paged_attn(const T* q, const T* kc, const T* vc, const uint32_t* table,
+                                                   const uint32_t* starts, const uint32_t* context, T* y, uint32_t requests,
+                                                   uint32_t tokens, uint32_t max_fresh, uint32_t qh, uint32_t kvh,
+                                                   uint32_t blocks, uint32_t page_log2, uint32_t pages, float scale_log2) {
+    __shared__ float qs[HD];
+    __shared__ float ps[64];
+    const uint32_t row = blockIdx.x, head = blockIdx.y, lane = threadIdx.x, page = 1u << page_log2;
+    if (row >= min(starts[requests], tokens)) return;
+    uint32_t lo = 0, hi = requests - 1;
+    while (lo < hi) {  // the first request that ends behind the row
+        const uint32_t m = (lo + hi) >> 1;
+        if (starts[m + 1] > row)
+            hi = m;
+        else
+            lo = m + 1;
+    }
+    const uint32_t first = starts[lo];
+    if (first > row || row - first >= max_fresh) return;
+    const int64_t fresh = int64_t(min(starts[lo + 1], tokens)) - first;
+    const int64_t keys = int64_t(min(context[lo], blocks * page)) - fresh + (row - first) + 1;
+    const T* qr = q + (size_t(row) * qh + head) * HD;
+    for (int d = lane; d < HD; d += 64) qs[d] = widen(qr[d]);
+    __syncthreads();
+    const uint32_t kvhead = head / (qh / kvh);
+    float m_run = -INFINITY, l_run = 0.f, o[HD / 64];
+    for (int i = 0; i < HD / 64; ++i) o[i] = 0.f;
+    for (int64_t k0 = 0; k0 < keys; k0 += 64) {
+        const uint32_t key = uint32_t(k0) + lane;
+        const uint32_t id = key < keys ? table[size_t(lo) * blocks + (key >> page_log2)] : paged::kNone;
+        float s = -INFINITY;
+        if (id < pages) {
+            const T* k = kc + (((size_t(id) * kvh + kvhead) << page_log2) + (key & (page - 1))) * HD;
+            s = 0.f;
+            for (int d = 0; d < HD; ++d) s = fmaf(qs[d], widen(k[d]), s);
+            s *= scale_log2;
+        }
+        const float m = fmaxf(m_run, wave_max(s));
+        const float base = m == -INFINITY ? 0.f : m;
+        const float p = exp2f(s - base), alpha = exp2f(m_run - base);
+        l_run = l_run * alpha + wave_sum(p);
+        m_run = m;
+        ps[lane] = p;
+        __syncthreads();
+        for (int i = 0; i < HD / 64; ++i) o[i] *= alpha;
+        for (uint32_t j = 0; j < 64 && k0 + j < keys; ++j) {
+            const uint32_t kj = uint32_t(k0) + j, ij = table[size_t(lo) * blocks + (kj >> page_log2)], off = kj & (page - 1);
+            if (ij >= pages) continue;
+            const T* v = vc + ((size_t(ij) * kvh + kvhead) << page_log2) * HD + size_t(off >> 3) * (8 * HD) + (off & 7);
+            for (int i = 0; i < HD / 64; ++i) o[i] = fmaf(ps[j], widen(v[(lane + 64 * i) * 8]), o[i]);
+        }
+        __syncthreads();
+    }
+    for (int i = 0; i < HD / 64; ++i)
+        y[(size_t(row) * qh + head) * HD + lane + 64 * i] = narrow<T>(l_run > 0.f ? o[i] / l_run : o[i]);
+}
+
+}  // namespace
+
+// ---------------------------------------------------------------- launchers
+
+static uint32_t log2_of(uint32_t page) { return uint32_t(__builtin_ctz(page)); }
+static float f32_of(uint32_t b) {
+    float f;
+    std::memcpy(&f, &b, 4);
+    return f;
+}
+static uint32_t dtype_of(const PreparedDispatch& pd, int field) {
+    for (const TokenUse& u : pd.tokens)
+        if (u.field == field) return u.row.dtype();
+    return 0;
+}
+
+// rows and new pages are shared out over at most 512 workgroups
+static uint32_t plan_blocks(uint32_t tokens) { return std::min(512u, (tokens + 255) / 256); }
+
+// past, fresh, free, table, starts, context, positions, slots, counts, requests, blocks, page, pages, free_count, tokens
+static void l_plan(const PreparedDispatch& pd, void* const* p, hipStream_t s) {
+    const uint32_t* w = pd.words.data();
+    auto u = [&](int i) { return (uint32_t*)p[i]; };
+    hipLaunchKernelGGL(k_paged_plan, dim3(plan_blocks(w[15])), dim3(256), 0, s, u(0), u(1), u(2), u(3), u(4), u(5), u(6),
+                       u(7), u(8), w[10], w[11], log2_of(w[12]), w[13], w[14], w[15]);
+}
+
+// qkv, q_norm, k_norm, cos_table, sin_table, starts, positions, slots, q, k_cache, v_cache, requests, tokens, q_heads,
+// kv_heads, head_dim, max_pos, page, pages, eps
+template <typename IN, typename T, int HD>
+static void launch_append(const uint32_t* w, void* const* p, hipStream_t s) {
+    hipLaunchKernelGGL((k_paged_append<IN, T, HD>), dim3(w[13], (w[14] + 2 * w[15] + 3) / 4), dim3(256), 0, s,
+                       (const IN*)p[0], (const uint16_t*)p[1], (const uint16_t*)p[2], (const float*)p[3],
+                       (const float*)p[4], (const uint32_t*)p[5], (const uint32_t*)p[6], (const uint32_t*)p[7], (T*)p[8],
+                       (T*)p[9], (T*)p[10], w[12], w[13], w[14], w[15], w[17], log2_of(w[18]), w[19], f32_of(w[20]));
+}
+template <typename IN, typename T>
+static void launch_append(const uint32_t* w, void* const* p, hipStream_t s) {
+    if (w[16] == 64)
+        launch_append<IN, T, 64>(w, p, s);
+    else
+        launch_append<IN, T, 128>(w, p, s);
+}
+static void l_append(const PreparedDispatch& pd, void* const* p, hipStream_t s) {
+    const uint32_t* w = pd.words.data();
+    const bool half = dtype_of(pd, 8) == F16;
+    if (dtype_of(pd, 0) == F32) {
+        if (half)
+            launch_append<float, _Float16>(w, p, s);
+        else
+            launch_append<float, __bf16>(w, p, s);
+    } else if (half) {
+        launch_append<_Float16, _Float16>(w, p, s);
+    } else {
+        launch_append<__bf16, __bf16>(w, p, s);
+    }
+}
+
+// q, k_cache, v_cache, table, starts, context, y, workspace, requests, tokens, max_fresh, q_heads, kv_heads, head_dim,
+// blocks, page, pages, scale
+template <typename T, int HD>
+static void launch_attn(const uint32_t* w, void* const* p, hipStream_t s) {
+    hipLaunchKernelGGL((k_paged_attn<T, HD>), dim3(w[10], w[12]), dim3(64), 0, s, (const T*)p[0], (const T*)p[1],
+                       (const T*)p[2], (const uint32_t*)p[3], (const uint32_t*)p[4], (const uint32_t*)p[5], (T*)p[6], w[9],
+                       w[10], w[11] ? w[11] : w[10], w[12], w[13], w[15], log2_of(w[16]), w[17],
+                       f32_of(w[18]) * 1.4426950408889634f);
+}
+static void l_attn(const PreparedDispatch& pd, void* const* p, hipStream_t s) {
+    const uint32_t* w = pd.words.data();
+    const bool half = dtype_of(pd, 0) == F16;
+    if (w[14] == 64) {
+        if (half)
+            launch_attn<_Float16, 64>(w, p, s);
+        else
+            launch_attn<__bf16, 64>(w, p, s);
+    } else if (half) {
+        launch_attn<_Float16, 128>(w, p, s);
+    } else {
+        launch_attn<__bf16, 128>(w, p, s);
+    }
+}
+
+const LaunchFn* paged_launchers() {
+    static const LaunchFn t[] = {l_plan, l_append, l_attn};
+    return t;
+}
+
+// ---------------------------------------------------------------- catalog entries (ids 47..49)
+
+#define DT(x) (1u << (x))
+#define TOK_R(n, m) FieldSpec{n, FieldKind::Token, Access::Read, m, nullptr}
+#define TOK_W(n, m) FieldSpec{n, FieldKind::Token, Access::Write, m, nullptr}
+#define TOK_RW(n, m) FieldSpec{n, FieldKind::Token, Access::ReadWrite, m, nullptr}
+#define U32F(n) FieldSpec{n, FieldKind::U32, Access::None, 0, nullptr}
+#define F32F(n) FieldSpec{n, FieldKind::F32, Access::None, 0, nullptr}
+
+static void need(const uint32_t* counts, int field, uint64_t elems, const char* kernel, const char* what) {
+    if (counts[field] < elems)
+        contract_fail("%s.%s holds %u elements; the dispatch touches %llu", kernel, what, counts[field],
+                      (unsigned long long)elems);
+}
+// a product of three words (each below 2^32, the last two of them dimensions of a tensor row) that cannot wrap
+static uint64_t times(uint64_t a, uint64_t b, uint64_t c = 1) {
+    const __uint128_t v = (__uint128_t)a * b * c;
+    return v >> 64 ? ~0ull : uint64_t(v);
+}
+
+static void need_step(const char* n, uint32_t requests, uint32_t tokens) {
+    if (requests < 1 || requests > paged::kMaxRequests)
+        contract_fail("%s: requests must be in 1 .. %u", n, paged::kMaxRequests);
+    if (tokens < 1) contract_fail("%s: tokens must be at least 1", n);
+}
+static void need_pages(const char* n, uint32_t page, uint32_t pages) {
+    if (!paged::page_ok(page)) contract_fail("%s: page must be a power of two in 16 .. 256", n);
+    if (pages < 1 || times(pages, page) > 0xFFFFFFFFull)
+        contract_fail("%s: pages must be at least 1, and pages * page at most 2^32 - 1", n);
+}
+static void need_table(const char* n, uint32_t blocks, uint32_t page) {
+    if (blocks < 1 || times(blocks, page) > 0xFFFFFFFFull)
+        contract_fail("%s: blocks must be at least 1, and blocks * page at most 2^32 - 1", n);
+}
+static void need_heads(const char* n, uint32_t qh, uint32_t kvh, uint32_t hd) {
+    if (kvh < 1 || qh < 1 || qh % kvh) contract_fail("%s: kv_heads must divide q_heads", n);
+    if (hd != 64 && hd != 128) contract_fail("%s: head_dim must be 64 or 128", n);
+}
+static void same_dtype(const char* n, const std::vector<TokenUse>& tokens, std::initializer_list<int> fields) {
+    uint32_t first = 0;
+    for (const TokenUse& u : tokens)
+        for (int f : fields)
+            if (u.field == f) {
+                if (!first) first = u.row.dtype();
+                if (u.row.dtype() != first)
+                    contract_fail("%s: %s and %s cannot be mixed in one dispatch", n, dtype_name(first),
+                                  dtype_name(u.row.dtype()));
+            }
+}
+
+std::vector<KernelSpec> paged_catalog() {
+    std::vector<KernelSpec> c;
+    const uint32_t U = DT(U32), H = DT(F16) | DT(BF16);
+    // 47 paged_plan
+    c.push_back({"paged_plan", "paged", {256, 1, 1}, true,
+                 [](const uint32_t* w) { return Grid3{plan_blocks(w[15]), 1, 1}; },
+                 {TOK_R("past", U), TOK_R("fresh", U), TOK_R("free", U), TOK_RW("table", U), TOK_W("starts", U),
+                  TOK_W("context", U), TOK_W("positions", U), TOK_W("slots", U), TOK_W("counts", U), U32F("requests"),
+                  U32F("blocks"), U32F("page"), U32F("pages"), U32F("free_count"), U32F("tokens")},
+                 [](const uint32_t* w, const uint32_t* c) {
+                     const char* n = "paged_plan";
+                     const uint32_t R = w[10], blocks = w[11], page = w[12], pages = w[13], free_count = w[14], T = w[15];
+                     need_step(n, R, T);
+                     need_pages(n, page, pages);
+                     need_table(n, blocks, page);
+                     need(c, 0, R, n, "past");
+                     need(c, 1, R, n, "fresh");
+                     need(c, 2, free_count, n, "free");
+                     need(c, 3, times(R, blocks), n, "table");
+                     need(c, 4, uint64_t(R) + 1, n, "starts");
+                     need(c, 5, R, n, "context");
+                     need(c, 6, T, n, "positions");
+                     need(c, 7, T, n, "slots");
+                     need(c, 8, 3, n, "counts");
+                 }});
+    // 48 qk_norm_rope_append_paged
+    c.push_back({"qk_norm_rope_append_paged", "paged", {256, 1, 1}, false,
+                 [](const uint32_t* w) { return Grid3{w[13], (int64_t(w[14]) + 2 * int64_t(w[15]) + 3) / 4, 1}; },
+                 {TOK_R("qkv", H | DT(F32)), TOK_R("q_norm", DT(BF16)), TOK_R("k_norm", DT(BF16)),
+                  TOK_R("cos_table", DT(F32)), TOK_R("sin_table", DT(F32)), TOK_R("starts", U), TOK_R("positions", U),
+                  TOK_R("slots", U), TOK_W("q", H), TOK_RW("k_cache", H), TOK_RW("v_cache", H), U32F("requests"),
+                  U32F("tokens"), U32F("q_heads"), U32F("kv_heads"), U32F("head_dim"), U32F("max_pos"), U32F("page"),
+                  U32F("pages"), F32F("eps")},
+                 [](const uint32_t* w, const uint32_t* c) {
+                     const char* n = "qk_norm_rope_append_paged";
+                     const uint32_t R = w[12], T = w[13], qh = w[14], kvh = w[15], hd = w[16], mp = w[17], page = w[18],
+                                    pages = w[19];
+                     need_step(n, R, T);
+                     need_heads(n, qh, kvh, hd);
+                     need_pages(n, page, pages);
+                     if (mp < 1) contract_fail("%s: max_pos must be at least 1", n);
+                     need(c, 0, times(T, uint64_t(qh) + 2 * uint64_t(kvh), hd), n, "qkv");
+                     need(c, 1, hd, n, "q_norm");
+                     need(c, 2, hd, n, "k_norm");
+                     need(c, 3, times(mp, hd / 2), n, "cos_table");
+                     need(c, 4, times(mp, hd / 2), n, "sin_table");
+                     need(c, 5, uint64_t(R) + 1, n, "starts");
+                     need(c, 6, T, n, "positions");
+                     need(c, 7, T, n, "slots");
+                     need(c, 8, times(T, qh, hd), n, "q");
+                     need(c, 9, times(uint64_t(pages) * page, kvh, hd), n, "k_cache");
+                     need(c, 10, times(uint64_t(pages) * page, kvh, hd), n, "v_cache");
+                 },
+                 [](const std::vector<TokenUse>& t) {
+                     same_dtype("qk_norm_rope_append_paged", t, {8, 9, 10});
+                     if (t[0].row.dtype() != F32) same_dtype("qk_norm_rope_append_paged", t, {0, 8});
+                 }});
+    // 49 attention_paged
+    c.push_back({"attention_paged", "paged", {64, 1, 1}, false, [](const uint32_t* w) { return Grid3{w[10], w[12], 1}; },
+                 {TOK_R("q", H), TOK_R("k_cache", H), TOK_R("v_cache", H), TOK_R("table", U), TOK_R("starts", U),
+                  TOK_R("context", U), TOK_W("y", H), TOK_RW("workspace", U), U32F("requests"), U32F("tokens"),
+                  U32F("max_fresh"), U32F("q_heads"), U32F("kv_heads"), U32F("head_dim"), U32F("blocks"), U32F("page"),
+                  U32F("pages"), F32F("scale")},
+                 [](const uint32_t* w, const uint32_t* c) {
+                     const char* n = "attention_paged";
+                     const uint32_t R = w[9], T = w[10], qh = w[12], kvh = w[13], hd = w[14], blocks = w[15], page = w[16],
+                                    pages = w[17];
+                     need_step(n, R, T);
+                     need_heads(n, qh, kvh, hd);
+                     need_pages(n, page, pages);
+                     need_table(n, blocks, page);
+                     const float scale = f32_of(w[18]);
+                     if (!(scale > 0.f) || std::isinf(scale)) contract_fail("%s: scale must be positive and finite", n);
+                     need(c, 0, times(T, qh, hd), n, "q");
+                     need(c, 1, times(uint64_t(pages) * page, kvh, hd), n, "k_cache");
+                     need(c, 2, times(uint64_t(pages) * page, kvh, hd), n, "v_cache");
+                     need(c, 3, times(R, blocks), n, "table");
+                     need(c, 4, uint64_t(R) + 1, n, "starts");
+                     need(c, 5, R, n, "context");
+                     need(c, 6, times(T, qh, hd), n, "y");
+                     need(c, 7, paged::workspace_words(R, T, qh, kvh, hd), n, "workspace");
+                 },
+                 [](const std::vector<TokenUse>& t) { same_dtype("attention_paged", t, {0, 1, 2, 6}); }});
+    return c;
+}
+
+}  // namespace lrm

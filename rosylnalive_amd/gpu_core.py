@@ -20,7 +20,7 @@ from ._native import Fp16RangeError, GpuContractException, HipDeviceError, LrmEr
 __all__ = [
     "Fp16RangeError", "GpuContractException", "HipDeviceError", "LrmError", "Heap", "DType", "Arena", "TensorFlags", "Catalog",
     "KernelSpec", "ArgBlock", "HeapLayout", "HeapPlanner", "TensorTable", "SealedTable", "HipBackendProvider",
-    "HipBackend", "HipHeap", "HipCommandList", "Submission", "Completion", "TimerResult", "prepare", "grid_physical",
+    "HipBackend", "HipHeap", "HeapView", "HipCommandList", "Submission", "Completion", "TimerResult", "prepare", "grid_physical",
 ]
 
 
@@ -161,6 +161,18 @@ def attention_prefill_workspace_words(rows: int, kv_heads: int) -> int:
     any length share one buffer. The counters (word 0 of each record) must be zero before the first launch; every
     launch leaves them zero."""
     return max(1, kv_heads * (((rows + 31) // 32) // 2)) * ATTN_PREFILL_RECORD_WORDS
+
+
+PAGED_NONE = 0xFFFFFFFF  # paged_plan, qk_norm_rope_append_paged, attention_paged: no page, no slot
+
+
+def attention_paged_workspace_words(requests: int, tokens: int, q_heads: int, kv_heads: int, head_dim: int) -> int:
+    """u32 words of attention_paged's workspace for dispatches of up to so many requests and tokens
+    (lrm_attention_paged_workspace). Its words must be zero before the first launch; every launch leaves the ones that it
+    counts in at zero, so launches of other lengths can follow. Dispatches that may overlap need a workspace each."""
+    words = C.c_uint64()
+    check(lib().lrm_attention_paged_workspace(requests, tokens, q_heads, kv_heads, head_dim, C.byref(words)))
+    return words.value
 
 
 def grid_physical(linear: bool, x: int, y: int, z: int) -> Tuple[int, int, int]:
@@ -476,6 +488,44 @@ class HipHeap:
         buf = C.create_string_buffer(nbytes)
         check(lib().lrm_hip_download(self.backend._h, slot, offset, buf, nbytes))
         return buf.raw
+
+    def address(self, slot: int, offset: int, nbytes: int) -> int:
+        """The device address of a range of a page (lrm_hip_address), valid until the backend closes."""
+        out = C.c_uint64()
+        check(lib().lrm_hip_address(self.backend._h, slot, offset, nbytes, C.byref(out)))
+        return out.value
+
+    def view(self, token: int) -> "HeapView":
+        """The tensor of a table token, shared with other libraries on this GPU."""
+        if self.table is None:
+            raise GpuContractException(N.LRM_E_CONTRACT, "the table has not been written")
+        row = self.table.row(token)
+        if token == 0 or not any(row):
+            raise GpuContractException(N.LRM_E_CONTRACT, f"token {token} is not in the table")
+        return HeapView(self, row)
+
+
+class HeapView:
+    """A heap tensor to other libraries that use this GPU in the process, without a copy (`__cuda_array_interface__`: torch,
+    cupy). bf16 and u32, which the interface lacks or few libraries take, come as the int16 and int32 that hold their
+    bits. Both sides have to use one HIP runtime: a program that uses torch imports it before this package loads its library,
+    which then finds torch's. It keeps the backend object alive, not its memory: nothing may use it after HipBackend.close. Nothing orders
+    the other library's work with the backend's stream: wait for a submission before reading what it wrote, and
+    synchronise the other library before submitting what reads its writes."""
+
+    TYPESTR = {DType.F32: "<f4", DType.BF16: "<i2", DType.F16: "<f2", DType.I32: "<i4", DType.U32: "<i4", DType.U8: "|u1",
+               DType.F64: "<f8", DType.I64: "<i8"}
+
+    def __init__(self, heap: "HipHeap", row: Sequence[int]):
+        self.heap = heap
+        slot, offset, dtype, rank = row[:4]
+        self.shape, strides = tuple(row[4:4 + rank]), tuple(row[8:8 + rank])
+        size = DType.SIZE[dtype]
+        extent = (1 + sum((d - 1) * s for d, s in zip(self.shape, strides))) * size
+        self.address = heap.address(slot, offset, extent)
+        self.__cuda_array_interface__ = {
+            "shape": self.shape, "typestr": self.TYPESTR[dtype], "data": (self.address, bool(row[13] & TensorFlags.READ_ONLY)),
+            "strides": None if row[13] & TensorFlags.CONTIGUOUS else tuple(s * size for s in strides), "version": 2}
 
 
 class HipCommandList:
