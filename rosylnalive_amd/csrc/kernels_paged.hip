@@ -4,9 +4,11 @@
 // index that comes from device memory is checked against its tensor before it is used.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
 #include <cstring>
+#include <type_traits>
 #include <vector>
 
 #include "contract.hpp"
@@ -215,6 +217,355 @@ __global__ __launch_bounds__(256) void k_paged_append(const IN* qkv, const uint1
 }
 
 // ---------------------------------------------------------------- 49 attention_paged
+struct AttnArgs {
+    const void *q, *kc, *vc;
+    const uint32_t *table, *starts, *context;
+    void* y;
+    uint32_t* ws;
+    uint32_t requests, tokens, max_fresh, qh, kvh, blocks, page_log2, pages;
+    float scale_log2;  // the scale times log2(e): weights are 2^(s scale_log2 - m scale_log2)
+};
+
+// A request as its lengths on the device give it, clamped to the tensors.
+struct Request {
+    int row0;  // its first row
+    int rows;  // the rows that this dispatch computes
+    int seen;  // the keys that row 0 sees; row i sees i more (below 1: none)
+};
+__device__ __forceinline__ Request request_of(const AttnArgs& a, uint32_t r) {
+    const uint32_t s0 = min(a.starts[r], a.tokens), s1 = min(a.starts[r + 1], a.tokens);
+    const int fresh = s1 > s0 ? int(s1 - s0) : 0, ctx = int(min(a.context[r], a.blocks << a.page_log2));
+    return Request{int(s0), min(fresh, int(a.max_fresh)), ctx - fresh + 1};
+}
+
+template <typename T>
+struct Mfma;
+template <>
+struct Mfma<_Float16> {
+    typedef f16x8 vec;
+    static __device__ __forceinline__ f32x4 m16(u32x4 a, u32x4 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(vec, a), __builtin_bit_cast(vec, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack2h(a, b); }
+};
+template <>
+struct Mfma<__bf16> {
+    typedef bf16x8 vec;
+    static __device__ __forceinline__ f32x4 m16(u32x4 a, u32x4 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(vec, a), __builtin_bit_cast(vec, b), c, 0, 0, 0);
+    }
+    // two floats to a bf16 pair, round to nearest even (one v_cvt_pk_bf16_f32)
+    static __device__ __forceinline__ uint32_t pack(float a, float b) {
+        typedef __bf16 h2 __attribute__((ext_vector_type(2)));
+        typedef float f2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2){a, b}, h2));
+    }
+};
+
+__device__ __forceinline__ void store_agent(float* p, float a, float b) {
+    __hip_atomic_store(reinterpret_cast<uint64_t*>(p), uint64_t(__float_as_uint(a)) | (uint64_t(__float_as_uint(b)) << 32),
+                       __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 load_agent(const float* p) {
+    const uint64_t v =
+        __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return make_float2(__uint_as_float(uint32_t(v)), __uint_as_float(uint32_t(v >> 32)));
+}
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// Rows of few query columns: up to 16 per request and KV head (column c = row c / group, head c % group of the KV head's).
+// Bound by the cache's bytes, so every wave streams its own keys straight into the registers that the matrix
+// instruction reads (no LDS, no barrier), two units in flight, and the four waves of a workgroup meet once per item.
+//
+// A unit is 128 keys of an item, 32 per wave. S^T = K Q^T on 16 x 16 x 32 tiles: the two tiles' rows i hold the keys
+// 8 (i / 4) + 4 tile + i % 4, so that lane group g = lane / 16 gets the scores of the eight keys 8 g .. 8 g + 7 of its column:
+// exactly the operand that O^T = V^T P^T wants from it, with V's operand one 16-byte read of eight positions of a dim.
+// No value crosses lanes but the maximum. Keys that no column sees and pages that are none are read past the buffer's
+// end, which gives zeros without an access.
+template <typename T, int HD>
+__global__ __launch_bounds__(256, 2) void k_attn_rows(AttnArgs a, uint32_t k_bytes, uint32_t v_bytes) {
+    using M = Mfma<T>;
+    constexpr int KS = HD / 32, DT = HD / 16, XR = HD + 4;  // dim steps, dim tiles, padded row of the exchange
+    constexpr uint32_t kOut = 0x80000000u;                   // an offset past every buffer
+    __shared__ uint32_t ends[paged::kMaxRequests];           // units of the requests up to and with r
+    __shared__ __attribute__((aligned(16))) float xo[4 * 16 * XR];
+    __shared__ float xm[4][16], xl[4][16];
+    __shared__ uint32_t red[4];
+    __shared__ uint32_t arrived;
+    const int t = threadIdx.x, lane = t & 63, wv = t >> 6, c16 = lane & 15, g = lane >> 4;
+    const int group = int(a.qh / a.kvh), kvh = int(a.kvh);
+    const uint32_t page_mask = (1u << a.page_log2) - 1;
+
+    // ---- the units of every request, and this workgroup's
+    auto units_of = [&](const Request& q) {  // of one item of the request
+        if (q.rows < 1) return 0;
+        return max(1, (q.seen + q.rows - 1 + int(paged::kUnitKeys) - 1) / int(paged::kUnitKeys));
+    };
+    {
+        const uint32_t per = (a.requests + 255) / 256, r0 = min(t * per, a.requests), r1 = min(r0 + per, a.requests);
+        uint32_t sum = 0;
+        for (uint32_t r = r0; r < r1; ++r) {
+            sum += uint32_t(units_of(request_of(a, r)) * kvh);
+            ends[r] = sum;
+        }
+        const uint32_t before = scan_sat(sum, red) - sum;
+        for (uint32_t r = r0; r < r1; ++r) ends[r] += before;
+        __syncthreads();
+    }
+    const uint32_t total = ends[a.requests - 1], G = min(uint32_t(gridDim.x), total), w = blockIdx.x;
+    if (w >= G) return;
+    auto first_unit = [&](uint32_t i) { return uint32_t(uint64_t(total) * i / G); };
+    auto group_of = [&](uint32_t u) { return uint32_t(((uint64_t(u) + 1) * G - 1) / total); };
+    const uint32_t u0 = first_unit(w), u1 = first_unit(w + 1);
+
+    // ---- a unit's place: request, KV head, key block
+    struct Place {
+        int r, h, k, n;       // unit k of the item's n
+        int row0, cols, keys; // the item's first row, its columns, the keys that its last row sees
+        int seen;             // the keys that its first row sees
+    };
+    auto enter = [&](Place& p, int r) {
+        const Request q = request_of(a, uint32_t(r));
+        p.r = r, p.n = uniform(units_of(q)), p.row0 = uniform(q.row0), p.cols = uniform(q.rows * group);
+        p.seen = uniform(q.seen), p.keys = uniform(max(0, q.seen + q.rows - 1));
+    };
+    auto next = [&](Place& p) {
+        if (++p.k < p.n) return;
+        p.k = 0;
+        if (++p.h < kvh) return;
+        p.h = 0;
+        int r = p.r + 1;
+        while (r < int(a.requests) - 1 && uniform(int(ends[r])) == uniform(int(ends[r - 1]))) ++r;
+        if (r < int(a.requests)) enter(p, r);  // past the last request the place is not used
+    };
+    Place p0{};
+    {
+        const int r = uniform(first_above(ends, int(a.requests), u0));
+        enter(p0, r);
+        const uint32_t in = u0 - (r ? uint32_t(uniform(int(ends[r - 1]))) : 0u);
+        p0.h = int(in) / p0.n, p0.k = int(in) % p0.n;
+    }
+
+    const __amdgpu_buffer_rsrc_t k_rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(a.kc), 0, k_bytes, 0x00020000);
+    const __amdgpu_buffer_rsrc_t v_rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(a.vc), 0, v_bytes, 0x00020000);
+    // this wave's keys of a unit start at 128 k + 32 wv; this lane's K rows of both tiles lie in the eight from 8 (c16 / 4),
+    // its V reads take the eight from 8 g
+    const int k8 = 32 * wv + 8 * (c16 >> 2), v8 = 32 * wv + 8 * g;
+    auto page_ids = [&](const Place& p, uint32_t& idk, uint32_t& idv) {
+        const uint32_t* row = a.table + size_t(p.r) * a.blocks;
+        const uint32_t kb = uint32_t(p.k) * paged::kUnitKeys;
+        idk = row[min((kb + k8) >> a.page_log2, a.blocks - 1)];
+        idv = row[min((kb + v8) >> a.page_log2, a.blocks - 1)];
+    };
+    u32x4 kr[2][2 * KS], vr[2][DT];
+    bool page_in[2];  // this lane's eight keys have a page
+    auto fetch = [&](auto set, const Place& p, uint32_t idk, uint32_t idv) __attribute__((always_inline)) {
+        constexpr int S = decltype(set)::value;
+        const int kk = p.k * int(paged::kUnitKeys) + k8, kv = p.k * int(paged::kUnitKeys) + v8;
+        const bool ink = kk < p.keys && idk < a.pages, inv = kv < p.keys && idv < a.pages;
+        page_in[S] = idv < a.pages;
+        const uint32_t ko = ink ? ((((idk * uint32_t(kvh) + p.h) << a.page_log2) + (uint32_t(kk) & page_mask) + (c16 & 3)) * HD +
+                                   8 * g) * 2
+                                : kOut;
+        const uint32_t vo = inv ? ((((idv * uint32_t(kvh) + p.h) << a.page_log2) + (uint32_t(kv) & page_mask)) * HD + 8 * c16) * 2
+                                : kOut;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int s = 0; s < KS; ++s)
+                kr[S][i * KS + s] = __builtin_amdgcn_raw_buffer_load_b128(k_rsrc, ko + i * 8 * HD + s * 64, 0, 0);
+#pragma unroll
+        for (int d = 0; d < DT; ++d) vr[S][d] = __builtin_amdgcn_raw_buffer_load_b128(v_rsrc, vo + d * 256, 0, 0);
+    };
+    u32x4 qf[KS], qn[KS];
+    auto fetch_q = [&](const Place& p) __attribute__((always_inline)) {
+        const int row = p.row0 + c16 / group, head = p.h * group + c16 % group;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            qn[s] = u32x4{0u, 0u, 0u, 0u};
+            if (c16 < p.cols)
+                qn[s] = *reinterpret_cast<const u32x4*>(static_cast<const T*>(a.q) + (size_t(row) * a.qh + head) * HD + 32 * s +
+                                                        8 * g);
+        }
+    };
+
+    float m_run = -INFINITY, l_run = 0.f;  // the column's reference maximum, this lane's share of its sum
+    f32x4 o[DT];
+    auto clear = [&]() __attribute__((always_inline)) {
+        m_run = -INFINITY, l_run = 0.f;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    };
+    auto compute = [&](auto set, const Place& p) __attribute__((always_inline)) {
+        constexpr int S = decltype(set)::value;
+        const int kb = p.k * int(paged::kUnitKeys) + 32 * wv;  // this wave's first key
+        f32x4 s0 = {0.f, 0.f, 0.f, 0.f}, s1 = s0;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            s0 = M::m16(kr[S][s], qf[s], s0);
+            s1 = M::m16(kr[S][KS + s], qf[s], s1);
+        }
+        float sc[8];  // keys kb + 8 g ..
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sc[e] = s0[e], sc[4 + e] = s1[e];
+        if (kb + 32 > p.seen || __any(!page_in[S])) {  // uniform: some key is hidden from some column
+            const int lim = page_in[S] && c16 < p.cols ? p.seen + c16 / group - kb - 8 * g : 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sc[e] = e < lim ? sc[e] : -INFINITY;
+            if (kb + 32 > p.keys) {  // what lies past the last key may be anything, and zero times NaN is NaN
+                const int left = p.keys - kb - 8 * g;
+                u32x4 keep;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    keep[e] = (2 * e < left ? 0x0000FFFFu : 0u) | (2 * e + 1 < left ? 0xFFFF0000u : 0u);
+#pragma unroll
+                for (int d = 0; d < DT; ++d) vr[S][d] &= keep;
+            }
+        }
+        float mx = fmaxf(fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3])), fmaxf(fmaxf(sc[4], sc[5]), fmaxf(sc[6], sc[7])));
+        mx = cross_rows_max(mx);
+        // the reference moves only when it is left behind by more than 8 in the exponent: weights stay at most 2^8
+        const bool grow = (mx - m_run) * a.scale_log2 > 8.0f;  // false for NaN (both -inf)
+        if (__any(grow)) {
+            const float alpha = grow ? __builtin_amdgcn_exp2f((m_run - mx) * a.scale_log2) : 1.0f;
+            m_run = grow ? mx : m_run;
+            l_run *= alpha;
+#pragma unroll
+            for (int d = 0; d < DT; ++d) o[d] *= alpha;
+        }
+        const float mc = m_run == -INFINITY ? 0.f : m_run * a.scale_log2;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            sc[e] = __builtin_amdgcn_exp2f(fmaf(sc[e], a.scale_log2, -mc));
+            l_run += sc[e];
+        }
+        // the weights go into the product rounded to the cache's type, as its values are; their sum stays float32
+        const u32x4 pb = {M::pack(sc[0], sc[1]), M::pack(sc[2], sc[3]), M::pack(sc[4], sc[5]), M::pack(sc[6], sc[7])};
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[d] = M::m16(vr[S][d], pb, o[d]);
+    };
+
+    // ---- the end of an item here: the waves' parts meet in LDS, then y, or a partial and the join
+    float* const slots = reinterpret_cast<float*>(a.ws + (uint64_t(a.requests) * a.kvh + 63) / 64 * 64);
+    constexpr int SW = int(2 * paged::kCols + paged::kCols * HD);
+    auto finish = [&](const Place& p, uint32_t u) {
+        const float l = cross_rows_sum(l_run);
+        if (g == 0) xm[wv][c16] = m_run, xl[wv][c16] = l;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(xo + (wv * 16 + c16) * XR + 16 * d + 4 * g) = o[d];
+        lds_barrier();
+        // thread t: four dims of column t / (HD / 4) + i 1024 / HD
+        const uint32_t begin = u - uint32_t(p.k), end = begin + uint32_t(p.n);
+        const bool whole = begin >= u0 && end <= u1;
+        const uint32_t wa = group_of(begin), wb = group_of(end - 1);
+        float* mine = slots + size_t(2 * w + (begin >= u0 ? 1 : 0)) * SW;
+        constexpr int Q4 = HD / 4;
+        for (int e = t; e < p.cols * Q4; e += 256) {
+            const int c = e / Q4, d = 4 * (e % Q4);
+            float m = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) m = fmaxf(m, xm[i][c]);
+            const float mc = m == -INFINITY ? 0.f : m * a.scale_log2;
+            float sum = 0.f;
+            f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float f = __builtin_amdgcn_exp2f(xm[i][c] * a.scale_log2 - mc);
+                sum = fmaf(xl[i][c], f, sum);
+                v += *reinterpret_cast<const f32x4*>(xo + (i * 16 + c) * XR + d) * f;
+            }
+            if (whole) {
+                const float inv = sum != 0.f ? 1.0f / sum : 0.f;  // no key at all: zeros
+                const int row = p.row0 + c / group, head = p.h * group + c % group;
+                T* y = static_cast<T*>(a.y) + (size_t(row) * a.qh + head) * HD + d;
+                *reinterpret_cast<uint2*>(y) = make_uint2(M::pack(v[0] * inv, v[1] * inv), M::pack(v[2] * inv, v[3] * inv));
+            } else {
+                store_agent(mine + 2 * paged::kCols + c * HD + d, v[0], v[1]);
+                store_agent(mine + 2 * paged::kCols + c * HD + d + 2, v[2], v[3]);
+                if (d == 0) store_agent(mine + 2 * c, m, sum);
+            }
+        }
+        if (!whole) {
+            __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0): this wave's stores are performed
+            lds_barrier();
+            uint32_t* counter = a.ws + size_t(p.r) * a.kvh + p.h;
+            if (t == 0) arrived = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            lds_barrier();
+            if (arrived == wb - wa) {  // the last one in joins the parts, in their order
+                for (int e = t; e < p.cols * Q4; e += 256) {
+                    const int c = e / Q4, d = 4 * (e % Q4);
+                    float m = -INFINITY, sum = 0.f;
+                    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+                    for (uint32_t i = wa; i <= wb; ++i) {
+                        const float* part = slots + size_t(2 * i + (i == wa ? 1 : 0)) * SW;
+                        const float2 ml = load_agent(part + 2 * c);
+                        const float2 x = load_agent(part + 2 * paged::kCols + c * HD + d);
+                        const float2 z = load_agent(part + 2 * paged::kCols + c * HD + d + 2);
+                        const float mn = fmaxf(m, ml.x), mc = mn == -INFINITY ? 0.f : mn * a.scale_log2;
+                        const float fo = __builtin_amdgcn_exp2f(m * a.scale_log2 - mc);
+                        const float fn = __builtin_amdgcn_exp2f(ml.x * a.scale_log2 - mc);
+                        sum = sum * fo + ml.y * fn;
+                        v = v * fo + f32x4{x.x, x.y, z.x, z.y} * fn;
+                        m = mn;
+                    }
+                    const float inv = sum != 0.f ? 1.0f / sum : 0.f;
+                    const int row = p.row0 + c / group, head = p.h * group + c % group;
+                    T* y = static_cast<T*>(a.y) + (size_t(row) * a.qh + head) * HD + d;
+                    *reinterpret_cast<uint2*>(y) =
+                        make_uint2(M::pack(v[0] * inv, v[1] * inv), M::pack(v[2] * inv, v[3] * inv));
+                }
+                if (t == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+        }
+        lds_barrier();  // the exchange is free again
+        clear();
+    };
+
+    // ---- the units: page ids two ahead, keys and values one ahead of the products
+    using A0 = std::integral_constant<int, 0>;
+    using A1 = std::integral_constant<int, 1>;
+    Place p1 = p0, p2 = p0;
+    uint32_t idk = 0, idv = 0, idk1 = 0, idv1 = 0;
+    page_ids(p0, idk, idv);
+    fetch_q(p0);
+    next(p1);
+    p2 = p1;
+    if (u0 + 1 < u1) page_ids(p1, idk1, idv1);
+    fetch(A0{}, p0, idk, idv);
+#pragma unroll
+    for (int s = 0; s < KS; ++s) qf[s] = qn[s];
+    clear();
+    auto step = [&](auto set, uint32_t u) __attribute__((always_inline)) {
+        constexpr int S = decltype(set)::value;
+        using N = std::integral_constant<int, 1 - S>;
+        // p0 is unit u, p1 unit u + 1 with its ids in idk1, idv1
+        const bool more = u + 1 < u1, item = more && p1.k == 0;
+        idk = idk1, idv = idv1;
+        if (u + 2 < u1) {
+            next(p2);
+            page_ids(p2, idk1, idv1);
+        }
+        if (more) {
+            if (item) fetch_q(p1);
+            fetch(N{}, p1, idk, idv);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        compute(set, p0);
+        if (!more || item) finish(p0, u);
+        if (item) {
+#pragma unroll
+            for (int s = 0; s < KS; ++s) qf[s] = qn[s];
+        }
+        p0 = p1, p1 = p2;
+    };
+    for (uint32_t u = u0; u < u1; u += 2) {
+        step(A0{}, u);
+        if (u + 1 >= u1) break;
+        step(A1{}, u + 1);
+    }
+}
+
+// Rows of many query columns.
 // One wave per (row, query head): a key per lane for the scores, a dim (or two) per lane for the products.
 template <typename T, int HD>
 __global__ __launch_bounds__(64) void k_paged_attn(const T* q, const T* kc, const T* vc, const uint32_t* table,
@@ -333,12 +684,24 @@ static void l_append(const PreparedDispatch& pd, void* const* p, hipStream_t s) 
 
 // q, k_cache, v_cache, table, starts, context, y, workspace, requests, tokens, max_fresh, q_heads, kv_heads, head_dim,
 // blocks, page, pages, scale
+// the most new rows of a request in the dispatch, and whether every item's columns fit the kernel for few
+static uint32_t most_fresh(const uint32_t* w) { return w[11] ? std::min(w[11], w[10]) : w[10]; }
+static bool few_columns(const uint32_t* w) {
+    return w[13] && uint64_t(most_fresh(w)) * (w[12] / w[13]) <= paged::kCols;
+}
 template <typename T, int HD>
 static void launch_attn(const uint32_t* w, void* const* p, hipStream_t s) {
+    const float scale_log2 = f32_of(w[18]) * 1.4426950408889634f;
+    if (few_columns(w)) {
+        const AttnArgs a{p[0], p[1], p[2], (const uint32_t*)p[3], (const uint32_t*)p[4], (const uint32_t*)p[5], p[6],
+                         (uint32_t*)p[7], w[9], w[10], most_fresh(w), w[12], w[13], w[15], log2_of(w[16]), w[17], scale_log2};
+        const uint32_t bytes = uint32_t(uint64_t(w[17]) * w[16] * w[13] * HD * 2);
+        hipLaunchKernelGGL((k_attn_rows<T, HD>), dim3(paged::kGroups), dim3(256), 0, s, a, bytes, bytes);
+        return;
+    }
     hipLaunchKernelGGL((k_paged_attn<T, HD>), dim3(w[10], w[12]), dim3(64), 0, s, (const T*)p[0], (const T*)p[1],
                        (const T*)p[2], (const uint32_t*)p[3], (const uint32_t*)p[4], (const uint32_t*)p[5], (T*)p[6], w[9],
-                       w[10], w[11] ? w[11] : w[10], w[12], w[13], w[15], log2_of(w[16]), w[17],
-                       f32_of(w[18]) * 1.4426950408889634f);
+                       w[10], most_fresh(w), w[12], w[13], w[15], log2_of(w[16]), w[17], scale_log2);
 }
 static void l_attn(const PreparedDispatch& pd, void* const* p, hipStream_t s) {
     const uint32_t* w = pd.words.data();
@@ -391,8 +754,8 @@ static void need_pages(const char* n, uint32_t page, uint32_t pages) {
         contract_fail("%s: pages must be at least 1, and pages * page at most 2^32 - 1", n);
 }
 static void need_table(const char* n, uint32_t blocks, uint32_t page) {
-    if (blocks < 1 || times(blocks, page) > 0xFFFFFFFFull)
-        contract_fail("%s: blocks must be at least 1, and blocks * page at most 2^32 - 1", n);
+    if (blocks < 1 || times(blocks, page) > 1ull << 30)
+        contract_fail("%s: blocks must be at least 1, and blocks * page at most 2^30", n);
 }
 static void need_heads(const char* n, uint32_t qh, uint32_t kvh, uint32_t hd) {
     if (kvh < 1 || qh < 1 || qh % kvh) contract_fail("%s: kv_heads must divide q_heads", n);
@@ -468,7 +831,10 @@ std::vector<KernelSpec> paged_catalog() {
                      if (t[0].row.dtype() != F32) same_dtype("qk_norm_rope_append_paged", t, {0, 8});
                  }});
     // 49 attention_paged
-    c.push_back({"attention_paged", "paged", {64, 1, 1}, false, [](const uint32_t* w) { return Grid3{w[10], w[12], 1}; },
+    c.push_back({"attention_paged", "paged", {256, 1, 1}, false,
+                 [](const uint32_t* w) {
+                     return few_columns(w) ? Grid3{int64_t(paged::kGroups), 1, 1} : Grid3{w[10], w[12], 1};
+                 },
                  {TOK_R("q", H), TOK_R("k_cache", H), TOK_R("v_cache", H), TOK_R("table", U), TOK_R("starts", U),
                   TOK_R("context", U), TOK_W("y", H), TOK_RW("workspace", U), U32F("requests"), U32F("tokens"),
                   U32F("max_fresh"), U32F("q_heads"), U32F("kv_heads"), U32F("head_dim"), U32F("blocks"), U32F("page"),
@@ -483,6 +849,8 @@ std::vector<KernelSpec> paged_catalog() {
                      need_table(n, blocks, page);
                      const float scale = f32_of(w[18]);
                      if (!(scale > 0.f) || std::isinf(scale)) contract_fail("%s: scale must be positive and finite", n);
+                     if (times(R, kvh, uint64_t(blocks) * page / paged::kUnitKeys + 1) > 1ull << 31)
+                         contract_fail("%s: requests * kv_heads * blocks * page is more than one dispatch shares out", n);
                      need(c, 0, times(T, qh, hd), n, "q");
                      need(c, 1, times(uint64_t(pages) * page, kvh, hd), n, "k_cache");
                      need(c, 2, times(uint64_t(pages) * page, kvh, hd), n, "v_cache");
