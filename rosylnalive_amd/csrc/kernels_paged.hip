@@ -238,6 +238,11 @@ __device__ __forceinline__ Request request_of(const AttnArgs& a, uint32_t r) {
     return Request{int(s0), min(fresh, int(a.max_fresh)), ctx - fresh + 1};
 }
 
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+// words that no launch writes while it reads them, at uniform addresses: scalar loads
+typedef const __attribute__((address_space(4))) uint32_t* const_words;
+
 template <typename T>
 struct Mfma;
 template <>
@@ -246,6 +251,9 @@ struct Mfma<_Float16> {
     static __device__ __forceinline__ f32x4 m16(u32x4 a, u32x4 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(vec, a), __builtin_bit_cast(vec, b), c, 0, 0, 0);
     }
+    static __device__ __forceinline__ f32x16 m32(u32x4 a, u32x4 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(vec, a), __builtin_bit_cast(vec, b), c, 0, 0, 0);
+    }
     static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack2h(a, b); }
 };
 template <>
@@ -253,6 +261,9 @@ struct Mfma<__bf16> {
     typedef bf16x8 vec;
     static __device__ __forceinline__ f32x4 m16(u32x4 a, u32x4 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(vec, a), __builtin_bit_cast(vec, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ f32x16 m32(u32x4 a, u32x4 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(vec, a), __builtin_bit_cast(vec, b), c, 0, 0, 0);
     }
     // two floats to a bf16 pair, round to nearest even (one v_cvt_pk_bf16_f32)
     static __device__ __forceinline__ uint32_t pack(float a, float b) {
@@ -299,7 +310,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(AttnArgs a, uint32_t k_byt
     // ---- the units of every request, and this workgroup's
     auto units_of = [&](const Request& q) {  // of one item of the request
         if (q.rows < 1) return 0;
-        return max(1, (q.seen + q.rows - 1 + int(paged::kUnitKeys) - 1) / int(paged::kUnitKeys));
+        return max(1, (q.seen + q.rows - 1 + int(paged::kRowsKeys) - 1) / int(paged::kRowsKeys));
     };
     {
         const uint32_t per = (a.requests + 255) / 256, r0 = min(t * per, a.requests), r1 = min(r0 + per, a.requests);
@@ -353,7 +364,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(AttnArgs a, uint32_t k_byt
     const int k8 = 32 * wv + 8 * (c16 >> 2), v8 = 32 * wv + 8 * g;
     auto page_ids = [&](const Place& p, uint32_t& idk, uint32_t& idv) {
         const uint32_t* row = a.table + size_t(p.r) * a.blocks;
-        const uint32_t kb = uint32_t(p.k) * paged::kUnitKeys;
+        const uint32_t kb = uint32_t(p.k) * paged::kRowsKeys;
         idk = row[min((kb + k8) >> a.page_log2, a.blocks - 1)];
         idv = row[min((kb + v8) >> a.page_log2, a.blocks - 1)];
     };
@@ -361,7 +372,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(AttnArgs a, uint32_t k_byt
     bool page_in[2];  // this lane's eight keys have a page
     auto fetch = [&](auto set, const Place& p, uint32_t idk, uint32_t idv) __attribute__((always_inline)) {
         constexpr int S = decltype(set)::value;
-        const int kk = p.k * int(paged::kUnitKeys) + k8, kv = p.k * int(paged::kUnitKeys) + v8;
+        const int kk = p.k * int(paged::kRowsKeys) + k8, kv = p.k * int(paged::kRowsKeys) + v8;
         const bool ink = kk < p.keys && idk < a.pages, inv = kv < p.keys && idv < a.pages;
         page_in[S] = idv < a.pages;
         const uint32_t ko = ink ? ((((idk * uint32_t(kvh) + p.h) << a.page_log2) + (uint32_t(kk) & page_mask) + (c16 & 3)) * HD +
@@ -398,7 +409,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(AttnArgs a, uint32_t k_byt
     };
     auto compute = [&](auto set, const Place& p) __attribute__((always_inline)) {
         constexpr int S = decltype(set)::value;
-        const int kb = p.k * int(paged::kUnitKeys) + 32 * wv;  // this wave's first key
+        const int kb = p.k * int(paged::kRowsKeys) + 32 * wv;  // this wave's first key
         f32x4 s0 = {0.f, 0.f, 0.f, 0.f}, s1 = s0;
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
@@ -446,8 +457,8 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(AttnArgs a, uint32_t k_byt
     };
 
     // ---- the end of an item here: the waves' parts meet in LDS, then y, or a partial and the join
-    float* const slots = reinterpret_cast<float*>(a.ws + (uint64_t(a.requests) * a.kvh + 63) / 64 * 64);
-    constexpr int SW = int(2 * paged::kCols + paged::kCols * HD);
+    float* const slots = reinterpret_cast<float*>(a.ws + paged::kGroups);
+    constexpr int SW = int(paged::slot_words(paged::kRowsCols, HD));
     auto finish = [&](const Place& p, uint32_t u) {
         const float l = cross_rows_sum(l_run);
         if (g == 0) xm[wv][c16] = m_run, xl[wv][c16] = l;
@@ -480,15 +491,15 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(AttnArgs a, uint32_t k_byt
                 T* y = static_cast<T*>(a.y) + (size_t(row) * a.qh + head) * HD + d;
                 *reinterpret_cast<uint2*>(y) = make_uint2(M::pack(v[0] * inv, v[1] * inv), M::pack(v[2] * inv, v[3] * inv));
             } else {
-                store_agent(mine + 2 * paged::kCols + c * HD + d, v[0], v[1]);
-                store_agent(mine + 2 * paged::kCols + c * HD + d + 2, v[2], v[3]);
+                store_agent(mine + 2 * paged::kRowsCols + c * HD + d, v[0], v[1]);
+                store_agent(mine + 2 * paged::kRowsCols + c * HD + d + 2, v[2], v[3]);
                 if (d == 0) store_agent(mine + 2 * c, m, sum);
             }
         }
         if (!whole) {
             __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0): this wave's stores are performed
             lds_barrier();
-            uint32_t* counter = a.ws + size_t(p.r) * a.kvh + p.h;
+            uint32_t* counter = a.ws + wa;
             if (t == 0) arrived = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             lds_barrier();
             if (arrived == wb - wa) {  // the last one in joins the parts, in their order
@@ -499,8 +510,8 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(AttnArgs a, uint32_t k_byt
                     for (uint32_t i = wa; i <= wb; ++i) {
                         const float* part = slots + size_t(2 * i + (i == wa ? 1 : 0)) * SW;
                         const float2 ml = load_agent(part + 2 * c);
-                        const float2 x = load_agent(part + 2 * paged::kCols + c * HD + d);
-                        const float2 z = load_agent(part + 2 * paged::kCols + c * HD + d + 2);
+                        const float2 x = load_agent(part + 2 * paged::kRowsCols + c * HD + d);
+                        const float2 z = load_agent(part + 2 * paged::kRowsCols + c * HD + d + 2);
                         const float mn = fmaxf(m, ml.x), mc = mn == -INFINITY ? 0.f : mn * a.scale_log2;
                         const float fo = __builtin_amdgcn_exp2f(m * a.scale_log2 - mc);
                         const float fn = __builtin_amdgcn_exp2f(ml.x * a.scale_log2 - mc);
@@ -565,63 +576,461 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(AttnArgs a, uint32_t k_byt
     }
 }
 
-// Rows of many query columns.
-// One wave per (row, query head): a key per lane for the scores, a dim (or two) per lane for the products.
+// sum over i < n of floor((b + i step) / 64) (Euclid's way down the two slopes), for sums below 2^31
+__device__ __forceinline__ uint32_t floor_sum64(uint32_t n, uint32_t step, uint32_t b) {
+    uint32_t m = 64, sum = 0;
+    while (n) {
+        sum += uint32_t(uint64_t(n) * (n - 1) / 2) * (step / m) + n * (b / m);
+        step %= m, b %= m;
+        const uint32_t y = step * n + b;
+        n = y / m, b = y % m;
+        const uint32_t s = step;
+        step = m, m = s;
+        if (!m) break;
+    }
+    return sum;
+}
+
+// Rows of many query columns, on 32 x 32 x 16 tiles. A tile of an item is up to 256 columns (whole rows of the request: 256 /
+// group of them), 64 per wave as two column tiles, so that each K and V operand read from LDS feeds two matrix
+// instructions (one instruction per read would take all of LDS's bandwidth). K and V blocks of 64 keys go from the pages
+// through registers into LDS (three K blocks, two V blocks), loaded a step before they are stored; one barrier per block. K rows hold their 16-byte
+// chunks in an order that depends on the row, so the 16 rows that a read phase takes lie in different banks; V's layout in
+// the cache is already the order in which it is read.
+// Step n: the scores of block n + 1 (matrix core) under the exponentials of block n (VALU), then block n's products
+// under the maxima of block n + 1. The rows of S^T's tiles hold the keys in the order in which P^T wants them (bits 2 and 3
+// of the row exchanged), so weights never cross lanes.
 template <typename T, int HD>
-__global__ __launch_bounds__(64) void k_paged_attn(const T* q, const T* kc, const T* vc, const uint32_t* table,
-                                                   const uint32_t* starts, const uint32_t* context, T* y, uint32_t requests,
-                                                   uint32_t tokens, uint32_t max_fresh, uint32_t qh, uint32_t kvh,
-                                                   uint32_t blocks, uint32_t page_log2, uint32_t pages, float scale_log2) {
-    __shared__ float qs[HD];
-    __shared__ float ps[64];
-    const uint32_t row = blockIdx.x, head = blockIdx.y, lane = threadIdx.x, page = 1u << page_log2;
-    if (row >= min(starts[requests], tokens)) return;
-    uint32_t lo = 0, hi = requests - 1;
-    while (lo < hi) {  // the first request that ends behind the row
-        const uint32_t m = (lo + hi) >> 1;
-        if (starts[m + 1] > row)
-            hi = m;
-        else
-            lo = m + 1;
-    }
-    const uint32_t first = starts[lo];
-    if (first > row || row - first >= max_fresh) return;
-    const int64_t fresh = int64_t(min(starts[lo + 1], tokens)) - first;
-    const int64_t keys = int64_t(min(context[lo], blocks * page)) - fresh + (row - first) + 1;
-    const T* qr = q + (size_t(row) * qh + head) * HD;
-    for (int d = lane; d < HD; d += 64) qs[d] = widen(qr[d]);
-    __syncthreads();
-    const uint32_t kvhead = head / (qh / kvh);
-    float m_run = -INFINITY, l_run = 0.f, o[HD / 64];
-    for (int i = 0; i < HD / 64; ++i) o[i] = 0.f;
-    for (int64_t k0 = 0; k0 < keys; k0 += 64) {
-        const uint32_t key = uint32_t(k0) + lane;
-        const uint32_t id = key < keys ? table[size_t(lo) * blocks + (key >> page_log2)] : paged::kNone;
-        float s = -INFINITY;
-        if (id < pages) {
-            const T* k = kc + (((size_t(id) * kvh + kvhead) << page_log2) + (key & (page - 1))) * HD;
-            s = 0.f;
-            for (int d = 0; d < HD; ++d) s = fmaf(qs[d], widen(k[d]), s);
-            s *= scale_log2;
+__global__ __launch_bounds__(256, 1) void k_attn_tiles(AttnArgs a, uint32_t bytes) {
+    using M = Mfma<T>;
+    constexpr int KB = int(paged::kTileKeys), KS = HD / 16, DT = HD / 32, RB = HD * 2, BLK = KB * RB;
+    constexpr int CH = RB / 16;            // 16-byte chunks of a K row
+    constexpr int LPB = BLK / 4096;        // loads of a block per wave and of 1 KB each: 16 keys
+    __shared__ __attribute__((aligned(16))) uint8_t lds[5 * BLK];  // K blocks n % 3, then V blocks n % 2
+    __shared__ uint32_t ends[paged::kMaxRequests];
+    __shared__ uint32_t red[4];
+    __shared__ uint32_t arrived;
+    const int t = threadIdx.x, lane = t & 63, wv = uniform(t >> 6), c32 = lane & 31, h = lane >> 5;
+    const int group = int(a.qh / a.kvh), kvh = int(a.kvh), TR = int(paged::kTileCols) / group;
+
+    // ---- the units of every request, and this workgroup's
+    // blocks of 64 keys of a request's first n tiles on one KV head: tile i's last row sees seen + min((i + 1) TR, rows) - 1
+    // keys, at least one block. All full tiles but the clamped ones follow a slope.
+    auto tile_keys = [&](const Request& q, int i) { return max(0, q.seen + min((i + 1) * TR, q.rows) - 1); };
+    auto tile_units = [&](const Request& q, int i) { return max(1, (tile_keys(q, i) + KB - 1) / KB); };
+    auto first_units = [&](const Request& q, int n) {
+        const int full = min(n, q.rows / TR);
+        // tiles of one block: seen + (i + 1) TR - 1 <= 64
+        const int ones = min(full, max(0, (KB + 1 - q.seen) / TR));
+        uint32_t sum = uint32_t(ones);
+        if (full > ones) sum += floor_sum64(uint32_t(full - ones), uint32_t(TR), uint32_t(q.seen + (ones + 1) * TR - 1 + KB - 1));
+        if (n > full) sum += uint32_t(tile_units(q, full));
+        return sum;
+    };
+    auto tiles_of = [&](const Request& q) { return (q.rows + TR - 1) / TR; };
+    {
+        const uint32_t per = (a.requests + 255) / 256, r0 = min(t * per, a.requests), r1 = min(r0 + per, a.requests);
+        uint32_t sum = 0;
+        for (uint32_t r = r0; r < r1; ++r) {
+            const Request q = request_of(a, r);
+            if (q.rows > 0) sum += first_units(q, tiles_of(q)) * uint32_t(kvh);
+            ends[r] = sum;
         }
-        const float m = fmaxf(m_run, wave_max(s));
-        const float base = m == -INFINITY ? 0.f : m;
-        const float p = exp2f(s - base), alpha = exp2f(m_run - base);
-        l_run = l_run * alpha + wave_sum(p);
-        m_run = m;
-        ps[lane] = p;
-        __syncthreads();
-        for (int i = 0; i < HD / 64; ++i) o[i] *= alpha;
-        for (uint32_t j = 0; j < 64 && k0 + j < keys; ++j) {
-            const uint32_t kj = uint32_t(k0) + j, ij = table[size_t(lo) * blocks + (kj >> page_log2)], off = kj & (page - 1);
-            if (ij >= pages) continue;
-            const T* v = vc + ((size_t(ij) * kvh + kvhead) << page_log2) * HD + size_t(off >> 3) * (8 * HD) + (off & 7);
-            for (int i = 0; i < HD / 64; ++i) o[i] = fmaf(ps[j], widen(v[(lane + 64 * i) * 8]), o[i]);
-        }
+        const uint32_t before = scan_sat(sum, red) - sum;
+        for (uint32_t r = r0; r < r1; ++r) ends[r] += before;
         __syncthreads();
     }
-    for (int i = 0; i < HD / 64; ++i)
-        y[(size_t(row) * qh + head) * HD + lane + 64 * i] = narrow<T>(l_run > 0.f ? o[i] / l_run : o[i]);
+    const uint32_t total = ends[a.requests - 1], G = min(uint32_t(gridDim.x), total);
+    // workgroups of one XCD (every eighth) take neighbouring units, which share a KV head's blocks in its L2
+    const uint32_t w = G == paged::kTileGroups ? (blockIdx.x % 8) * (paged::kTileGroups / 8) + blockIdx.x / 8 : blockIdx.x;
+    if (w >= G) return;
+    auto first_unit = [&](uint32_t i) { return uint32_t(uint64_t(total) * i / G); };
+    auto group_of = [&](uint32_t u) { return uint32_t(((uint64_t(u) + 1) * G - 1) / total); };
+    const uint32_t u0 = first_unit(w), u1 = first_unit(w + 1);
+
+    const __amdgpu_buffer_rsrc_t k_rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(a.kc), 0, bytes, 0x00020000);
+    const __amdgpu_buffer_rsrc_t v_rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(a.vc), 0, bytes, 0x00020000);
+    // this wave moves keys 16 wv .. + 15 of a block, 16 bytes per lane and load: both caches hold them in one piece
+    int kst[LPB];  // where a K chunk goes in its block
+#pragma unroll
+    for (int i = 0; i < LPB; ++i) {
+        const int p = 64 * i + lane, row = p / CH, ch = p % CH;  // row of the wave's 16, place in the row
+        kst[i] = (16 * wv + row) * RB + (ch ^ (HD == 128 ? row & 15 : (row >> 1) & 7)) * 16;
+    }
+    // operand reads: K row of matrix row c32 is key 16 (c32 / 16) + 8 (c32 / 4 % 2) + 4 (c32 / 8 % 2) + c32 % 4
+    const int krow = (c32 & 19) | ((c32 & 4) << 1) | ((c32 & 8) >> 1);
+    const int kswz = (h ^ (HD == 128 ? krow & 15 : (krow >> 1) & 7)) * 16;
+    const int kbase = krow * RB + kswz, vbase = 3 * BLK + h * (8 * RB) + c32 * 16;
+
+    Request rq{};
+    int r = uniform(first_above(ends, int(a.requests), u0));
+    int hk = 0, tile = 0, kfirst = 0;
+    {
+        rq = request_of(a, uint32_t(r));
+        rq.row0 = uniform(rq.row0), rq.rows = uniform(rq.rows), rq.seen = uniform(rq.seen);
+        uint32_t in = u0 - (r ? uint32_t(uniform(int(ends[r - 1]))) : 0u);
+        const int tiles = tiles_of(rq);
+        const uint32_t per_head = uint32_t(uniform(int(first_units(rq, tiles))));
+        hk = int(in / per_head), in %= per_head;
+        int lo = 0, hi = tiles - 1;  // the last tile whose first unit is at or before `in`
+        while (lo < hi) {
+            const int m = (lo + hi + 1) >> 1;
+            if (first_units(rq, m) <= in)
+                lo = m;
+            else
+                hi = m - 1;
+        }
+        tile = uniform(lo), kfirst = uniform(int(in - first_units(rq, lo)));
+    }
+    float* const slots = reinterpret_cast<float*>(a.ws + paged::kGroups);
+    constexpr int SW = int(paged::slot_words(paged::kTileCols, HD));
+
+    for (uint32_t u = u0; u < u1;) {
+        // ---- a piece: blocks j0 .. j0 + nb - 1 of a tile
+        const int units = tile_units(rq, tile), keys = tile_keys(rq, tile), j0 = kfirst;
+        const int nb = min(units - j0, int(u1 - u));
+        const int row_first = tile * TR, cols = min(TR, rq.rows - row_first) * group;
+        const int cw = 64 * wv;  // this wave's first column
+        // blocks that some column of the wave sees
+        int nbw = 0;
+        if (cw < cols) nbw = (max(0, rq.seen + row_first + min(cw + 63, cols - 1) / group) + KB - 1) / KB - j0;
+        nbw = uniform(min(max(nbw, 0), nb));
+        const int wave_seen = uniform(rq.seen + row_first + cw / group);  // keys that the wave's first column sees
+        int vis[2];  // keys that this lane's columns see
+        u32x4 qf[2][KS];
+#pragma unroll
+        for (int ct = 0; ct < 2; ++ct) {
+            const int c = cw + 32 * ct + c32, row = row_first + c / group, head = hk * group + c % group;
+            vis[ct] = rq.seen + row;
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                qf[ct][s] = u32x4{0u, 0u, 0u, 0u};
+                if (c < cols)
+                    qf[ct][s] = *reinterpret_cast<const u32x4*>(
+                        static_cast<const T*>(a.q) + (size_t(rq.row0 + row) * a.qh + head) * HD + 16 * s + 8 * h);
+            }
+        }
+        const const_words trow = const_words(a.table) + size_t(r) * a.blocks;
+        // the pages of block j's four 16-key parts (scalar loads, a step before their use); then its place in the caches for
+        // this wave's 16 keys, and the set of the parts that have none
+        uint32_t ids[4];
+        auto page_ids = [&](int j) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                ids[i] = trow[min(uint32_t((j0 + j) * KB + 16 * i) >> a.page_log2, a.blocks - 1)];
+        };
+        auto locate = [&](int j, int& soff, uint32_t& bad) __attribute__((always_inline)) {
+            bad = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) bad |= uint32_t(ids[i] >= a.pages) << i;
+            const uint32_t mine = wv == 0 ? ids[0] : wv == 1 ? ids[1] : wv == 2 ? ids[2] : ids[3];
+            const uint32_t off = uint32_t((j0 + j) * KB + 16 * wv) & ((1u << a.page_log2) - 1);
+            soff = mine < a.pages ? int((((mine * uint32_t(kvh) + hk) << a.page_log2) + off) * RB) : 0;
+        };
+        u32x4 rk[LPB], rv[LPB];
+        auto load_k = [&](int soff) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < LPB; ++i) rk[i] = __builtin_amdgcn_raw_buffer_load_b128(k_rsrc, 16 * lane + 1024 * i, soff, 0);
+        };
+        auto load_v = [&](int soff) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < LPB; ++i) rv[i] = __builtin_amdgcn_raw_buffer_load_b128(v_rsrc, 16 * lane + 1024 * i, soff, 0);
+        };
+        auto store_k = [&](int slot) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < LPB; ++i) *reinterpret_cast<u32x4*>(lds + slot * BLK + kst[i]) = rk[i];
+        };
+        auto store_v = [&](int slot, int j, uint32_t bad) __attribute__((always_inline)) {
+            const int left = keys - (j0 + j) * KB;  // keys of the block that any column sees
+            if (left < KB || bad) {  // uniform: what is hidden may be anything, and zero times NaN is NaN
+#pragma unroll
+                for (int i = 0; i < LPB; ++i) {
+                    const int in = (bad >> wv & 1u) ? 0 : left - 16 * wv - 8 * ((64 * i + lane) / HD);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        rv[i][e] &= (2 * e < in ? 0x0000FFFFu : 0u) | (2 * e + 1 < in ? 0xFFFF0000u : 0u);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < LPB; ++i)
+                *reinterpret_cast<u32x4*>(lds + (3 + slot) * BLK + 1024 * (LPB * wv + i) + 16 * lane) = rv[i];
+        };
+        f32x16 sa[2], sb[2], o[2][DT];  // scores of a block's first and last 32 keys, [column tile]; [column tile][dim tile]
+        float m_run[2], l_run[2];
+#pragma unroll
+        for (int ct = 0; ct < 2; ++ct) {
+            m_run[ct] = -INFINITY, l_run[ct] = 0.f;
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[ct][d][e] = 0.f;
+        }
+        auto scores = [&](int slot, int kt, f32x16(&out)[2]) __attribute__((always_inline)) {
+            const uint8_t* k0 = lds + slot * BLK + kt * 32 * RB;
+#pragma unroll
+            for (int ct = 0; ct < 2; ++ct)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) out[ct][e] = 0.f;
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                const u32x4 k = *reinterpret_cast<const u32x4*>(k0 + (kbase ^ (32 * s)));
+                out[0] = M::m32(k, qf[0][s], out[0]);
+                out[1] = M::m32(k, qf[1][s], out[1]);
+            }
+        };
+        auto maxima = [&](f32x16(&s)[2], float(&mx)[2]) __attribute__((always_inline)) {
+#pragma unroll
+            for (int ct = 0; ct < 2; ++ct) {
+                float m = s[ct][0];
+#pragma unroll
+                for (int e = 1; e < 16; ++e) m = fmaxf(m, s[ct][e]);
+                const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
+                mx[ct] = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+            }
+        };
+        // hides what the columns do not see of the 32 keys, and moves the reference maxima where they are left behind
+        auto settle = [&](int j, int kt, uint32_t bad, f32x16(&s)[2], float(&mx)[2]) __attribute__((always_inline)) {
+            const int kb = (j0 + j) * KB + 32 * kt;
+            if (kb + 32 > wave_seen || bad) {  // uniform
+#pragma unroll
+                for (int ct = 0; ct < 2; ++ct) {
+                    const int lim = vis[ct] - kb - 8 * h;
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        if (16 * (e >> 3) + (e & 7) >= lim || (bad >> (2 * kt + (e >> 3)) & 1u)) s[ct][e] = -INFINITY;
+                }
+                maxima(s, mx);
+            }
+            bool grow[2];
+#pragma unroll
+            for (int ct = 0; ct < 2; ++ct) grow[ct] = (mx[ct] - m_run[ct]) * a.scale_log2 > 8.0f;  // false for NaN (both -inf)
+            if (__any(grow[0] || grow[1])) {
+#pragma unroll
+                for (int ct = 0; ct < 2; ++ct) {
+                    const float alpha = grow[ct] ? __builtin_amdgcn_exp2f((m_run[ct] - mx[ct]) * a.scale_log2) : 1.0f;
+                    m_run[ct] = grow[ct] ? mx[ct] : m_run[ct];
+                    l_run[ct] *= alpha;
+#pragma unroll
+                    for (int d = 0; d < DT; ++d) o[ct][d] *= alpha;
+                }
+            }
+        };
+        // 32 keys: the scores of the next 32 (matrix core) under the weights of these (VALU), then their products under the
+        // next ones' maxima, two matrix instructions and their share of the VALU's work at a time: the scheduling barriers
+        // keep that order (without them all the instructions of one kind follow each other, and either unit waits for the
+        // other), with each operand read two pairs ahead.
+        auto half = [&](int kslot, int nkt, f32x16(&nxt)[2], int vslot, int kt, f32x16(&cur)[2],
+                        float(&mx)[2]) __attribute__((always_inline)) {
+            const uint8_t* k0 = lds + kslot * BLK + nkt * 32 * RB;
+            const uint8_t* v0 = lds + vslot * BLK + vbase + kt * 32 * RB;
+            auto read_k = [&](int s) __attribute__((always_inline)) {
+                return *reinterpret_cast<const u32x4*>(k0 + (kbase ^ (32 * s)));
+            };
+            auto read_v = [&](int i) __attribute__((always_inline)) {
+                return *reinterpret_cast<const u32x4*>(v0 + (i / DT) * 16 * RB + (i % DT) * 512);
+            };
+            constexpr int NV = 2 * DT, PER = 16 / KS;  // products' pairs; weights of a column tile per pair of scores
+            u32x4 kf[KS], vf[NV], pb[2][2];  // (pb: weights packed as the products' operands, [column tile][16 keys])
+            float mc[2];
+#pragma unroll
+            for (int ct = 0; ct < 2; ++ct) {
+                mc[ct] = m_run[ct] == -INFINITY ? 0.f : m_run[ct] * a.scale_log2;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) nxt[ct][e] = 0.f;
+            }
+            kf[0] = read_k(0), kf[1] = read_k(1);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                if (s + 2 < KS) kf[s + 2] = read_k(s + 2);
+                if (s + 2 >= KS) vf[s + 2 - KS] = read_v(s + 2 - KS);
+                nxt[0] = M::m32(kf[s], qf[0][s], nxt[0]);
+                nxt[1] = M::m32(kf[s], qf[1][s], nxt[1]);
+#pragma unroll
+                for (int ct = 0; ct < 2; ++ct) {
+#pragma unroll
+                    for (int e = PER * s; e < PER * (s + 1); ++e) {
+                        cur[ct][e] = __builtin_amdgcn_exp2f(fmaf(cur[ct][e], a.scale_log2, -mc[ct]));
+                        l_run[ct] += cur[ct][e];
+                    }
+#pragma unroll
+                    for (int e = PER * s; e < PER * (s + 1); e += 2)
+                        pb[ct][e >> 3][(e & 7) >> 1] = M::pack(cur[ct][e], cur[ct][e + 1]);
+                    asm volatile("" : "+v"(l_run[ct]));
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            constexpr int PM = 16 / NV;
+            float m[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                if (i + 2 < NV) vf[i + 2] = read_v(i + 2);
+                o[0][i % DT] = M::m32(vf[i], pb[0][i / DT], o[0][i % DT]);
+                o[1][i % DT] = M::m32(vf[i], pb[1][i / DT], o[1][i % DT]);
+#pragma unroll
+                for (int ct = 0; ct < 2; ++ct)
+#pragma unroll
+                    for (int e = PM * i; e < PM * (i + 1); e += 2) m[ct] = fmaxf(fmaxf(m[ct], nxt[ct][e]), nxt[ct][e + 1]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+#pragma unroll
+            for (int ct = 0; ct < 2; ++ct) {
+                const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(m[ct]), __float_as_uint(m[ct]), false, false);
+                mx[ct] = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+            }
+        };
+
+        // Step n stores K(n + 2) and V(n + 1), loaded by step n - 1, and loads K(n + 3) and V(n + 2).
+        int s1, s2, s3;
+        uint32_t b0, b1, b2, b3;
+        page_ids(0);
+        locate(0, s1, b0);
+        load_k(s1);
+        load_v(s1);
+        page_ids(1);
+        locate(1, s1, b1);
+        lds_barrier();  // the blocks of the piece before this one are read
+        store_k(0);
+        store_v(0, 0, b0);
+        if (nb > 1) load_k(s1);
+        page_ids(2);
+        locate(2, s2, b2);
+        if (nb > 1) {
+            store_k(1);
+            load_v(s1);
+        }
+        if (nb > 2) load_k(s2);
+        page_ids(3);
+        s3 = s2, b3 = b2;
+        lds_barrier();
+        float mx[2];
+        if (nbw > 0) {
+            scores(0, 0, sa);
+            maxima(sa, mx);
+            settle(0, 0, b0, sa, mx);
+        }
+        int kslot = 0;  // n % 3
+        for (int n = 0; n < nb; ++n) {
+            const int kslot1 = kslot == 2 ? 0 : kslot + 1, kslot2 = kslot1 == 2 ? 0 : kslot1 + 1;
+            if (n) lds_barrier();
+            if (n + 1 < nb) {
+                if (n + 2 < nb) store_k(kslot2);
+                store_v((n + 1) & 1, n + 1, b1);
+                if (n + 3 < nb) {
+                    locate(n + 3, s3, b3);
+                    load_k(s3);
+                    page_ids(n + 4);
+                }
+                if (n + 2 < nb) load_v(s2);
+            }
+            if (n < nbw) {
+                half(kslot, 1, sb, n & 1, 0, sa, mx);
+                settle(n, 1, b0, sb, mx);
+                half(kslot1, 0, sa, n & 1, 1, sb, mx);  // (scores behind the last block: not used)
+                if (n + 1 < nbw) settle(n + 1, 0, b1, sa, mx);
+            }
+            s2 = s3, b0 = b1, b1 = b2, b2 = b3, kslot = kslot1;
+        }
+#pragma unroll
+        for (int ct = 0; ct < 2; ++ct) {
+            const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(l_run[ct]), __float_as_uint(l_run[ct]), false, false);
+            l_run[ct] = __uint_as_float(x[0]) + __uint_as_float(x[1]);
+        }
+
+        auto write = [&]() __attribute__((always_inline)) {
+#pragma unroll
+            for (int ct = 0; ct < 2; ++ct) {
+                const int c = cw + 32 * ct + c32;
+                const float inv = l_run[ct] != 0.f ? 1.0f / l_run[ct] : 0.f;  // no key at all: zeros
+                const int row = rq.row0 + row_first + c / group, head = hk * group + c % group;
+                T* y = static_cast<T*>(a.y) + (size_t(row) * a.qh + head) * HD + 4 * h;
+                if (c < cols) {
+#pragma unroll
+                    for (int d = 0; d < DT; ++d)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)  // dims 32 d + 8 e + 4 h ..
+                            *reinterpret_cast<uint2*>(y + 32 * d + 8 * e) =
+                                make_uint2(M::pack(o[ct][d][4 * e] * inv, o[ct][d][4 * e + 1] * inv),
+                                           M::pack(o[ct][d][4 * e + 2] * inv, o[ct][d][4 * e + 3] * inv));
+                }
+            }
+        };
+        const uint32_t begin = u - uint32_t(j0), end = begin + uint32_t(units);
+        if (begin >= u0 && end <= u1) {
+            write();
+        } else {
+            const uint32_t wa = group_of(begin), wb = group_of(end - 1);
+            // column tile x, 16 bytes i of lane l: ((2 wave + x) 4 DT + i) 64 + l, after the maxima and sums
+            auto at = [&](float* slot, int ct, int i) {
+                return slot + 2 * paged::kTileCols + (((2 * wv + ct) * 4 * DT + i) * 64 + lane) * 4;
+            };
+            if (cw < cols) {
+                float* mine = slots + size_t(2 * w + (begin >= u0 ? 1 : 0)) * SW;
+#pragma unroll
+                for (int ct = 0; ct < 2; ++ct) {
+                    if (h == 0) store_agent(mine + 2 * (cw + 32 * ct + c32), m_run[ct], l_run[ct]);
+#pragma unroll
+                    for (int i = 0; i < 4 * DT; ++i) {
+                        const f32x16& x = o[ct][i >> 2];
+                        store_agent(at(mine, ct, i), x[4 * (i & 3)], x[4 * (i & 3) + 1]);
+                        store_agent(at(mine, ct, i) + 2, x[4 * (i & 3) + 2], x[4 * (i & 3) + 3]);
+                    }
+                }
+            }
+            __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0): this wave's stores are performed
+            lds_barrier();
+            uint32_t* counter = a.ws + wa;
+            if (t == 0) arrived = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            lds_barrier();
+            if (arrived == wb - wa) {  // the last one in joins the parts, in their order
+                if (cw < cols) {
+#pragma unroll
+                    for (int ct = 0; ct < 2; ++ct) {
+                        m_run[ct] = -INFINITY, l_run[ct] = 0.f;
+#pragma unroll
+                        for (int d = 0; d < DT; ++d)
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) o[ct][d][e] = 0.f;
+                    }
+                    for (uint32_t i = wa; i <= wb; ++i) {
+                        float* part = slots + size_t(2 * i + (i == wa ? 1 : 0)) * SW;
+#pragma unroll
+                        for (int ct = 0; ct < 2; ++ct) {
+                            const float2 ml = load_agent(part + 2 * (cw + 32 * ct + c32));
+                            const float mn = fmaxf(m_run[ct], ml.x), mc = mn == -INFINITY ? 0.f : mn * a.scale_log2;
+                            const float fo = __builtin_amdgcn_exp2f(m_run[ct] * a.scale_log2 - mc);
+                            const float fn = __builtin_amdgcn_exp2f(ml.x * a.scale_log2 - mc);
+                            l_run[ct] = l_run[ct] * fo + ml.y * fn;
+                            m_run[ct] = mn;
+#pragma unroll
+                            for (int j = 0; j < 4 * DT; ++j) {
+                                const float2 x = load_agent(at(part, ct, j)), z = load_agent(at(part, ct, j) + 2);
+                                f32x16& v = o[ct][j >> 2];
+                                const int e = 4 * (j & 3);
+                                v[e] = v[e] * fo + x.x * fn, v[e + 1] = v[e + 1] * fo + x.y * fn;
+                                v[e + 2] = v[e + 2] * fo + z.x * fn, v[e + 3] = v[e + 3] * fo + z.y * fn;
+                            }
+                        }
+                    }
+                    write();
+                }
+                if (t == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+        }
+        // ---- the next piece
+        u += uint32_t(nb);
+        kfirst = 0;
+        if (u < u1 && ++tile >= tiles_of(rq)) {
+            tile = 0;
+            if (++hk >= kvh) {
+                hk = 0;
+                ++r;
+                while (r < int(a.requests) - 1 && uniform(int(ends[r])) == uniform(int(ends[r - 1]))) ++r;
+                rq = request_of(a, uint32_t(r));
+                rq.row0 = uniform(rq.row0), rq.rows = uniform(rq.rows), rq.seen = uniform(rq.seen);
+            }
+        }
+    }
 }
 
 }  // namespace
@@ -687,21 +1096,18 @@ static void l_append(const PreparedDispatch& pd, void* const* p, hipStream_t s) 
 // the most new rows of a request in the dispatch, and whether every item's columns fit the kernel for few
 static uint32_t most_fresh(const uint32_t* w) { return w[11] ? std::min(w[11], w[10]) : w[10]; }
 static bool few_columns(const uint32_t* w) {
-    return w[13] && uint64_t(most_fresh(w)) * (w[12] / w[13]) <= paged::kCols;
+    return w[13] && uint64_t(most_fresh(w)) * (w[12] / w[13]) <= paged::kRowsCols;
 }
 template <typename T, int HD>
 static void launch_attn(const uint32_t* w, void* const* p, hipStream_t s) {
     const float scale_log2 = f32_of(w[18]) * 1.4426950408889634f;
-    if (few_columns(w)) {
-        const AttnArgs a{p[0], p[1], p[2], (const uint32_t*)p[3], (const uint32_t*)p[4], (const uint32_t*)p[5], p[6],
-                         (uint32_t*)p[7], w[9], w[10], most_fresh(w), w[12], w[13], w[15], log2_of(w[16]), w[17], scale_log2};
-        const uint32_t bytes = uint32_t(uint64_t(w[17]) * w[16] * w[13] * HD * 2);
-        hipLaunchKernelGGL((k_attn_rows<T, HD>), dim3(paged::kGroups), dim3(256), 0, s, a, bytes, bytes);
-        return;
-    }
-    hipLaunchKernelGGL((k_paged_attn<T, HD>), dim3(w[10], w[12]), dim3(64), 0, s, (const T*)p[0], (const T*)p[1],
-                       (const T*)p[2], (const uint32_t*)p[3], (const uint32_t*)p[4], (const uint32_t*)p[5], (T*)p[6], w[9],
-                       w[10], most_fresh(w), w[12], w[13], w[15], log2_of(w[16]), w[17], scale_log2);
+    const AttnArgs a{p[0], p[1], p[2], (const uint32_t*)p[3], (const uint32_t*)p[4], (const uint32_t*)p[5], p[6],
+                     (uint32_t*)p[7], w[9], w[10], most_fresh(w), w[12], w[13], w[15], log2_of(w[16]), w[17], scale_log2};
+    const uint32_t bytes = uint32_t(uint64_t(w[17]) * w[16] * w[13] * HD * 2);  // of each cache
+    if (few_columns(w))
+        hipLaunchKernelGGL((k_attn_rows<T, HD>), dim3(paged::kRowsGroups), dim3(256), 0, s, a, bytes, bytes);
+    else
+        hipLaunchKernelGGL((k_attn_tiles<T, HD>), dim3(paged::kTileGroups), dim3(256), 0, s, a, bytes);
 }
 static void l_attn(const PreparedDispatch& pd, void* const* p, hipStream_t s) {
     const uint32_t* w = pd.words.data();
@@ -833,7 +1239,7 @@ std::vector<KernelSpec> paged_catalog() {
     // 49 attention_paged
     c.push_back({"attention_paged", "paged", {256, 1, 1}, false,
                  [](const uint32_t* w) {
-                     return few_columns(w) ? Grid3{int64_t(paged::kGroups), 1, 1} : Grid3{w[10], w[12], 1};
+                     return Grid3{int64_t(few_columns(w) ? paged::kRowsGroups : paged::kTileGroups), 1, 1};
                  },
                  {TOK_R("q", H), TOK_R("k_cache", H), TOK_R("v_cache", H), TOK_R("table", U), TOK_R("starts", U),
                   TOK_R("context", U), TOK_W("y", H), TOK_RW("workspace", U), U32F("requests"), U32F("tokens"),
@@ -849,8 +1255,12 @@ std::vector<KernelSpec> paged_catalog() {
                      need_table(n, blocks, page);
                      const float scale = f32_of(w[18]);
                      if (!(scale > 0.f) || std::isinf(scale)) contract_fail("%s: scale must be positive and finite", n);
-                     if (times(R, kvh, uint64_t(blocks) * page / paged::kUnitKeys + 1) > 1ull << 31)
-                         contract_fail("%s: requests * kv_heads * blocks * page is more than one dispatch shares out", n);
+                     if (qh / kvh > paged::kTileCols)
+                         contract_fail("%s: at most %u query heads per KV head", n, paged::kTileCols);
+                     // units: a tile of a request's rows (at least one a request) x the blocks of keys, on every KV head
+                     const uint64_t tiles = R + uint64_t(T) / (paged::kTileCols / (qh / kvh));
+                     if (times(few_columns(w) ? R : tiles, kvh, uint64_t(blocks) * page / paged::kTileKeys + 1) > 1ull << 31)
+                         contract_fail("%s: rows * kv_heads * blocks * page are more than one dispatch shares out", n);
                      need(c, 0, times(T, qh, hd), n, "q");
                      need(c, 1, times(uint64_t(pages) * page, kvh, hd), n, "k_cache");
                      need(c, 2, times(uint64_t(pages) * page, kvh, hd), n, "v_cache");

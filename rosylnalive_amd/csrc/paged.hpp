@@ -22,22 +22,27 @@ constexpr uint32_t kMaxRequests = 4096;
 
 inline bool page_ok(uint32_t page) { return page >= 16 && page <= 256 && (page & (page - 1)) == 0; }
 
-// attention_paged shares its work out in units of kUnitKeys keys of one item (a request's rows on one KV head): workgroup w of
-// G = min(kGroups, units) takes the units [w units / G, (w + 1) units / G) of all items in order, whatever the lengths are.
-// An item that ends in another workgroup than it began in is joined from partials in the workspace: words 0 .. items - 1
-// count an item's partials in (zero between launches), then two slots per workgroup hold them: slot 2 w the part of the item
-// that w finds begun, slot 2 w + 1 the part of the item that w begins and does not end.
-constexpr uint32_t kGroups = 512;
-constexpr uint32_t kUnitKeys = 128;
-constexpr uint32_t kCols = 16;  // query columns (rows of a request x heads of a group) of an item
-constexpr uint64_t slot_words(uint64_t head_dim) { return 2 * kCols + kCols * head_dim; }  // maxima, sums, products
+// attention_paged shares its work out in units, a block of keys of one item (query columns of one request on one KV head):
+// workgroup w of G takes the units [w units / G, (w + 1) units / G) of all items in order, whatever the lengths are. An item
+// that ends in another workgroup than it began in is joined from partials in the workspace. Word w counts the partials of
+// the item that workgroup w begins and does not end (zero between launches); after the kGroups counters, slot 2 w holds the
+// part of the item that w finds begun, slot 2 w + 1 the part of the one that it begins and does not end.
+constexpr uint32_t kGroups = 512;  // the most workgroups of a launch
+// Items of few columns (a request's rows x the heads of a group up to 16): two workgroups per CU, units of 128 keys.
+constexpr uint32_t kRowsGroups = 512, kRowsKeys = 128, kRowsCols = 16;
+// Items of many columns: one workgroup per CU, tiles of up to 256 columns, units of 64 keys.
+constexpr uint32_t kTileGroups = 256, kTileKeys = 64, kTileCols = 256;
+// a slot: per column its maximum, its sum and its products
+constexpr uint64_t slot_words(uint64_t cols, uint64_t head_dim) { return cols * (2 + head_dim); }
 
-// u32 words of attention_paged's workspace.
+// u32 words of attention_paged's workspace. The lengths of a launch come from the device, so any launch of a batch may
+// split; one whose requests could not together have more than 16 columns on a KV head never takes the tiles.
 inline uint64_t workspace_words(uint64_t requests, uint64_t tokens, uint64_t q_heads, uint64_t kv_heads,
                                 uint64_t head_dim) {
-    (void)tokens, (void)q_heads;
-    const uint64_t counters = (requests * kv_heads + 63) / 64 * 64;
-    return counters + 2 * kGroups * slot_words(head_dim);
+    (void)requests;
+    const uint64_t rows = kGroups + 2 * kRowsGroups * slot_words(kRowsCols, head_dim);
+    const uint64_t tiles = kGroups + 2 * kTileGroups * slot_words(kTileCols, head_dim);
+    return kv_heads && tokens * (q_heads / kv_heads) <= kRowsCols ? rows : (tiles > rows ? tiles : rows);
 }
 
 }  // namespace paged

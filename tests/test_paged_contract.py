@@ -68,7 +68,7 @@ BAD = [("requests", 0, "requests"), ("requests", 4097, "requests"), ("tokens", 0
        ("max_pos", 0, "max_pos"), ("scale", 0.0, "scale"), ("scale", -1.0, "scale"), ("scale", float("nan"), "scale"),
        ("scale", float("inf"), "scale"),
        # sizes whose products wrap 32 or 64 bits
-       ("tokens", 0xFFFFFFFF, "elements|grid"), ("q_heads", 0xFFFFFFFE, "elements|grid"), ("max_pos", 0xFFFFFFFF, "elements"),
+       ("tokens", 0xFFFFFFFF, "elements|grid"), ("q_heads", 0xFFFFFFFE, "elements|grid|query heads"), ("q_heads", 514, "elements|query heads"), ("max_pos", 0xFFFFFFFF, "elements"),
        ("pages", 0x0FFFFFFF, "elements|pages")]
 
 
