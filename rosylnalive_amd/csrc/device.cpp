@@ -4,6 +4,8 @@
 
 #include <dlfcn.h>
 
+#include <algorithm>
+#include <chrono>
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
@@ -99,8 +101,9 @@ std::string f16_range_sites(uint32_t bits) {
 Device::~Device() {
     (void)hipSetDevice(index_);
     (void)hipStreamSynchronize(stream_);
+    for (const Mark& m : marks_) (void)hipEventDestroy(m.event);
+    for (hipEvent_t e : spare_events_) (void)hipEventDestroy(e);
     for (auto& kv : pending_) {
-        (void)hipEventDestroy(kv.second.done);
         for (auto& e : kv.second.timer_events) {
             (void)hipEventDestroy(e.first);
             (void)hipEventDestroy(e.second);
@@ -299,7 +302,7 @@ void CommandList::check_open() const {
 
 void CommandList::dispatch(int kernel, const uint32_t* words) {
     check_open();
-    if (exec_) contract_fail("a reusable list cannot be changed after its first submission");
+    if (replayed_) contract_fail("a reusable list cannot be changed after its first submission");
     if (!dev_->kernels_loaded()) contract_fail("Dispatch before LoadKernels");
     if (!dev_->contains(kernel)) contract_fail("kernel %d is not in the loaded kernel set", kernel);
     Cmd c{};
@@ -325,7 +328,7 @@ void CommandList::dispatch_library(int kernel, const uint32_t* words, int librar
 
 void CommandList::dispatch_library_all(const LibraryDispatch* d, size_t n, const LibraryCheck& check) {
     check_open();
-    if (exec_) contract_fail("a reusable list cannot be changed after its first submission");
+    if (replayed_) contract_fail("a reusable list cannot be changed after its first submission");
     if (!dev_->kernels_loaded()) contract_fail("Dispatch before LoadKernels");
     std::vector<Cmd> staged;
     staged.reserve(n);
@@ -370,7 +373,7 @@ void CommandList::barrier() {
     // The main stream is in order: every earlier command on it has finished its writes before a later one starts.
     // Overlapped dispatches are joined here.
     if (side_open_) {
-        if (exec_) contract_fail("a reusable list cannot be changed after its first submission");
+        if (replayed_) contract_fail("a reusable list cannot be changed after its first submission");
         Cmd c{};
         c.kind = Cmd::Join;
         cmds_.push_back(std::move(c));
@@ -380,7 +383,7 @@ void CommandList::barrier() {
 
 void CommandList::copy(int ss, uint64_t so, int ds, uint64_t dof, uint64_t bytes) {
     check_open();
-    if (exec_) contract_fail("a reusable list cannot be changed after its first submission");
+    if (replayed_) contract_fail("a reusable list cannot be changed after its first submission");
     check_copy(dev_->layout(), ss, so, ds, dof, bytes);
     Cmd c{};
     c.kind = Cmd::Copy;
@@ -412,6 +415,10 @@ void CommandList::end_timer(int timer) {
     c.kind = Cmd::TimerEnd;
     c.timer = timer;
     cmds_.push_back(std::move(c));
+}
+
+static int64_t host_ns() {
+    return std::chrono::duration_cast<std::chrono::nanoseconds>(std::chrono::steady_clock::now().time_since_epoch()).count();
 }
 
 CommandList* Device::begin(bool reusable) {
@@ -529,9 +536,13 @@ uint64_t Device::submit(CommandList* l, uint32_t repeat) {
         pend.timer_events = all;
         pend.timer_names = names;
         l->closed_ = true;
-    } else if (!graphs_enabled()) {
-        // Profilers that cannot follow stream capture: replay by launching the recorded commands directly.
+    } else if (!graphs_enabled() ||
+               (l->cmds_.size() <= kDirectLaunches &&
+                std::all_of(l->cmds_.begin(), l->cmds_.end(),
+                            [](const CommandList::Cmd& c) { return c.kind == CommandList::Cmd::Launch; }))) {
+        // A few launches, or a profiler that cannot follow stream capture: replay by launching the recorded commands.
         if (!l->timer_names_.empty()) contract_fail("a reusable list cannot hold timers");
+        l->replayed_ = true;
         for (uint32_t r = 0; r < repeat; ++r) run(l);
         HIPC(hipGetLastError());
     } else {
@@ -548,14 +559,45 @@ uint64_t Device::submit(CommandList* l, uint32_t repeat) {
             }
             HIPC(hipStreamEndCapture(stream_, &l->graph_));
             HIPC(hipGraphInstantiate(&l->exec_, l->graph_, nullptr, nullptr, 0));
+            l->replayed_ = true;
         }
         for (uint32_t r = 0; r < repeat; ++r) HIPC(hipGraphLaunch(l->exec_, stream_));
     }
-    HIPC(hipEventCreate(&pend.done));
-    HIPC(hipEventRecord(pend.done, stream_));
     uint64_t fence = next_fence_++;
     pending_[fence] = std::move(pend);
+    if (host_ns() - marked_ns_ >= kMarkNs) mark(fence);
     return fence;
+}
+
+void Device::mark(uint64_t fence) {
+    hipEvent_t e = nullptr;
+    if (spare_events_.empty()) {
+        HIPC(hipEventCreateWithFlags(&e, hipEventDisableTiming));
+    } else {
+        e = spare_events_.back();
+        spare_events_.pop_back();
+    }
+    const hipError_t r = hipEventRecord(e, stream_);
+    if (r != hipSuccess) {
+        spare_events_.push_back(e);
+        hip_check(r, "hipEventRecord");
+    }
+    marks_.push_back(Mark{fence, e});
+    marked_ns_ = host_ns();
+}
+
+void Device::reach(uint64_t fence) {
+    if (fence <= reached_) return;
+    HIPC(hipSetDevice(index_));
+    if (marks_.empty() || marks_.back().fence < fence) mark(next_fence_ - 1);
+    while (marks_.front().fence < fence) {  // older ones are behind the one waited for
+        spare_events_.push_back(marks_.front().event);
+        marks_.pop_front();
+    }
+    hip_check(hipEventSynchronize(marks_.front().event), "waiting for a submission (device lost or a kernel faulted)");
+    reached_ = marks_.front().fence;
+    spare_events_.push_back(marks_.front().event);
+    marks_.pop_front();
 }
 
 const Completion& Device::wait(uint64_t fence) {
@@ -569,10 +611,7 @@ const Completion& Device::wait(uint64_t fence) {
         contract_fail("submission %llu was never made on this backend", (unsigned long long)fence);
     }
     Pending& p = it->second;
-    hipError_t e = hipEventSynchronize(p.done);
-    if (e != hipSuccess) {
-        hip_check(e, "waiting for a submission (device lost or a kernel faulted)");
-    }
+    reach(fence);
     Completion c;
     c.submission = fence;
     c.dispatches = p.dispatches;
@@ -584,7 +623,6 @@ const Completion& Device::wait(uint64_t fence) {
         (void)hipEventDestroy(p.timer_events[i].first);
         (void)hipEventDestroy(p.timer_events[i].second);
     }
-    (void)hipEventDestroy(p.done);
     pending_.erase(it);
     // Waiting again returns the same completion (gpu-backend.md, IGpuBackend.Wait), for the most recent
     // kKeptCompletions submissions waited on; older ones are dropped, so a decode loop that submits and waits once per

@@ -5,15 +5,18 @@
 //   - one in-order HIP stream per device, so Barrier() costs nothing and Copy() is ordered on both sides;
 //   - the sealed table is kept on the host too: every token is resolved to a device pointer when a dispatch is
 //     recorded, and kernels receive plain pointers and the scalar argument words;
-//   - a fence is a hipEvent recorded after a submission; Wait synchronises it and returns the stored Completion;
+//   - a fence is a submission's number; Wait synchronises a hipEvent recorded at or after it and returns the stored
+//     Completion;
 //   - a command list created reusable is captured into a hipGraph at its first submission and replayed by every later
-//     submission (the decode step of the executor): zero host work per replay.
+//     submission (the decode step of the executor); one of a few launches is launched again instead, which takes less host
+//     time than a graph (kDirectLaunches).
 #pragma once
 
 #include <hip/hip_runtime_api.h>
 
 #include <array>
 #include <cstdint>
+#include <deque>
 #include <functional>
 #include <map>
 #include <memory>
@@ -142,6 +145,7 @@ class CommandList {
     std::vector<int> open_timers_;
     int dispatches_ = 0;
     bool side_open_ = false;  // an overlapped dispatch not yet joined
+    bool replayed_ = false;   // a reusable list that was submitted
     hipGraph_t graph_ = nullptr;
     hipGraphExec_t exec_ = nullptr;
 };
@@ -216,6 +220,9 @@ class Device {
     void launch_side(const CommandList::Cmd& c);  // fork from the main stream, launch on the side stream
     void join_side();                             // the main stream waits for the side stream
     static bool graphs_enabled();
+    // A graph's launch takes 17 us of host time on MI355X whatever it holds, a kernel's 2.6: lists of up to this many
+    // launches and nothing else are launched one by one.
+    static constexpr size_t kDirectLaunches = 6;
     void run_probe();
     DeviceInfo info_{};
     int index_;
@@ -239,12 +246,25 @@ class Device {
     std::array<uint32_t, 7> probe_results_{};
     uint64_t next_fence_ = 1;
     struct Pending {
-        hipEvent_t done;
         std::vector<std::pair<hipEvent_t, hipEvent_t>> timer_events;
         std::vector<std::string> timer_names;
         int dispatches;
     };
     std::map<uint64_t, Pending> pending_;
+    // Completion of submissions: events on the stream, each for every submission up to its own, oldest first. Recording one
+    // costs 4 us of host time on MI355X, more than a kernel's launch (2.6 us), so submissions that follow each other within
+    // kMarkNs share one; a wait for a submission that has none behind it records one then.
+    struct Mark {
+        uint64_t fence;
+        hipEvent_t event;
+    };
+    static constexpr int64_t kMarkNs = 20000;
+    void mark(uint64_t fence);
+    void reach(uint64_t fence);  // waits until every submission up to `fence` has completed
+    std::deque<Mark> marks_;
+    std::vector<hipEvent_t> spare_events_;
+    int64_t marked_ns_ = 0;       // host clock at the last mark
+    uint64_t reached_ = 0;        // submissions up to this one have completed
     std::map<uint64_t, Completion> done_;  // the last kKeptCompletions waited on, by fence
 
   public:

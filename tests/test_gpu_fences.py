@@ -1,0 +1,92 @@
+"""Submissions that share a completion event: short lists made right behind each other, waited for in any order; and replays of
+short reusable lists, which are launched again rather than captured, next to captured ones."""
+import numpy as np
+import pytest
+
+from gpu_session import Session
+from rosylnalive_amd.gpu_core import DType, GpuContractException
+
+pytestmark = pytest.mark.gpu
+
+F32 = DType.F32
+N = 5000
+
+
+@pytest.fixture()
+def sess():
+    x = np.arange(N, dtype=np.float32)
+    s = Session({"x": (F32, (N,), 0, x), "y": (F32, (N,), 0, None), "z": (F32, (N,), 0, None)})
+    yield s
+    s.close()
+
+
+def _scale(s, cl, a, times=1, src="x", dst="y"):
+    for _ in range(times):
+        cl.dispatch("scale_f32", s.fields("scale_f32", x=src, y=dst, n=N, a=a))
+
+
+@pytest.mark.parametrize("order", ["first to last", "last to first", "shuffled"])
+def test_waits_in_any_order(sess, order):
+    lists, fences = [], []
+    for i in range(150):
+        cl = sess.backend.begin()
+        _scale(sess, cl, float(i), times=1 + i % 3)
+        fences.append(sess.backend.submit(cl))
+        lists.append(cl)
+    assert fences == sorted(set(fences))
+    turn = list(range(150))
+    if order == "last to first":
+        turn.reverse()
+    elif order == "shuffled":
+        np.random.default_rng(4).shuffle(turn)
+    for i in turn:
+        c = sess.backend.wait(fences[i])
+        assert c.submission == fences[i] and c.dispatches == 1 + i % 3
+        if i == 149:  # the newest: its result is there once its wait returns
+            assert np.array_equal(sess.read("y"), np.arange(N, dtype=np.float32) * np.float32(149))
+    assert sess.backend.wait(fences[3]).dispatches == 1  # again
+    with pytest.raises(GpuContractException, match="never made"):
+        sess.backend.wait(int(fences[-1]) + 1)
+    for cl in lists:
+        cl.release()
+
+
+def test_a_wait_between_submissions(sess):
+    """A program that keeps two submissions under way: each waited-for one is complete when its wait returns."""
+    prev = None
+    for i in range(1, 60):
+        cl = sess.backend.begin()
+        _scale(sess, cl, float(i))
+        _scale(sess, cl, 2.0, src="y", dst="z")
+        fence = sess.backend.submit(cl)
+        if prev is not None:
+            assert sess.backend.wait(prev[0]).dispatches == 2
+            prev[1].release()
+        prev = (fence, cl)
+    sess.backend.wait(prev[0])
+    assert np.array_equal(sess.read("z"), np.arange(N, dtype=np.float32) * np.float32(118))
+
+
+@pytest.mark.parametrize("launches", [1, 6, 7, 20])
+def test_replays_of_short_and_long_lists(sess, launches):
+    """z = x 2^launches by doubling in place, replayed `repeat` times with new inputs between, however the list is replayed; no
+    change after the first submission."""
+    cl = sess.backend.begin(reusable=True)
+    for _ in range(launches):
+        cl.dispatch("scale_f32", sess.fields("scale_f32", x="z", y="z", n=N, a=2.0))
+    for repeat in (1, 3, 2):
+        x = np.random.default_rng(repeat).standard_normal(N).astype(np.float32)
+        sess.write("z", x)
+        c = sess.backend.wait(sess.backend.submit(cl, repeat))
+        assert c.dispatches == launches * repeat
+        assert np.array_equal(sess.read("z"), x * np.float32(2.0 ** (launches * repeat)))
+        with pytest.raises(GpuContractException, match="cannot be changed"):
+            _scale(sess, cl, 1.0)
+    cl.release()
+    cl = sess.backend.begin(reusable=True)
+    cl.begin_timer("t")
+    _scale(sess, cl, 1.0)
+    cl.end_timer(0)
+    with pytest.raises(GpuContractException, match="timers"):
+        sess.backend.submit(cl)
+    cl.release()
