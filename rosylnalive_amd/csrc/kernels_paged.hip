@@ -172,47 +172,145 @@ __device__ __forceinline__ __bf16 narrow<__bf16>(float v) {
     return __builtin_bit_cast(__bf16, f2bf(v));
 }
 
+// two floats to a pair of the type, round to nearest even (one conversion instruction)
+template <typename T>
+__device__ __forceinline__ uint32_t pack(float a, float b) {
+    typedef T t2 __attribute__((ext_vector_type(2)));
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2){a, b}, t2));
+}
+
+// N consecutive elements as floats, in one load
+template <typename T, int N>
+__device__ __forceinline__ void load_n(const T* p, float (&v)[N]) {
+    typedef T vec __attribute__((ext_vector_type(N)));
+    const vec x = *reinterpret_cast<const vec*>(p);
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = widen<T>(x[i]);
+}
+// N consecutive floats narrowed, in one store
+template <typename T, int N>
+__device__ __forceinline__ void store_n(T* p, const float (&v)[N]) {
+    typedef uint32_t vec __attribute__((ext_vector_type(N / 2)));
+    vec x;
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) x[i] = pack<T>(v[2 * i], v[2 * i + 1]);
+    *reinterpret_cast<vec*>(p) = x;
+}
+
+// the sum over the N lanes of an aligned group
+template <int N>
+__device__ __forceinline__ float sum_lanes(float v) {
+    v = quad4_sum(v);
+    if constexpr (N >= 8) v += dpp_f<0x141>(v);
+    if constexpr (N >= 16) v += dpp_f<0x140>(v);
+    return v;
+}
+
 // ---------------------------------------------------------------- 48 qk_norm_rope_append_paged
-// One wave per (row, head): the head's sum of squares over the wave, its norm and rotation, one store. The values' eight
-// positions of a tile come from eight rows, so their stores are two bytes each.
+// Bound by the projections' bytes. Queries and keys: a head is 4 to 16 lanes with 16 bytes of its lower and of its upper
+// half each, so a lane holds the pairs that the rotation turns, the sum of squares is a few DPP adds, and a wave takes 4 to
+// 16 heads of a row at a time; the row's rotation and the norm weights are loaded once per wave. Values: a wave takes the
+// runs of rows that begin in its 8 rows, a run being rows whose slots follow each other in one tile of 8 positions; a
+// whole run's 8 rows of a dim are one 16-byte store, and shorter runs (a single token, the ends of a chunk) store each value
+// alone. Rows whose slot or position has no place are not appended.
 template <typename IN, typename T, int HD>
 __global__ __launch_bounds__(256) void k_paged_append(const IN* qkv, const uint16_t* qn, const uint16_t* kn,
                                                       const float* cos_t, const float* sin_t, const uint32_t* starts,
                                                       const uint32_t* positions, const uint32_t* slots, T* q, T* kc, T* vc,
                                                       uint32_t requests, uint32_t tokens, uint32_t qh, uint32_t kvh,
-                                                      uint32_t max_pos, uint32_t page_log2, uint32_t pages, float eps) {
-    constexpr int H = HD / 2;
-    const uint32_t row = blockIdx.x, lane = threadIdx.x & 63, head = blockIdx.y * 4 + (threadIdx.x >> 6);
-    if (row >= min(starts[requests], tokens) || head >= qh + 2 * kvh) return;
-    const uint32_t pos = positions[row], slot = slots[row], id = slot >> page_log2, off = slot & ((1u << page_log2) - 1);
-    const bool in = lane < H;
-    const IN* x = qkv + (size_t(row) * (qh + 2 * kvh) + head) * HD;
-    const float a = in ? widen(x[lane]) : 0.f, b = in ? widen(x[lane + H]) : 0.f;
-    if (head >= qh + kvh) {
-        if (id >= pages || pos >= max_pos || !in) return;
-        T* v = vc + ((size_t(id) * kvh + (head - qh - kvh)) << page_log2) * HD + size_t(off >> 3) * (8 * HD) + (off & 7);
-        v[lane * 8] = narrow<T>(a);
-        v[(lane + H) * 8] = narrow<T>(b);
+                                                      uint32_t max_pos, uint32_t page_log2, uint32_t pages, float eps,
+                                                      uint32_t qk_blocks, uint32_t parts, uint32_t v_chunks) {
+    constexpr int H = HD / 2, VEC = 16 / int(sizeof(IN)), LPH = H / VEC, HPW = 64 / LPH;
+    const uint32_t lane = threadIdx.x & 63, page_mask = (1u << page_log2) - 1, w = qh + 2 * kvh;
+    const uint32_t rows = min(starts[requests], tokens);
+    auto place = [&](uint32_t slot, uint32_t pos) { return (slot >> page_log2) < pages && pos < max_pos; };
+    const uint32_t block = blockIdx.y * gridDim.x + blockIdx.x;  // (a grid past 65,535 is folded)
+    if (block < qk_blocks) {
+        const uint32_t wave = block * 4 + uint32_t(__builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6)));
+        const uint32_t row = wave / parts, part = wave % parts;
+        if (row >= rows) return;
+        const uint32_t pos = positions[row], slot = slots[row], heads = qh + kvh, sub = lane % LPH;
+        const bool turn = pos < max_pos, keep = place(slot, pos);
+        const size_t angle = size_t(turn ? pos : 0) * H + VEC * sub;
+        float c[VEC], s[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; i += 4) {
+            load_n(cos_t + angle + i, *reinterpret_cast<float(*)[4]>(c + i));
+            load_n(sin_t + angle + i, *reinterpret_cast<float(*)[4]>(s + i));
+        }
+        typedef uint16_t wvec __attribute__((ext_vector_type(VEC)));
+        const wvec q0 = *reinterpret_cast<const wvec*>(qn + VEC * sub), q1 = *reinterpret_cast<const wvec*>(qn + H + VEC * sub);
+        const wvec k0 = *reinterpret_cast<const wvec*>(kn + VEC * sub), k1 = *reinterpret_cast<const wvec*>(kn + H + VEC * sub);
+        const IN* x = qkv + size_t(row) * w * HD + VEC * sub;
+        T* const krow = kc + ((size_t(slot >> page_log2) * kvh << page_log2) + (slot & page_mask)) * HD + VEC * sub;
+#pragma unroll 2
+        for (uint32_t head = part * HPW + lane / LPH; head < heads; head += parts * HPW) {
+            float a[VEC], b[VEC];
+            load_n(x + size_t(head) * HD, a);
+            load_n(x + size_t(head) * HD + H, b);
+            float sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) sum = fmaf(a[i], a[i], fmaf(b[i], b[i], sum));
+            const float r = 1.0f / sqrtf(sum_lanes<LPH>(sum) / float(HD) + eps);
+            float lo[VEC], hi[VEC];
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                const float an = bf2f(head < qh ? q0[i] : k0[i]) * (a[i] * r), bn = bf2f(head < qh ? q1[i] : k1[i]) * (b[i] * r);
+                lo[i] = turn ? an * c[i] - bn * s[i] : 0.f;
+                hi[i] = turn ? bn * c[i] + an * s[i] : 0.f;
+            }
+            if (head < qh) {
+                T* y = q + (size_t(row) * qh + head) * HD + VEC * sub;
+                store_n(y, lo);
+                store_n(y + H, hi);
+            } else if (keep) {
+                T* y = krow + (size_t(head - qh) << page_log2) * HD;
+                store_n(y, lo);
+                store_n(y + H, hi);
+            }
+        }
         return;
     }
-    const float r = 1.0f / sqrtf(wave_sum(a * a + b * b) / float(HD) + eps);
-    if (!in) return;
-    const uint16_t* w = head < qh ? qn : kn;
-    const float an = bf2f(w[lane]) * (a * r), bn = bf2f(w[lane + H]) * (b * r);
-    float lo = 0.f, hi = 0.f;
-    if (pos < max_pos) {
-        const float c = cos_t[size_t(pos) * H + lane], s = sin_t[size_t(pos) * H + lane];
-        lo = an * c - bn * s;
-        hi = bn * c + an * s;
-    }
-    if (head < qh) {
-        T* y = q + (size_t(row) * qh + head) * HD;
-        y[lane] = narrow<T>(lo);
-        y[lane + H] = narrow<T>(hi);
-    } else if (id < pages && pos < max_pos) {
-        T* k = kc + (((size_t(id) * kvh + (head - qh)) << page_log2) + off) * HD;
-        k[lane] = narrow<T>(lo);
-        k[lane + H] = narrow<T>(hi);
+    // ---- values: 8 rows and 128 elements of the row's value heads per wave
+    constexpr int E = 2;
+    const uint32_t wave = (block - qk_blocks) * 4 + uint32_t(__builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6)));
+    const uint32_t row0 = wave / v_chunks * 8, flat = (wave % v_chunks) * (64 * E) + E * lane;
+    if (row0 >= rows) return;
+    // lane i looks at row row0 - 1 + i: does it go on where the row before it stood, in the same tile?
+    const uint32_t mine = row0 + lane - 1;  // (row0 = 0, lane 0: past every row)
+    const bool there = lane < 16 && mine < rows;
+    const uint32_t slot = there ? slots[mine] : paged::kNone;
+    const bool good = there && place(slot, positions[mine]);
+    const uint32_t before = uint32_t(__shfl_up(int(slot), 1, 64));
+    const uint32_t goods = uint32_t(__ballot(good)) & 0xFFFFu;
+    const bool goes_on = good && lane > 0 && (goods >> (lane - 1) & 1u) && slot == before + 1 && (slot & 7) != 0;
+    const uint32_t on = uint32_t(__ballot(goes_on)) & 0xFFFFu;
+    uint32_t firsts = goods & ~on & 0x1FEu;  // runs that begin in this wave's rows, bit i for row0 - 1 + i
+    const uint32_t head = flat / HD, dim = flat % HD;
+    while (firsts) {
+        const int i = __builtin_ctz(firsts);
+        firsts &= firsts - 1;
+        const int n = 1 + __builtin_ctz(~(on >> (i + 1)));  // rows of the run, at most 8: a tile ends it
+        const uint32_t first = row0 + i - 1, at = uint32_t(__builtin_amdgcn_readlane(int(slot), i));
+        if (head >= kvh) continue;
+        const IN* x = qkv + (size_t(first) * w + qh + kvh) * HD + flat;
+        T* y = vc + ((size_t(at >> page_log2) * kvh + head) << page_log2) * HD + size_t((at & page_mask) >> 3) * (8 * HD) + dim * 8;
+        float v[8][E];
+        if (n == 8) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) load_n(x + size_t(j) * w * HD, v[j]);
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                *reinterpret_cast<u32x4*>(y + 8 * e) = u32x4{pack<T>(v[0][e], v[1][e]), pack<T>(v[2][e], v[3][e]),
+                                                             pack<T>(v[4][e], v[5][e]), pack<T>(v[6][e], v[7][e])};
+        } else {
+            for (int j = 0; j < n; ++j) {
+                load_n(x + size_t(j) * w * HD, v[0]);
+#pragma unroll
+                for (int e = 0; e < E; ++e) y[8 * e + (at & 7) + j] = narrow<T>(v[0][e]);
+            }
+        }
     }
 }
 
@@ -254,7 +352,6 @@ struct Mfma<_Float16> {
     static __device__ __forceinline__ f32x16 m32(u32x4 a, u32x4 b, f32x16 c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(vec, a), __builtin_bit_cast(vec, b), c, 0, 0, 0);
     }
-    static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack2h(a, b); }
 };
 template <>
 struct Mfma<__bf16> {
@@ -264,12 +361,6 @@ struct Mfma<__bf16> {
     }
     static __device__ __forceinline__ f32x16 m32(u32x4 a, u32x4 b, f32x16 c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(vec, a), __builtin_bit_cast(vec, b), c, 0, 0, 0);
-    }
-    // two floats to a bf16 pair, round to nearest even (one v_cvt_pk_bf16_f32)
-    static __device__ __forceinline__ uint32_t pack(float a, float b) {
-        typedef __bf16 h2 __attribute__((ext_vector_type(2)));
-        typedef float f2 __attribute__((ext_vector_type(2)));
-        return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2){a, b}, h2));
     }
 };
 
@@ -451,7 +542,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(AttnArgs a, uint32_t k_byt
             l_run += sc[e];
         }
         // the weights go into the product rounded to the cache's type, as its values are; their sum stays float32
-        const u32x4 pb = {M::pack(sc[0], sc[1]), M::pack(sc[2], sc[3]), M::pack(sc[4], sc[5]), M::pack(sc[6], sc[7])};
+        const u32x4 pb = {pack<T>(sc[0], sc[1]), pack<T>(sc[2], sc[3]), pack<T>(sc[4], sc[5]), pack<T>(sc[6], sc[7])};
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[d] = M::m16(vr[S][d], pb, o[d]);
     };
@@ -489,7 +580,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(AttnArgs a, uint32_t k_byt
                 const float inv = sum != 0.f ? 1.0f / sum : 0.f;  // no key at all: zeros
                 const int row = p.row0 + c / group, head = p.h * group + c % group;
                 T* y = static_cast<T*>(a.y) + (size_t(row) * a.qh + head) * HD + d;
-                *reinterpret_cast<uint2*>(y) = make_uint2(M::pack(v[0] * inv, v[1] * inv), M::pack(v[2] * inv, v[3] * inv));
+                *reinterpret_cast<uint2*>(y) = make_uint2(pack<T>(v[0] * inv, v[1] * inv), pack<T>(v[2] * inv, v[3] * inv));
             } else {
                 store_agent(mine + 2 * paged::kRowsCols + c * HD + d, v[0], v[1]);
                 store_agent(mine + 2 * paged::kRowsCols + c * HD + d + 2, v[2], v[3]);
@@ -523,7 +614,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(AttnArgs a, uint32_t k_byt
                     const int row = p.row0 + c / group, head = p.h * group + c % group;
                     T* y = static_cast<T*>(a.y) + (size_t(row) * a.qh + head) * HD + d;
                     *reinterpret_cast<uint2*>(y) =
-                        make_uint2(M::pack(v[0] * inv, v[1] * inv), M::pack(v[2] * inv, v[3] * inv));
+                        make_uint2(pack<T>(v[0] * inv, v[1] * inv), pack<T>(v[2] * inv, v[3] * inv));
                 }
                 if (t == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             }
@@ -855,7 +946,7 @@ __global__ __launch_bounds__(256, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
                     }
 #pragma unroll
                     for (int e = PER * s; e < PER * (s + 1); e += 2)
-                        pb[ct][e >> 3][(e & 7) >> 1] = M::pack(cur[ct][e], cur[ct][e + 1]);
+                        pb[ct][e >> 3][(e & 7) >> 1] = pack<T>(cur[ct][e], cur[ct][e + 1]);
                     asm volatile("" : "+v"(l_run[ct]));
                 }
                 __builtin_amdgcn_sched_barrier(0);
@@ -950,8 +1041,8 @@ __global__ __launch_bounds__(256, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
 #pragma unroll
                         for (int e = 0; e < 4; ++e)  // dims 32 d + 8 e + 4 h ..
                             *reinterpret_cast<uint2*>(y + 32 * d + 8 * e) =
-                                make_uint2(M::pack(o[ct][d][4 * e] * inv, o[ct][d][4 * e + 1] * inv),
-                                           M::pack(o[ct][d][4 * e + 2] * inv, o[ct][d][4 * e + 3] * inv));
+                                make_uint2(pack<T>(o[ct][d][4 * e] * inv, o[ct][d][4 * e + 1] * inv),
+                                           pack<T>(o[ct][d][4 * e + 2] * inv, o[ct][d][4 * e + 3] * inv));
                 }
             }
         };
@@ -1062,32 +1153,49 @@ static void l_plan(const PreparedDispatch& pd, void* const* p, hipStream_t s) {
 
 // qkv, q_norm, k_norm, cos_table, sin_table, starts, positions, slots, q, k_cache, v_cache, requests, tokens, q_heads,
 // kv_heads, head_dim, max_pos, page, pages, eps
+// The grid of 48: waves of queries and keys, then waves of values. A wave takes 1024 elements of a row's query and key heads,
+// or, from 2048 rows on, which fill the GPU so, all of them (the row's rotation is then loaded once); 8 rows x 128
+// elements of the value heads.
+struct AppendGrid {
+    uint32_t parts, qk_blocks, v_chunks, v_blocks;
+};
+static AppendGrid append_grid(const uint32_t* w) {
+    const uint64_t T = w[13];
+    AppendGrid g;
+    g.parts = T >= 2048 ? 1 : uint32_t(((uint64_t(w[14]) + w[15]) * w[16] + 1023) / 1024);
+    g.qk_blocks = uint32_t((T * g.parts + 3) / 4);
+    g.v_chunks = uint32_t((uint64_t(w[15]) * w[16] + 127) / 128);
+    g.v_blocks = uint32_t(((T + 7) / 8 * g.v_chunks + 3) / 4);
+    return g;
+}
 template <typename IN, typename T, int HD>
-static void launch_append(const uint32_t* w, void* const* p, hipStream_t s) {
-    hipLaunchKernelGGL((k_paged_append<IN, T, HD>), dim3(w[13], (w[14] + 2 * w[15] + 3) / 4), dim3(256), 0, s,
+static void launch_append(const uint32_t* w, const Physical& d, void* const* p, hipStream_t s) {
+    const AppendGrid g = append_grid(w);
+    hipLaunchKernelGGL((k_paged_append<IN, T, HD>), dim3(d.x, d.y), dim3(256), 0, s,
                        (const IN*)p[0], (const uint16_t*)p[1], (const uint16_t*)p[2], (const float*)p[3],
                        (const float*)p[4], (const uint32_t*)p[5], (const uint32_t*)p[6], (const uint32_t*)p[7], (T*)p[8],
-                       (T*)p[9], (T*)p[10], w[12], w[13], w[14], w[15], w[17], log2_of(w[18]), w[19], f32_of(w[20]));
+                       (T*)p[9], (T*)p[10], w[12], w[13], w[14], w[15], w[17], log2_of(w[18]), w[19], f32_of(w[20]),
+                       g.qk_blocks, g.parts, g.v_chunks);
 }
 template <typename IN, typename T>
-static void launch_append(const uint32_t* w, void* const* p, hipStream_t s) {
+static void launch_append(const uint32_t* w, const Physical& d, void* const* p, hipStream_t s) {
     if (w[16] == 64)
-        launch_append<IN, T, 64>(w, p, s);
+        launch_append<IN, T, 64>(w, d, p, s);
     else
-        launch_append<IN, T, 128>(w, p, s);
+        launch_append<IN, T, 128>(w, d, p, s);
 }
 static void l_append(const PreparedDispatch& pd, void* const* p, hipStream_t s) {
     const uint32_t* w = pd.words.data();
     const bool half = dtype_of(pd, 8) == F16;
     if (dtype_of(pd, 0) == F32) {
         if (half)
-            launch_append<float, _Float16>(w, p, s);
+            launch_append<float, _Float16>(w, pd.physical, p, s);
         else
-            launch_append<float, __bf16>(w, p, s);
+            launch_append<float, __bf16>(w, pd.physical, p, s);
     } else if (half) {
-        launch_append<_Float16, _Float16>(w, p, s);
+        launch_append<_Float16, _Float16>(w, pd.physical, p, s);
     } else {
-        launch_append<__bf16, __bf16>(w, p, s);
+        launch_append<__bf16, __bf16>(w, pd.physical, p, s);
     }
 }
 
@@ -1205,8 +1313,11 @@ std::vector<KernelSpec> paged_catalog() {
                      need(c, 8, 3, n, "counts");
                  }});
     // 48 qk_norm_rope_append_paged
-    c.push_back({"qk_norm_rope_append_paged", "paged", {256, 1, 1}, false,
-                 [](const uint32_t* w) { return Grid3{w[13], (int64_t(w[14]) + 2 * int64_t(w[15]) + 3) / 4, 1}; },
+    c.push_back({"qk_norm_rope_append_paged", "paged", {256, 1, 1}, true,
+                 [](const uint32_t* w) {
+                     const AppendGrid g = append_grid(w);
+                     return Grid3{int64_t(g.qk_blocks) + g.v_blocks, 1, 1};
+                 },
                  {TOK_R("qkv", H | DT(F32)), TOK_R("q_norm", DT(BF16)), TOK_R("k_norm", DT(BF16)),
                   TOK_R("cos_table", DT(F32)), TOK_R("sin_table", DT(F32)), TOK_R("starts", U), TOK_R("positions", U),
                   TOK_R("slots", U), TOK_W("q", H), TOK_RW("k_cache", H), TOK_RW("v_cache", H), U32F("requests"),

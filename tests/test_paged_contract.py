@@ -64,7 +64,7 @@ def test_workspace_too_small():
 BAD = [("requests", 0, "requests"), ("requests", 4097, "requests"), ("tokens", 0, "tokens|grid"), ("page", 8, "page"),
        ("page", 24, "page"), ("page", 512, "page"), ("page", 0, "page"), ("pages", 0, "pages"),
        ("pages", 1 << 28, "pages"), ("blocks", 0, "blocks"), ("blocks", 1 << 28, "blocks"), ("kv_heads", 0, "kv_heads"),
-       ("kv_heads", 3, "kv_heads"), ("q_heads", 0, "kv_heads|grid"), ("head_dim", 32, "head_dim"), ("head_dim", 0, "head_dim"),
+       ("kv_heads", 3, "kv_heads"), ("q_heads", 0, "kv_heads|grid"), ("head_dim", 32, "head_dim"), ("head_dim", 0, "head_dim|grid"),
        ("max_pos", 0, "max_pos"), ("scale", 0.0, "scale"), ("scale", -1.0, "scale"), ("scale", float("nan"), "scale"),
        ("scale", float("inf"), "scale"),
        # sizes whose products wrap 32 or 64 bits
