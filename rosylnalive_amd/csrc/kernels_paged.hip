@@ -364,14 +364,23 @@ struct Mfma<__bf16> {
     }
 };
 
-__device__ __forceinline__ void store_agent(float* p, float a, float b) {
-    __hip_atomic_store(reinterpret_cast<uint64_t*>(p), uint64_t(__float_as_uint(a)) | (uint64_t(__float_as_uint(b)) << 32),
-                       __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+// Partials pass between workgroups, which may run on other XCDs: stores that go through to memory and loads that do not take
+// an older line from the XCD's L2 (device scope), 16 or 8 bytes each and as many under way as there are registers (the
+// atomic loads of that scope are waited for one by one: a join of two parts took 25 us, of 32 parts 320).
+constexpr int kDeviceScope = 16;  // the sc1 bit of a buffer instruction
+__device__ __forceinline__ void store_part(__amdgpu_buffer_rsrc_t r, int word, f32x4 v) {
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), r, word * 4, 0, kDeviceScope);
 }
-__device__ __forceinline__ float2 load_agent(const float* p) {
-    const uint64_t v =
-        __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    return make_float2(__uint_as_float(uint32_t(v)), __uint_as_float(uint32_t(v >> 32)));
+__device__ __forceinline__ f32x4 load_part(__amdgpu_buffer_rsrc_t r, int word) {
+    return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, word * 4, 0, kDeviceScope));
+}
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ void store_part2(__amdgpu_buffer_rsrc_t r, int word, float a, float b) {
+    __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(a), __float_as_uint(b)}, r, word * 4, 0, kDeviceScope);
+}
+__device__ __forceinline__ float2 load_part2(__amdgpu_buffer_rsrc_t r, int word) {
+    const u32x2 v = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, word * 4, 0, kDeviceScope));
+    return make_float2(__uint_as_float(v[0]), __uint_as_float(v[1]));
 }
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
@@ -548,8 +557,17 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(AttnArgs a, uint32_t k_byt
     };
 
     // ---- the end of an item here: the waves' parts meet in LDS, then y, or a partial and the join
-    float* const slots = reinterpret_cast<float*>(a.ws + paged::kGroups);
+    auto add_part = [&](float& m, float& sum, f32x4& v, float mo, float so, f32x4 vo) __attribute__((always_inline)) {
+        const float mn = fmaxf(m, mo), mc = mn == -INFINITY ? 0.f : mn * a.scale_log2;
+        const float fo = __builtin_amdgcn_exp2f(m * a.scale_log2 - mc), fn = __builtin_amdgcn_exp2f(mo * a.scale_log2 - mc);
+        sum = sum * fo + so * fn;
+        v = v * fo + vo * fn;
+        m = mn;
+    };
     constexpr int SW = int(paged::slot_words(paged::kRowsCols, HD));
+    const __amdgpu_buffer_rsrc_t ws = __builtin_amdgcn_make_buffer_rsrc(
+        a.ws, 0, int(4 * (paged::kGroups + 2 * paged::kRowsGroups * SW)), 0x00020000);
+    auto slot_at = [&](uint32_t i, bool begins) { return int(paged::kGroups) + int(2 * i + (begins ? 1 : 0)) * SW; };
     auto finish = [&](const Place& p, uint32_t u) {
         const float l = cross_rows_sum(l_run);
         if (g == 0) xm[wv][c16] = m_run, xl[wv][c16] = l;
@@ -560,7 +578,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(AttnArgs a, uint32_t k_byt
         const uint32_t begin = u - uint32_t(p.k), end = begin + uint32_t(p.n);
         const bool whole = begin >= u0 && end <= u1;
         const uint32_t wa = group_of(begin), wb = group_of(end - 1);
-        float* mine = slots + size_t(2 * w + (begin >= u0 ? 1 : 0)) * SW;
+        const int mine = slot_at(w, begin >= u0);
         constexpr int Q4 = HD / 4;
         for (int e = t; e < p.cols * Q4; e += 256) {
             const int c = e / Q4, d = 4 * (e % Q4);
@@ -582,9 +600,8 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(AttnArgs a, uint32_t k_byt
                 T* y = static_cast<T*>(a.y) + (size_t(row) * a.qh + head) * HD + d;
                 *reinterpret_cast<uint2*>(y) = make_uint2(pack<T>(v[0] * inv, v[1] * inv), pack<T>(v[2] * inv, v[3] * inv));
             } else {
-                store_agent(mine + 2 * paged::kRowsCols + c * HD + d, v[0], v[1]);
-                store_agent(mine + 2 * paged::kRowsCols + c * HD + d + 2, v[2], v[3]);
-                if (d == 0) store_agent(mine + 2 * c, m, sum);
+                store_part(ws, mine + 2 * int(paged::kRowsCols) + c * HD + d, v);
+                if (d == 0) store_part2(ws, mine + 2 * c, m, sum);
             }
         }
         if (!whole) {
@@ -594,27 +611,51 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(AttnArgs a, uint32_t k_byt
             if (t == 0) arrived = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             lds_barrier();
             if (arrived == wb - wa) {  // the last one in joins the parts, in their order
-                for (int e = t; e < p.cols * Q4; e += 256) {
+                // a thread takes four dims of a column over the parts wa + k, wa + k + K, ..: K threads share a column's
+                // dims where there are that many, and meet in LDS
+                const int lanes = p.cols * Q4, share = lanes >= 256 ? 1 : 256 / lanes;
+                for (int e0 = 0; e0 < lanes; e0 += 256) {
+                    const int e = share > 1 ? t % lanes : e0 + t, k = share > 1 ? t / lanes : 0;
                     const int c = e / Q4, d = 4 * (e % Q4);
                     float m = -INFINITY, sum = 0.f;
                     f32x4 v = {0.f, 0.f, 0.f, 0.f};
-                    for (uint32_t i = wa; i <= wb; ++i) {
-                        const float* part = slots + size_t(2 * i + (i == wa ? 1 : 0)) * SW;
-                        const float2 ml = load_agent(part + 2 * c);
-                        const float2 x = load_agent(part + 2 * paged::kRowsCols + c * HD + d);
-                        const float2 z = load_agent(part + 2 * paged::kRowsCols + c * HD + d + 2);
-                        const float mn = fmaxf(m, ml.x), mc = mn == -INFINITY ? 0.f : mn * a.scale_log2;
-                        const float fo = __builtin_amdgcn_exp2f(m * a.scale_log2 - mc);
-                        const float fn = __builtin_amdgcn_exp2f(ml.x * a.scale_log2 - mc);
-                        sum = sum * fo + ml.y * fn;
-                        v = v * fo + f32x4{x.x, x.y, z.x, z.y} * fn;
-                        m = mn;
+                    if (e < lanes && k < share) {
+                        constexpr int PF = 4;
+                        for (uint32_t i = wa + k; i <= wb; i += PF * share) {
+                            float2 ml[PF];
+                            f32x4 x[PF];
+#pragma unroll
+                            for (int q = 0; q < PF; ++q) {
+                                const uint32_t part = min(i + q * share, wb);
+                                const int at = slot_at(part, part == wa);
+                                ml[q] = load_part2(ws, at + 2 * c);
+                                x[q] = load_part(ws, at + 2 * int(paged::kRowsCols) + c * HD + d);
+                            }
+#pragma unroll
+                            for (int q = 0; q < PF; ++q) {
+                                if (i + q * share > wb) continue;
+                                add_part(m, sum, v, ml[q].x, ml[q].y, x[q]);
+                            }
+                        }
                     }
-                    const float inv = sum != 0.f ? 1.0f / sum : 0.f;
-                    const int row = p.row0 + c / group, head = p.h * group + c % group;
-                    T* y = static_cast<T*>(a.y) + (size_t(row) * a.qh + head) * HD + d;
-                    *reinterpret_cast<uint2*>(y) =
-                        make_uint2(pack<T>(v[0] * inv, v[1] * inv), pack<T>(v[2] * inv, v[3] * inv));
+                    if (share > 1) {
+                        float* const mine = xo + t * 8;
+                        *reinterpret_cast<f32x4*>(mine) = v;
+                        mine[4] = m, mine[5] = sum;
+                        lds_barrier();
+                        if (t < lanes)
+                            for (int j = 1; j < share; ++j) {
+                                const float* other = xo + (t + j * lanes) * 8;
+                                add_part(m, sum, v, other[4], other[5], *reinterpret_cast<const f32x4*>(other));
+                            }
+                    }
+                    if (e < lanes && k == 0) {
+                        const float inv = sum != 0.f ? 1.0f / sum : 0.f;
+                        const int row = p.row0 + c / group, head = p.h * group + c % group;
+                        T* y = static_cast<T*>(a.y) + (size_t(row) * a.qh + head) * HD + d;
+                        *reinterpret_cast<uint2*>(y) =
+                            make_uint2(pack<T>(v[0] * inv, v[1] * inv), pack<T>(v[2] * inv, v[3] * inv));
+                    }
                 }
                 if (t == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             }
@@ -773,8 +814,10 @@ __global__ __launch_bounds__(256, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
         }
         tile = uniform(lo), kfirst = uniform(int(in - first_units(rq, lo)));
     }
-    float* const slots = reinterpret_cast<float*>(a.ws + paged::kGroups);
     constexpr int SW = int(paged::slot_words(paged::kTileCols, HD));
+    const __amdgpu_buffer_rsrc_t ws = __builtin_amdgcn_make_buffer_rsrc(
+        a.ws, 0, int(4 * (paged::kGroups + 2 * paged::kTileGroups * SW)), 0x00020000);
+    auto slot_at = [&](uint32_t i, bool begins) { return int(paged::kGroups) + int(2 * i + (begins ? 1 : 0)) * SW; };
 
     for (uint32_t u = u0; u < u1;) {
         // ---- a piece: blocks j0 .. j0 + nb - 1 of a tile
@@ -980,18 +1023,19 @@ __global__ __launch_bounds__(256, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
         load_v(s1);
         page_ids(1);
         locate(1, s1, b1);
+        u32x4 r1[LPB];  // K(1), beside K(0)
+#pragma unroll
+        for (int i = 0; i < LPB; ++i) r1[i] = __builtin_amdgcn_raw_buffer_load_b128(k_rsrc, 16 * lane + 1024 * i, s1, 0);
+        page_ids(2);
+        locate(2, s2, b2);
         lds_barrier();  // the blocks of the piece before this one are read
         store_k(0);
         store_v(0, 0, b0);
-        if (nb > 1) load_k(s1);
-        page_ids(2);
-        locate(2, s2, b2);
-        if (nb > 1) {
-            store_k(1);
-            load_v(s1);
-        }
-        if (nb > 2) load_k(s2);
+        load_k(s2);
+        load_v(s1);
         page_ids(3);
+#pragma unroll
+        for (int i = 0; i < LPB; ++i) *reinterpret_cast<u32x4*>(lds + BLK + kst[i]) = r1[i];
         s3 = s2, b3 = b2;
         lds_barrier();
         float mx[2];
@@ -1052,19 +1096,19 @@ __global__ __launch_bounds__(256, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
         } else {
             const uint32_t wa = group_of(begin), wb = group_of(end - 1);
             // column tile x, 16 bytes i of lane l: ((2 wave + x) 4 DT + i) 64 + l, after the maxima and sums
-            auto at = [&](float* slot, int ct, int i) {
-                return slot + 2 * paged::kTileCols + (((2 * wv + ct) * 4 * DT + i) * 64 + lane) * 4;
+            auto at = [&](int slot, int ct, int i) {
+                return slot + 2 * int(paged::kTileCols) + (((2 * wv + ct) * 4 * DT + i) * 64 + lane) * 4;
             };
             if (cw < cols) {
-                float* mine = slots + size_t(2 * w + (begin >= u0 ? 1 : 0)) * SW;
+                const int mine = slot_at(w, begin >= u0);
 #pragma unroll
                 for (int ct = 0; ct < 2; ++ct) {
-                    if (h == 0) store_agent(mine + 2 * (cw + 32 * ct + c32), m_run[ct], l_run[ct]);
+                    if (h == 0) store_part2(ws, mine + 2 * (cw + 32 * ct + c32), m_run[ct], l_run[ct]);
 #pragma unroll
                     for (int i = 0; i < 4 * DT; ++i) {
                         const f32x16& x = o[ct][i >> 2];
-                        store_agent(at(mine, ct, i), x[4 * (i & 3)], x[4 * (i & 3) + 1]);
-                        store_agent(at(mine, ct, i) + 2, x[4 * (i & 3) + 2], x[4 * (i & 3) + 3]);
+                        const int e = 4 * (i & 3);
+                        store_part(ws, at(mine, ct, i), f32x4{x[e], x[e + 1], x[e + 2], x[e + 3]});
                     }
                 }
             }
@@ -1084,23 +1128,30 @@ __global__ __launch_bounds__(256, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
                             for (int e = 0; e < 16; ++e) o[ct][d][e] = 0.f;
                     }
                     for (uint32_t i = wa; i <= wb; ++i) {
-                        float* part = slots + size_t(2 * i + (i == wa ? 1 : 0)) * SW;
+                        const int part = slot_at(i, i == wa);
+                        float2 ml[2];
+                        f32x4 x[2][4 * DT];
 #pragma unroll
                         for (int ct = 0; ct < 2; ++ct) {
-                            const float2 ml = load_agent(part + 2 * (cw + 32 * ct + c32));
-                            const float mn = fmaxf(m_run[ct], ml.x), mc = mn == -INFINITY ? 0.f : mn * a.scale_log2;
+                            ml[ct] = load_part2(ws, part + 2 * (cw + 32 * ct + c32));
+#pragma unroll
+                            for (int j = 0; j < 4 * DT; ++j) x[ct][j] = load_part(ws, at(part, ct, j));
+                        }
+                        __builtin_amdgcn_sched_barrier(0);  // (all under way before the first is waited for)
+#pragma unroll
+                        for (int ct = 0; ct < 2; ++ct) {
+                            const float mn = fmaxf(m_run[ct], ml[ct].x), mc = mn == -INFINITY ? 0.f : mn * a.scale_log2;
                             const float fo = __builtin_amdgcn_exp2f(m_run[ct] * a.scale_log2 - mc);
-                            const float fn = __builtin_amdgcn_exp2f(ml.x * a.scale_log2 - mc);
-                            l_run[ct] = l_run[ct] * fo + ml.y * fn;
+                            const float fn = __builtin_amdgcn_exp2f(ml[ct].x * a.scale_log2 - mc);
+                            l_run[ct] = l_run[ct] * fo + ml[ct].y * fn;
                             m_run[ct] = mn;
 #pragma unroll
-                            for (int j = 0; j < 4 * DT; ++j) {
-                                const float2 x = load_agent(at(part, ct, j)), z = load_agent(at(part, ct, j) + 2);
-                                f32x16& v = o[ct][j >> 2];
-                                const int e = 4 * (j & 3);
-                                v[e] = v[e] * fo + x.x * fn, v[e + 1] = v[e + 1] * fo + x.y * fn;
-                                v[e + 2] = v[e + 2] * fo + z.x * fn, v[e + 3] = v[e + 3] * fo + z.y * fn;
-                            }
+                            for (int j = 0; j < 4 * DT; ++j)
+#pragma unroll
+                                for (int q = 0; q < 4; ++q) {
+                                    const int e = 4 * (j & 3) + q;
+                                    o[ct][j >> 2][e] = o[ct][j >> 2][e] * fo + x[ct][j][q] * fn;
+                                }
                         }
                     }
                     write();
