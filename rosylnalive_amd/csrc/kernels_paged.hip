@@ -726,9 +726,8 @@ __device__ __forceinline__ uint32_t floor_sum64(uint32_t n, uint32_t step, uint3
 // Rows of many query columns, on 32 x 32 x 16 tiles. A tile of an item is up to 256 columns (whole rows of the request: 256 /
 // group of them), 64 per wave as two column tiles, so that each K and V operand read from LDS feeds two matrix
 // instructions (one instruction per read would take all of LDS's bandwidth). K and V blocks of 64 keys go from the pages
-// through registers into LDS (three K blocks, two V blocks), loaded a step before they are stored; one barrier per block. K rows hold their 16-byte
-// chunks in an order that depends on the row, so the 16 rows that a read phase takes lie in different banks; V's layout in
-// the cache is already the order in which it is read.
+// through registers into LDS (three K blocks, two V blocks), loaded a step before they are stored; one barrier per block.
+// V's layout in the cache is already the order in which it is read.
 // Step n: the scores of block n + 1 (matrix core) under the exponentials of block n (VALU), then block n's products
 // under the maxima of block n + 1. The rows of S^T's tiles hold the keys in the order in which P^T wants them (bits 2 and 3
 // of the row exchanged), so weights never cross lanes.
@@ -736,9 +735,10 @@ template <typename T, int HD>
 __global__ __launch_bounds__(256, 1) void k_attn_tiles(AttnArgs a, uint32_t bytes) {
     using M = Mfma<T>;
     constexpr int KB = int(paged::kTileKeys), KS = HD / 16, DT = HD / 32, RB = HD * 2, BLK = KB * RB;
+    constexpr int KR = RB + 16, KBLK = KB * KR;  // a K row in LDS is padded by 16 bytes: 16 rows lie in different banks
     constexpr int CH = RB / 16;            // 16-byte chunks of a K row
     constexpr int LPB = BLK / 4096;        // loads of a block per wave and of 1 KB each: 16 keys
-    __shared__ __attribute__((aligned(16))) uint8_t lds[5 * BLK];  // K blocks n % 3, then V blocks n % 2
+    __shared__ __attribute__((aligned(16))) uint8_t lds[3 * KBLK + 2 * BLK];  // K blocks n % 3, then V blocks n % 2
     __shared__ uint32_t ends[paged::kMaxRequests];
     __shared__ uint32_t red[4];
     __shared__ uint32_t arrived;
@@ -787,12 +787,11 @@ __global__ __launch_bounds__(256, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
 #pragma unroll
     for (int i = 0; i < LPB; ++i) {
         const int p = 64 * i + lane, row = p / CH, ch = p % CH;  // row of the wave's 16, place in the row
-        kst[i] = (16 * wv + row) * RB + (ch ^ (HD == 128 ? row & 15 : (row >> 1) & 7)) * 16;
+        kst[i] = (16 * wv + row) * KR + ch * 16;
     }
     // operand reads: K row of matrix row c32 is key 16 (c32 / 16) + 8 (c32 / 4 % 2) + 4 (c32 / 8 % 2) + c32 % 4
     const int krow = (c32 & 19) | ((c32 & 4) << 1) | ((c32 & 8) >> 1);
-    const int kswz = (h ^ (HD == 128 ? krow & 15 : (krow >> 1) & 7)) * 16;
-    const int kbase = krow * RB + kswz, vbase = 3 * BLK + h * (8 * RB) + c32 * 16;
+    const int kbase = krow * KR + 16 * h, vbase = 3 * KBLK + h * (8 * RB) + c32 * 16;
 
     Request rq{};
     int r = uniform(first_above(ends, int(a.requests), u0));
@@ -844,22 +843,24 @@ __global__ __launch_bounds__(256, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
                         static_cast<const T*>(a.q) + (size_t(rq.row0 + row) * a.qh + head) * HD + 16 * s + 8 * h);
             }
         }
-        const const_words trow = const_words(a.table) + size_t(r) * a.blocks;
-        // the pages of block j's four 16-key parts (scalar loads, a step before their use); then its place in the caches for
-        // this wave's 16 keys, and the set of the parts that have none
-        uint32_t ids[4];
+        const uint32_t* const trow = a.table + size_t(r) * a.blocks;
+        // the pages of 16 blocks at a time, lane 4 i + p those of part p (16 keys) of block i: its place in the caches for
+        // this wave's part is a lane read, the set of parts without a page four bits of a ballot
         auto page_ids = [&](int j) __attribute__((always_inline)) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                ids[i] = trow[min(uint32_t((j0 + j) * KB + 16 * i) >> a.page_log2, a.blocks - 1)];
+            return trow[min(uint32_t((j0 + j) * KB + 16 * lane) >> a.page_log2, a.blocks - 1)];
         };
+        uint32_t ids = page_ids(0), ids_next = ids;
+        uint64_t no_page = __ballot(ids >= a.pages);
         auto locate = [&](int j, int& soff, uint32_t& bad) __attribute__((always_inline)) {
-            bad = 0;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) bad |= uint32_t(ids[i] >= a.pages) << i;
-            const uint32_t mine = wv == 0 ? ids[0] : wv == 1 ? ids[1] : wv == 2 ? ids[2] : ids[3];
+            if ((j & 15) == 8) ids_next = page_ids((j & ~15) + 16);
+            if ((j & 15) == 0 && j) {
+                ids = ids_next;
+                no_page = __ballot(ids >= a.pages);
+            }
+            bad = uint32_t(no_page >> (4 * (j & 15))) & 15u;
+            const uint32_t id = uint32_t(__builtin_amdgcn_readlane(int(ids), 4 * (j & 15) + wv));
             const uint32_t off = uint32_t((j0 + j) * KB + 16 * wv) & ((1u << a.page_log2) - 1);
-            soff = mine < a.pages ? int((((mine * uint32_t(kvh) + hk) << a.page_log2) + off) * RB) : 0;
+            soff = id < a.pages ? int((((id * uint32_t(kvh) + hk) << a.page_log2) + off) * RB) : 0;
         };
         u32x4 rk[LPB], rv[LPB];
         auto load_k = [&](int soff) __attribute__((always_inline)) {
@@ -872,9 +873,9 @@ __global__ __launch_bounds__(256, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
         };
         auto store_k = [&](int slot) __attribute__((always_inline)) {
 #pragma unroll
-            for (int i = 0; i < LPB; ++i) *reinterpret_cast<u32x4*>(lds + slot * BLK + kst[i]) = rk[i];
+            for (int i = 0; i < LPB; ++i) *reinterpret_cast<u32x4*>(lds + slot * KBLK + kst[i]) = rk[i];
         };
-        auto store_v = [&](int slot, int j, uint32_t bad) __attribute__((always_inline)) {
+        auto hide_v = [&](int j, uint32_t bad) __attribute__((always_inline)) {
             const int left = keys - (j0 + j) * KB;  // keys of the block that any column sees
             if (left < KB || bad) {  // uniform: what is hidden may be anything, and zero times NaN is NaN
 #pragma unroll
@@ -885,29 +886,29 @@ __global__ __launch_bounds__(256, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
                         rv[i][e] &= (2 * e < in ? 0x0000FFFFu : 0u) | (2 * e + 1 < in ? 0xFFFF0000u : 0u);
                 }
             }
-#pragma unroll
-            for (int i = 0; i < LPB; ++i)
-                *reinterpret_cast<u32x4*>(lds + (3 + slot) * BLK + 1024 * (LPB * wv + i) + 16 * lane) = rv[i];
+        };
+        auto store_v = [&](int slot, int i) __attribute__((always_inline)) {
+            *reinterpret_cast<u32x4*>(lds + 3 * KBLK + slot * BLK + 1024 * (LPB * wv + i) + 16 * lane) = rv[i];
         };
         f32x16 sa[2], sb[2], o[2][DT];  // scores of a block's first and last 32 keys, [column tile]; [column tile][dim tile]
-        float m_run[2], l_run[2];
+        float m_run[2], mc[2], l_run[2];  // reference maxima, the same in the exponent (0 while there is none), sums
 #pragma unroll
         for (int ct = 0; ct < 2; ++ct) {
-            m_run[ct] = -INFINITY, l_run[ct] = 0.f;
+            m_run[ct] = -INFINITY, mc[ct] = l_run[ct] = 0.f;
 #pragma unroll
             for (int d = 0; d < DT; ++d)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) o[ct][d][e] = 0.f;
         }
         auto scores = [&](int slot, int kt, f32x16(&out)[2]) __attribute__((always_inline)) {
-            const uint8_t* k0 = lds + slot * BLK + kt * 32 * RB;
+            const uint8_t* k0 = lds + slot * KBLK + kt * 32 * KR + kbase;
 #pragma unroll
             for (int ct = 0; ct < 2; ++ct)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) out[ct][e] = 0.f;
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
-                const u32x4 k = *reinterpret_cast<const u32x4*>(k0 + (kbase ^ (32 * s)));
+                const u32x4 k = *reinterpret_cast<const u32x4*>(k0 + 32 * s);
                 out[0] = M::m32(k, qf[0][s], out[0]);
                 out[1] = M::m32(k, qf[1][s], out[1]);
             }
@@ -925,7 +926,10 @@ __global__ __launch_bounds__(256, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
         // hides what the columns do not see of the 32 keys, and moves the reference maxima where they are left behind
         auto settle = [&](int j, int kt, uint32_t bad, f32x16(&s)[2], float(&mx)[2]) __attribute__((always_inline)) {
             const int kb = (j0 + j) * KB + 32 * kt;
-            if (kb + 32 > wave_seen || bad) {  // uniform
+            if (j >= nbw) {  // behind the last block: nothing to see (a branch around all of this instead would have the
+                             // compiler move the products' registers on either way)
+                mx[0] = mx[1] = -INFINITY;
+            } else if (kb + 32 > wave_seen || bad) {  // uniform
 #pragma unroll
                 for (int ct = 0; ct < 2; ++ct) {
                     const int lim = vis[ct] - kb - 8 * h;
@@ -943,6 +947,7 @@ __global__ __launch_bounds__(256, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
                 for (int ct = 0; ct < 2; ++ct) {
                     const float alpha = grow[ct] ? __builtin_amdgcn_exp2f((m_run[ct] - mx[ct]) * a.scale_log2) : 1.0f;
                     m_run[ct] = grow[ct] ? mx[ct] : m_run[ct];
+                    mc[ct] = m_run[ct] == -INFINITY ? 0.f : m_run[ct] * a.scale_log2;
                     l_run[ct] *= alpha;
 #pragma unroll
                     for (int d = 0; d < DT; ++d) o[ct][d] *= alpha;
@@ -950,61 +955,69 @@ __global__ __launch_bounds__(256, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
             }
         };
         // 32 keys: the scores of the next 32 (matrix core) under the weights of these (VALU), then their products under the
-        // next ones' maxima, two matrix instructions and their share of the VALU's work at a time: the scheduling barriers
-        // keep that order (without them all the instructions of one kind follow each other, and either unit waits for the
-        // other), with each operand read two pairs ahead.
-        auto half = [&](int kslot, int nkt, f32x16(&nxt)[2], int vslot, int kt, f32x16(&cur)[2],
-                        float(&mx)[2]) __attribute__((always_inline)) {
-            const uint8_t* k0 = lds + kslot * BLK + nkt * 32 * RB;
+        // last of the weights and the next ones' maxima, two matrix instructions and their share of the VALU's work at a time:
+        // the scheduling barriers keep that order (without them all the instructions of one kind follow each other, and
+        // either unit waits for the other), with each operand read two pairs ahead.
+        u32x4 kp[2];  // the first two operands of the next scores, read under the products before them
+        auto half = [&](int kslot, int nkt, f32x16(&nxt)[2], int vslot, int kt, f32x16(&cur)[2], float(&mx)[2], int pslot,
+                        int pkt, auto&& side) __attribute__((always_inline)) {
+            const uint8_t* k0 = lds + kslot * KBLK + nkt * 32 * KR + kbase;
+            const uint8_t* p0 = lds + pslot * KBLK + pkt * 32 * KR + kbase;
             const uint8_t* v0 = lds + vslot * BLK + vbase + kt * 32 * RB;
-            auto read_k = [&](int s) __attribute__((always_inline)) {
-                return *reinterpret_cast<const u32x4*>(k0 + (kbase ^ (32 * s)));
-            };
+            auto read_k = [&](int s) __attribute__((always_inline)) { return *reinterpret_cast<const u32x4*>(k0 + 32 * s); };
             auto read_v = [&](int i) __attribute__((always_inline)) {
                 return *reinterpret_cast<const u32x4*>(v0 + (i / DT) * 16 * RB + (i % DT) * 512);
             };
-            constexpr int NV = 2 * DT, PER = 16 / KS;  // products' pairs; weights of a column tile per pair of scores
+            constexpr int NV = 2 * DT;
             u32x4 kf[KS], vf[NV], pb[2][2];  // (pb: weights packed as the products' operands, [column tile][16 keys])
-            float mc[2];
+            // two weights of a column: pair p of 16 in the order in which the products need them
+            auto weigh = [&](int p) __attribute__((always_inline)) {
+                const int ks = p / 8, ct = p / 4 % 2, i = p % 4, e = 8 * ks + 2 * i;
+                const float x = __builtin_amdgcn_exp2f(fmaf(cur[ct][e], a.scale_log2, -mc[ct]));
+                const float y = __builtin_amdgcn_exp2f(fmaf(cur[ct][e + 1], a.scale_log2, -mc[ct]));
+                l_run[ct] += x;
+                l_run[ct] += y;
+                pb[ct][ks][i] = pack<T>(x, y);
+                asm volatile("" : "+v"(l_run[ct]));  // (the sums stay here)
+            };
+            constexpr int EARLY = 12;  // pairs under the scores; the other four under the first products
 #pragma unroll
-            for (int ct = 0; ct < 2; ++ct) {
-                mc[ct] = m_run[ct] == -INFINITY ? 0.f : m_run[ct] * a.scale_log2;
+            for (int ct = 0; ct < 2; ++ct)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) nxt[ct][e] = 0.f;
-            }
-            kf[0] = read_k(0), kf[1] = read_k(1);
+            kf[0] = kp[0], kf[1] = kp[1];
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
                 if (s + 2 < KS) kf[s + 2] = read_k(s + 2);
                 if (s + 2 >= KS) vf[s + 2 - KS] = read_v(s + 2 - KS);
+                side(s, KS + NV);
                 nxt[0] = M::m32(kf[s], qf[0][s], nxt[0]);
                 nxt[1] = M::m32(kf[s], qf[1][s], nxt[1]);
 #pragma unroll
-                for (int ct = 0; ct < 2; ++ct) {
-#pragma unroll
-                    for (int e = PER * s; e < PER * (s + 1); ++e) {
-                        cur[ct][e] = __builtin_amdgcn_exp2f(fmaf(cur[ct][e], a.scale_log2, -mc[ct]));
-                        l_run[ct] += cur[ct][e];
-                    }
-#pragma unroll
-                    for (int e = PER * s; e < PER * (s + 1); e += 2)
-                        pb[ct][e >> 3][(e & 7) >> 1] = pack<T>(cur[ct][e], cur[ct][e + 1]);
-                    asm volatile("" : "+v"(l_run[ct]));
-                }
+                for (int p = EARLY * s / KS; p < EARLY * (s + 1) / KS; ++p) weigh(p);
                 __builtin_amdgcn_sched_barrier(0);
             }
-            constexpr int PM = 16 / NV;
             float m[2] = {-INFINITY, -INFINITY};
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 if (i + 2 < NV) vf[i + 2] = read_v(i + 2);
+                if (i + 2 >= NV) kp[i + 2 - NV] = *reinterpret_cast<const u32x4*>(p0 + 32 * (i + 2 - NV));
+                side(KS + i, KS + NV);
                 o[0][i % DT] = M::m32(vf[i], pb[0][i / DT], o[0][i % DT]);
                 o[1][i % DT] = M::m32(vf[i], pb[1][i / DT], o[1][i % DT]);
+                if (i < DT)
 #pragma unroll
-                for (int ct = 0; ct < 2; ++ct)
+                    for (int p = EARLY + 4 * i / DT; p < EARLY + 4 * (i + 1) / DT; ++p) weigh(p);
 #pragma unroll
-                    for (int e = PM * i; e < PM * (i + 1); e += 2) m[ct] = fmaxf(fmaxf(m[ct], nxt[ct][e]), nxt[ct][e + 1]);
+                for (int ct = 0; ct < 2; ++ct)  // (the last scores are two pairs of products old)
+#pragma unroll
+                    for (int p = i < 2 ? 0 : 8 * (i - 2) / (NV - 2); i >= 2 && p < 8 * (i - 1) / (NV - 2); ++p) {
+                        float x = nxt[ct][2 * p], y = nxt[ct][2 * p + 1];
+                        asm volatile("" : "+v"(x), "+v"(y));  // from here on in registers that the VALU reads
+                        m[ct] = fmaxf(fmaxf(m[ct], x), y);
+                        nxt[ct][2 * p] = x, nxt[ct][2 * p + 1] = y;
+                    }
                 __builtin_amdgcn_sched_barrier(0);
             }
 #pragma unroll
@@ -1014,55 +1027,62 @@ __global__ __launch_bounds__(256, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
             }
         };
 
-        // Step n stores K(n + 2) and V(n + 1), loaded by step n - 1, and loads K(n + 3) and V(n + 2).
+        // Step n stores K(n + 2) and V(n + 1), loaded by step n - 1, under its second half, and loads K(n + 3) and V(n + 2) into
+        // the registers that this frees (behind the last block: the last one again, never read).
         int s1, s2, s3;
         uint32_t b0, b1, b2, b3;
-        page_ids(0);
         locate(0, s1, b0);
         load_k(s1);
         load_v(s1);
-        page_ids(1);
-        locate(1, s1, b1);
+        locate(min(1, nb - 1), s1, b1);
         u32x4 r1[LPB];  // K(1), beside K(0)
 #pragma unroll
         for (int i = 0; i < LPB; ++i) r1[i] = __builtin_amdgcn_raw_buffer_load_b128(k_rsrc, 16 * lane + 1024 * i, s1, 0);
-        page_ids(2);
-        locate(2, s2, b2);
+        locate(min(2, nb - 1), s2, b2);
         lds_barrier();  // the blocks of the piece before this one are read
         store_k(0);
-        store_v(0, 0, b0);
+        hide_v(0, b0);
+#pragma unroll
+        for (int i = 0; i < LPB; ++i) store_v(0, i);
         load_k(s2);
         load_v(s1);
-        page_ids(3);
 #pragma unroll
-        for (int i = 0; i < LPB; ++i) *reinterpret_cast<u32x4*>(lds + BLK + kst[i]) = r1[i];
-        s3 = s2, b3 = b2;
+        for (int i = 0; i < LPB; ++i) *reinterpret_cast<u32x4*>(lds + KBLK + kst[i]) = r1[i];
         lds_barrier();
         float mx[2];
         if (nbw > 0) {
             scores(0, 0, sa);
             maxima(sa, mx);
             settle(0, 0, b0, sa, mx);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) kp[i] = *reinterpret_cast<const u32x4*>(lds + 32 * KR + kbase + 32 * i);
         }
         int kslot = 0;  // n % 3
         for (int n = 0; n < nb; ++n) {
             const int kslot1 = kslot == 2 ? 0 : kslot + 1, kslot2 = kslot1 == 2 ? 0 : kslot1 + 1;
             if (n) lds_barrier();
-            if (n + 1 < nb) {
-                if (n + 2 < nb) store_k(kslot2);
-                store_v((n + 1) & 1, n + 1, b1);
-                if (n + 3 < nb) {
-                    locate(n + 3, s3, b3);
-                    load_k(s3);
-                    page_ids(n + 4);
+            s3 = s2, b3 = b2;
+            if (n + 3 < nb) locate(n + 3, s3, b3);
+            if (n + 1 < nb) hide_v(n + 1, b1);
+            const int vslot = n & 1, vslot1 = 1 - vslot;
+            // one store or load of a K or V chunk: 4 LPB of them shared out over the parts of a half
+            auto move = [&](int part, int parts) __attribute__((always_inline)) {
+#pragma unroll
+                for (int x = 4 * LPB * part / parts; x < 4 * LPB * (part + 1) / parts; ++x) {
+                    const int i = x >> 2;
+                    if ((x & 3) == 0) *reinterpret_cast<u32x4*>(lds + kslot2 * KBLK + kst[i]) = rk[i];
+                    if ((x & 3) == 1) rk[i] = __builtin_amdgcn_raw_buffer_load_b128(k_rsrc, 16 * lane + 1024 * i, s3, 0);
+                    if ((x & 3) == 2) store_v(vslot1, i);
+                    if ((x & 3) == 3) rv[i] = __builtin_amdgcn_raw_buffer_load_b128(v_rsrc, 16 * lane + 1024 * i, s2, 0);
                 }
-                if (n + 2 < nb) load_v(s2);
-            }
+            };
             if (n < nbw) {
-                half(kslot, 1, sb, n & 1, 0, sa, mx);
+                half(kslot, 1, sb, vslot, 0, sa, mx, kslot1, 0, [](int, int) {});
                 settle(n, 1, b0, sb, mx);
-                half(kslot1, 0, sa, n & 1, 1, sb, mx);  // (scores behind the last block: not used)
-                if (n + 1 < nbw) settle(n + 1, 0, b1, sa, mx);
+                half(kslot1, 0, sa, vslot, 1, sb, mx, kslot1, 1, move);  // (scores behind the last block: not used)
+                settle(n + 1, 0, b1, sa, mx);
+            } else {
+                move(0, 1);
             }
             s2 = s3, b0 = b1, b1 = b2, b2 = b3, kslot = kslot1;
         }
