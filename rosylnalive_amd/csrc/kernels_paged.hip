@@ -28,7 +28,7 @@ __device__ __forceinline__ uint32_t add_sat(uint32_t a, uint32_t b) {
     return s < a ? 0xFFFFFFFFu : s;
 }
 
-// The inclusive scan of v over the workgroup's 256 threads; red: 4 words of LDS, free again after the next barrier.
+// The inclusive scan of v over the workgroup's threads; red: a word of LDS per wave, free again after the next barrier.
 __device__ __forceinline__ uint32_t scan_sat(uint32_t v, uint32_t* red) {
     const int t = threadIdx.x, lane = t & 63, wv = t >> 6;
 #pragma unroll
@@ -724,23 +724,23 @@ __device__ __forceinline__ uint32_t floor_sum64(uint32_t n, uint32_t step, uint3
 }
 
 // Rows of many query columns, on 32 x 32 x 16 tiles. A tile of an item is up to 256 columns (whole rows of the request: 256 /
-// group of them), 64 per wave as two column tiles, so that each K and V operand read from LDS feeds two matrix
-// instructions (one instruction per read would take all of LDS's bandwidth). K and V blocks of 64 keys go from the pages
+// group of them), 32 per wave, eight waves: two per SIMD, so that one's VALU work runs beside the other's matrix
+// instructions. K and V blocks of 64 keys go from the pages
 // through registers into LDS (three K blocks, two V blocks), loaded a step before they are stored; one barrier per block.
 // V's layout in the cache is already the order in which it is read.
 // Step n: the scores of block n + 1 (matrix core) under the exponentials of block n (VALU), then block n's products
 // under the maxima of block n + 1. The rows of S^T's tiles hold the keys in the order in which P^T wants them (bits 2 and 3
 // of the row exchanged), so weights never cross lanes.
 template <typename T, int HD>
-__global__ __launch_bounds__(256, 1) void k_attn_tiles(AttnArgs a, uint32_t bytes) {
+__global__ __launch_bounds__(512, 1) void k_attn_tiles(AttnArgs a, uint32_t bytes) {
     using M = Mfma<T>;
     constexpr int KB = int(paged::kTileKeys), KS = HD / 16, DT = HD / 32, RB = HD * 2, BLK = KB * RB;
     constexpr int KR = RB + 16, KBLK = KB * KR;  // a K row in LDS is padded by 16 bytes: 16 rows lie in different banks
     constexpr int CH = RB / 16;            // 16-byte chunks of a K row
-    constexpr int LPB = BLK / 4096;        // loads of a block per wave and of 1 KB each: 16 keys
+    constexpr int LPB = BLK / 8192;        // loads of a block per wave and of 1 KB each: 8 keys
     __shared__ __attribute__((aligned(16))) uint8_t lds[3 * KBLK + 2 * BLK];  // K blocks n % 3, then V blocks n % 2
     __shared__ uint32_t ends[paged::kMaxRequests];
-    __shared__ uint32_t red[4];
+    __shared__ uint32_t red[8];
     __shared__ uint32_t arrived;
     const int t = threadIdx.x, lane = t & 63, wv = uniform(t >> 6), c32 = lane & 31, h = lane >> 5;
     const int group = int(a.qh / a.kvh), kvh = int(a.kvh), TR = int(paged::kTileCols) / group;
@@ -761,7 +761,7 @@ __global__ __launch_bounds__(256, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
     };
     auto tiles_of = [&](const Request& q) { return (q.rows + TR - 1) / TR; };
     {
-        const uint32_t per = (a.requests + 255) / 256, r0 = min(t * per, a.requests), r1 = min(r0 + per, a.requests);
+        const uint32_t per = (a.requests + 511) / 512, r0 = min(t * per, a.requests), r1 = min(r0 + per, a.requests);
         uint32_t sum = 0;
         for (uint32_t r = r0; r < r1; ++r) {
             const Request q = request_of(a, r);
@@ -782,12 +782,12 @@ __global__ __launch_bounds__(256, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
 
     const __amdgpu_buffer_rsrc_t k_rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(a.kc), 0, bytes, 0x00020000);
     const __amdgpu_buffer_rsrc_t v_rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(a.vc), 0, bytes, 0x00020000);
-    // this wave moves keys 16 wv .. + 15 of a block, 16 bytes per lane and load: both caches hold them in one piece
+    // this wave moves keys 8 wv .. + 7 of a block, 16 bytes per lane and load: both caches hold them in one piece
     int kst[LPB];  // where a K chunk goes in its block
 #pragma unroll
     for (int i = 0; i < LPB; ++i) {
-        const int p = 64 * i + lane, row = p / CH, ch = p % CH;  // row of the wave's 16, place in the row
-        kst[i] = (16 * wv + row) * KR + ch * 16;
+        const int p = 64 * i + lane, row = p / CH, ch = p % CH;  // row of the wave's 8, place in the row
+        kst[i] = (8 * wv + row) * KR + ch * 16;
     }
     // operand reads: K row of matrix row c32 is key 16 (c32 / 16) + 8 (c32 / 4 % 2) + 4 (c32 / 8 % 2) + c32 % 4
     const int krow = (c32 & 19) | ((c32 & 4) << 1) | ((c32 & 8) >> 1);
@@ -823,25 +823,21 @@ __global__ __launch_bounds__(256, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
         const int units = tile_units(rq, tile), keys = tile_keys(rq, tile), j0 = kfirst;
         const int nb = min(units - j0, int(u1 - u));
         const int row_first = tile * TR, cols = min(TR, rq.rows - row_first) * group;
-        const int cw = 64 * wv;  // this wave's first column
+        const int cw = 32 * wv;  // this wave's first column
         // blocks that some column of the wave sees
         int nbw = 0;
-        if (cw < cols) nbw = (max(0, rq.seen + row_first + min(cw + 63, cols - 1) / group) + KB - 1) / KB - j0;
+        if (cw < cols) nbw = (max(0, rq.seen + row_first + min(cw + 31, cols - 1) / group) + KB - 1) / KB - j0;
         nbw = uniform(min(max(nbw, 0), nb));
         const int wave_seen = uniform(rq.seen + row_first + cw / group);  // keys that the wave's first column sees
-        int vis[2];  // keys that this lane's columns see
-        u32x4 qf[2][KS];
+        const int mycol = cw + c32, myrow = row_first + mycol / group, myhead = hk * group + mycol % group;
+        const int vis = rq.seen + myrow;  // keys that this lane's column sees
+        u32x4 qf[KS];
 #pragma unroll
-        for (int ct = 0; ct < 2; ++ct) {
-            const int c = cw + 32 * ct + c32, row = row_first + c / group, head = hk * group + c % group;
-            vis[ct] = rq.seen + row;
-#pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                qf[ct][s] = u32x4{0u, 0u, 0u, 0u};
-                if (c < cols)
-                    qf[ct][s] = *reinterpret_cast<const u32x4*>(
-                        static_cast<const T*>(a.q) + (size_t(rq.row0 + row) * a.qh + head) * HD + 16 * s + 8 * h);
-            }
+        for (int s = 0; s < KS; ++s) {
+            qf[s] = u32x4{0u, 0u, 0u, 0u};
+            if (mycol < cols)
+                qf[s] = *reinterpret_cast<const u32x4*>(
+                    static_cast<const T*>(a.q) + (size_t(rq.row0 + myrow) * a.qh + myhead) * HD + 16 * s + 8 * h);
         }
         const uint32_t* const trow = a.table + size_t(r) * a.blocks;
         // the pages of 16 blocks at a time, lane 4 i + p those of part p (16 keys) of block i: its place in the caches for
@@ -858,8 +854,8 @@ __global__ __launch_bounds__(256, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
                 no_page = __ballot(ids >= a.pages);
             }
             bad = uint32_t(no_page >> (4 * (j & 15))) & 15u;
-            const uint32_t id = uint32_t(__builtin_amdgcn_readlane(int(ids), 4 * (j & 15) + wv));
-            const uint32_t off = uint32_t((j0 + j) * KB + 16 * wv) & ((1u << a.page_log2) - 1);
+            const uint32_t id = uint32_t(__builtin_amdgcn_readlane(int(ids), 4 * (j & 15) + (wv >> 1)));
+            const uint32_t off = uint32_t((j0 + j) * KB + 8 * wv) & ((1u << a.page_log2) - 1);
             soff = id < a.pages ? int((((id * uint32_t(kvh) + hk) << a.page_log2) + off) * RB) : 0;
         };
         u32x4 rk[LPB], rv[LPB];
@@ -880,7 +876,7 @@ __global__ __launch_bounds__(256, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
             if (left < KB || bad) {  // uniform: what is hidden may be anything, and zero times NaN is NaN
 #pragma unroll
                 for (int i = 0; i < LPB; ++i) {
-                    const int in = (bad >> wv & 1u) ? 0 : left - 16 * wv - 8 * ((64 * i + lane) / HD);
+                    const int in = (bad >> (wv >> 1) & 1u) ? 0 : left - 8 * wv;
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
                         rv[i][e] &= (2 * e < in ? 0x0000FFFFu : 0u) | (2 * e + 1 < in ? 0xFFFF0000u : 0u);
@@ -890,77 +886,51 @@ __global__ __launch_bounds__(256, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
         auto store_v = [&](int slot, int i) __attribute__((always_inline)) {
             *reinterpret_cast<u32x4*>(lds + 3 * KBLK + slot * BLK + 1024 * (LPB * wv + i) + 16 * lane) = rv[i];
         };
-        f32x16 sa[2], sb[2], o[2][DT];  // scores of a block's first and last 32 keys, [column tile]; [column tile][dim tile]
-        float m_run[2], mc[2], l_run[2];  // reference maxima, the same in the exponent (0 while there is none), sums
+        f32x16 sa, sb, o[DT];  // scores of a block's first and last 32 keys; products, [dim tile]
+        float m_run = -INFINITY, mc = 0.f, l_run = 0.f;  // reference maximum, the same in the exponent (0: none yet), sum
 #pragma unroll
-        for (int ct = 0; ct < 2; ++ct) {
-            m_run[ct] = -INFINITY, mc[ct] = l_run[ct] = 0.f;
+        for (int d = 0; d < DT; ++d)
 #pragma unroll
-            for (int d = 0; d < DT; ++d)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) o[ct][d][e] = 0.f;
-        }
-        auto scores = [&](int slot, int kt, f32x16(&out)[2]) __attribute__((always_inline)) {
-            const uint8_t* k0 = lds + slot * KBLK + kt * 32 * KR + kbase;
-#pragma unroll
-            for (int ct = 0; ct < 2; ++ct)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) out[ct][e] = 0.f;
-#pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                const u32x4 k = *reinterpret_cast<const u32x4*>(k0 + 32 * s);
-                out[0] = M::m32(k, qf[0][s], out[0]);
-                out[1] = M::m32(k, qf[1][s], out[1]);
-            }
+            for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
+        auto join_halves = [&](float m) __attribute__((always_inline)) {  // the maximum over lanes l and l + 32
+            const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
+            return fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
         };
-        auto maxima = [&](f32x16(&s)[2], float(&mx)[2]) __attribute__((always_inline)) {
+        auto maximum = [&](f32x16& s) __attribute__((always_inline)) {
+            float m = s[0];
 #pragma unroll
-            for (int ct = 0; ct < 2; ++ct) {
-                float m = s[ct][0];
-#pragma unroll
-                for (int e = 1; e < 16; ++e) m = fmaxf(m, s[ct][e]);
-                const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
-                mx[ct] = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
-            }
+            for (int e = 1; e < 16; ++e) m = fmaxf(m, s[e]);
+            return join_halves(m);
         };
         // hides what the columns do not see of the 32 keys, and moves the reference maxima where they are left behind
-        auto settle = [&](int j, int kt, uint32_t bad, f32x16(&s)[2], float(&mx)[2]) __attribute__((always_inline)) {
+        auto settle = [&](int j, int kt, uint32_t bad, f32x16& s, float mx) __attribute__((always_inline)) {
             const int kb = (j0 + j) * KB + 32 * kt;
-            if (j >= nbw) {  // behind the last block: nothing to see (a branch around all of this instead would have the
-                             // compiler move the products' registers on either way)
-                mx[0] = mx[1] = -INFINITY;
+            if (j >= nbw) {  // behind the last block: nothing to see
+                mx = -INFINITY;
             } else if (kb + 32 > wave_seen || bad) {  // uniform
+                const int lim = vis - kb - 8 * h;
 #pragma unroll
-                for (int ct = 0; ct < 2; ++ct) {
-                    const int lim = vis[ct] - kb - 8 * h;
-#pragma unroll
-                    for (int e = 0; e < 16; ++e)
-                        if (16 * (e >> 3) + (e & 7) >= lim || (bad >> (2 * kt + (e >> 3)) & 1u)) s[ct][e] = -INFINITY;
-                }
-                maxima(s, mx);
+                for (int e = 0; e < 16; ++e)
+                    if (16 * (e >> 3) + (e & 7) >= lim || (bad >> (2 * kt + (e >> 3)) & 1u)) s[e] = -INFINITY;
+                mx = maximum(s);
             }
-            bool grow[2];
+            const bool grow = (mx - m_run) * a.scale_log2 > 8.0f;  // false for NaN (both -inf)
+            if (__any(grow)) {
+                const float alpha = grow ? __builtin_amdgcn_exp2f((m_run - mx) * a.scale_log2) : 1.0f;
+                m_run = grow ? mx : m_run;
+                mc = m_run == -INFINITY ? 0.f : m_run * a.scale_log2;
+                l_run *= alpha;
 #pragma unroll
-            for (int ct = 0; ct < 2; ++ct) grow[ct] = (mx[ct] - m_run[ct]) * a.scale_log2 > 8.0f;  // false for NaN (both -inf)
-            if (__any(grow[0] || grow[1])) {
-#pragma unroll
-                for (int ct = 0; ct < 2; ++ct) {
-                    const float alpha = grow[ct] ? __builtin_amdgcn_exp2f((m_run[ct] - mx[ct]) * a.scale_log2) : 1.0f;
-                    m_run[ct] = grow[ct] ? mx[ct] : m_run[ct];
-                    mc[ct] = m_run[ct] == -INFINITY ? 0.f : m_run[ct] * a.scale_log2;
-                    l_run[ct] *= alpha;
-#pragma unroll
-                    for (int d = 0; d < DT; ++d) o[ct][d] *= alpha;
-                }
+                for (int d = 0; d < DT; ++d) o[d] *= alpha;
             }
         };
         // 32 keys: the scores of the next 32 (matrix core) under the weights of these (VALU), then their products under the
-        // last of the weights and the next ones' maxima, two matrix instructions and their share of the VALU's work at a time:
-        // the scheduling barriers keep that order (without them all the instructions of one kind follow each other, and
-        // either unit waits for the other), with each operand read two pairs ahead.
+        // last of the weights and the next ones' maxima, a matrix instruction and its share of the VALU's work at a time: the
+        // scheduling barriers keep that order (without them all the instructions of one kind follow each other, and either
+        // unit waits for the other), with each operand read two ahead.
         u32x4 kp[2];  // the first two operands of the next scores, read under the products before them
-        auto half = [&](int kslot, int nkt, f32x16(&nxt)[2], int vslot, int kt, f32x16(&cur)[2], float(&mx)[2], int pslot,
-                        int pkt, auto&& side) __attribute__((always_inline)) {
+        auto half = [&](int kslot, int nkt, f32x16& nxt, int vslot, int kt, f32x16& cur, int pslot, int pkt,
+                        auto&& side) __attribute__((always_inline)) {
             const uint8_t* k0 = lds + kslot * KBLK + nkt * 32 * KR + kbase;
             const uint8_t* p0 = lds + pslot * KBLK + pkt * 32 * KR + kbase;
             const uint8_t* v0 = lds + vslot * BLK + vbase + kt * 32 * RB;
@@ -969,22 +939,19 @@ __global__ __launch_bounds__(256, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
                 return *reinterpret_cast<const u32x4*>(v0 + (i / DT) * 16 * RB + (i % DT) * 512);
             };
             constexpr int NV = 2 * DT;
-            u32x4 kf[KS], vf[NV], pb[2][2];  // (pb: weights packed as the products' operands, [column tile][16 keys])
-            // two weights of a column: pair p of 16 in the order in which the products need them
+            u32x4 kf[KS], vf[NV], pb[2];  // (pb: weights packed as the products' operands, [16 keys])
+            // two weights: pair p of 8
             auto weigh = [&](int p) __attribute__((always_inline)) {
-                const int ks = p / 8, ct = p / 4 % 2, i = p % 4, e = 8 * ks + 2 * i;
-                const float x = __builtin_amdgcn_exp2f(fmaf(cur[ct][e], a.scale_log2, -mc[ct]));
-                const float y = __builtin_amdgcn_exp2f(fmaf(cur[ct][e + 1], a.scale_log2, -mc[ct]));
-                l_run[ct] += x;
-                l_run[ct] += y;
-                pb[ct][ks][i] = pack<T>(x, y);
-                asm volatile("" : "+v"(l_run[ct]));  // (the sums stay here)
+                const float x = __builtin_amdgcn_exp2f(fmaf(cur[2 * p], a.scale_log2, -mc));
+                const float y = __builtin_amdgcn_exp2f(fmaf(cur[2 * p + 1], a.scale_log2, -mc));
+                l_run += x;
+                l_run += y;
+                pb[p / 4][p % 4] = pack<T>(x, y);
+                asm volatile("" : "+v"(l_run));  // (the sums stay here)
             };
-            constexpr int EARLY = 12;  // pairs under the scores; the other four under the first products
+            constexpr int EARLY = 6;  // pairs under the scores; the other two under the first products
 #pragma unroll
-            for (int ct = 0; ct < 2; ++ct)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) nxt[ct][e] = 0.f;
+            for (int e = 0; e < 16; ++e) nxt[e] = 0.f;
             kf[0] = kp[0], kf[1] = kp[1];
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -992,39 +959,27 @@ __global__ __launch_bounds__(256, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
                 if (s + 2 < KS) kf[s + 2] = read_k(s + 2);
                 if (s + 2 >= KS) vf[s + 2 - KS] = read_v(s + 2 - KS);
                 side(s, KS + NV);
-                nxt[0] = M::m32(kf[s], qf[0][s], nxt[0]);
-                nxt[1] = M::m32(kf[s], qf[1][s], nxt[1]);
+                nxt = M::m32(kf[s], qf[s], nxt);
 #pragma unroll
                 for (int p = EARLY * s / KS; p < EARLY * (s + 1) / KS; ++p) weigh(p);
                 __builtin_amdgcn_sched_barrier(0);
             }
-            float m[2] = {-INFINITY, -INFINITY};
+            float m = -INFINITY;
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 if (i + 2 < NV) vf[i + 2] = read_v(i + 2);
                 if (i + 2 >= NV) kp[i + 2 - NV] = *reinterpret_cast<const u32x4*>(p0 + 32 * (i + 2 - NV));
                 side(KS + i, KS + NV);
-                o[0][i % DT] = M::m32(vf[i], pb[0][i / DT], o[0][i % DT]);
-                o[1][i % DT] = M::m32(vf[i], pb[1][i / DT], o[1][i % DT]);
+                o[i % DT] = M::m32(vf[i], pb[i / DT], o[i % DT]);
                 if (i < DT)
 #pragma unroll
-                    for (int p = EARLY + 4 * i / DT; p < EARLY + 4 * (i + 1) / DT; ++p) weigh(p);
+                    for (int p = EARLY + 2 * i / DT; p < EARLY + 2 * (i + 1) / DT; ++p) weigh(p);
 #pragma unroll
-                for (int ct = 0; ct < 2; ++ct)  // (the last scores are two pairs of products old)
-#pragma unroll
-                    for (int p = i < 2 ? 0 : 8 * (i - 2) / (NV - 2); i >= 2 && p < 8 * (i - 1) / (NV - 2); ++p) {
-                        float x = nxt[ct][2 * p], y = nxt[ct][2 * p + 1];
-                        asm volatile("" : "+v"(x), "+v"(y));  // from here on in registers that the VALU reads
-                        m[ct] = fmaxf(fmaxf(m[ct], x), y);
-                        nxt[ct][2 * p] = x, nxt[ct][2 * p + 1] = y;
-                    }
+                for (int p = i < 2 ? 0 : 8 * (i - 2) / (NV - 2); i >= 2 && p < 8 * (i - 1) / (NV - 2); ++p)
+                    m = fmaxf(fmaxf(m, nxt[2 * p]), nxt[2 * p + 1]);  // (the last scores are two products old)
                 __builtin_amdgcn_sched_barrier(0);
             }
-#pragma unroll
-            for (int ct = 0; ct < 2; ++ct) {
-                const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(m[ct]), __float_as_uint(m[ct]), false, false);
-                mx[ct] = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
-            }
+            return join_halves(m);
         };
 
         // Step n stores K(n + 2) and V(n + 1), loaded by step n - 1, under its second half, and loads K(n + 3) and V(n + 2) into
@@ -1049,11 +1004,12 @@ __global__ __launch_bounds__(256, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
 #pragma unroll
         for (int i = 0; i < LPB; ++i) *reinterpret_cast<u32x4*>(lds + KBLK + kst[i]) = r1[i];
         lds_barrier();
-        float mx[2];
         if (nbw > 0) {
-            scores(0, 0, sa);
-            maxima(sa, mx);
-            settle(0, 0, b0, sa, mx);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) sa[e] = 0.f;
+#pragma unroll
+            for (int s = 0; s < KS; ++s) sa = M::m32(*reinterpret_cast<const u32x4*>(lds + kbase + 32 * s), qf[s], sa);
+            settle(0, 0, b0, sa, maximum(sa));
 #pragma unroll
             for (int i = 0; i < 2; ++i) kp[i] = *reinterpret_cast<const u32x4*>(lds + 32 * KR + kbase + 32 * i);
         }
@@ -1077,37 +1033,31 @@ __global__ __launch_bounds__(256, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
                 }
             };
             if (n < nbw) {
-                half(kslot, 1, sb, vslot, 0, sa, mx, kslot1, 0, [](int, int) {});
+                float mx = half(kslot, 1, sb, vslot, 0, sa, kslot1, 0, [](int, int) {});
                 settle(n, 1, b0, sb, mx);
-                half(kslot1, 0, sa, vslot, 1, sb, mx, kslot1, 1, move);  // (scores behind the last block: not used)
+                mx = half(kslot1, 0, sa, vslot, 1, sb, kslot1, 1, move);  // (scores behind the last block: not used)
                 settle(n + 1, 0, b1, sa, mx);
             } else {
                 move(0, 1);
             }
             s2 = s3, b0 = b1, b1 = b2, b2 = b3, kslot = kslot1;
         }
-#pragma unroll
-        for (int ct = 0; ct < 2; ++ct) {
-            const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(l_run[ct]), __float_as_uint(l_run[ct]), false, false);
-            l_run[ct] = __uint_as_float(x[0]) + __uint_as_float(x[1]);
+        {
+            const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(l_run), __float_as_uint(l_run), false, false);
+            l_run = __uint_as_float(x[0]) + __uint_as_float(x[1]);
         }
 
         auto write = [&]() __attribute__((always_inline)) {
+            const float inv = l_run != 0.f ? 1.0f / l_run : 0.f;  // no key at all: zeros
+            T* y = static_cast<T*>(a.y) + (size_t(rq.row0 + myrow) * a.qh + myhead) * HD + 4 * h;
+            if (mycol < cols) {
 #pragma unroll
-            for (int ct = 0; ct < 2; ++ct) {
-                const int c = cw + 32 * ct + c32;
-                const float inv = l_run[ct] != 0.f ? 1.0f / l_run[ct] : 0.f;  // no key at all: zeros
-                const int row = rq.row0 + row_first + c / group, head = hk * group + c % group;
-                T* y = static_cast<T*>(a.y) + (size_t(row) * a.qh + head) * HD + 4 * h;
-                if (c < cols) {
+                for (int d = 0; d < DT; ++d)
 #pragma unroll
-                    for (int d = 0; d < DT; ++d)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)  // dims 32 d + 8 e + 4 h ..
-                            *reinterpret_cast<uint2*>(y + 32 * d + 8 * e) =
-                                make_uint2(pack<T>(o[ct][d][4 * e] * inv, o[ct][d][4 * e + 1] * inv),
-                                           pack<T>(o[ct][d][4 * e + 2] * inv, o[ct][d][4 * e + 3] * inv));
-                }
+                    for (int e = 0; e < 4; ++e)  // dims 32 d + 8 e + 4 h ..
+                        *reinterpret_cast<uint2*>(y + 32 * d + 8 * e) =
+                            make_uint2(pack<T>(o[d][4 * e] * inv, o[d][4 * e + 1] * inv),
+                                       pack<T>(o[d][4 * e + 2] * inv, o[d][4 * e + 3] * inv));
             }
         };
         const uint32_t begin = u - uint32_t(j0), end = begin + uint32_t(units);
@@ -1115,21 +1065,18 @@ __global__ __launch_bounds__(256, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
             write();
         } else {
             const uint32_t wa = group_of(begin), wb = group_of(end - 1);
-            // column tile x, 16 bytes i of lane l: ((2 wave + x) 4 DT + i) 64 + l, after the maxima and sums
-            auto at = [&](int slot, int ct, int i) {
-                return slot + 2 * int(paged::kTileCols) + (((2 * wv + ct) * 4 * DT + i) * 64 + lane) * 4;
+            // 16 bytes i of lane l: (4 DT wave + i) 64 + l, after the maxima and sums
+            auto at = [&](int slot, int i) {
+                return slot + 2 * int(paged::kTileCols) + ((wv * 4 * DT + i) * 64 + lane) * 4;
             };
             if (cw < cols) {
                 const int mine = slot_at(w, begin >= u0);
+                if (h == 0) store_part2(ws, mine + 2 * mycol, m_run, l_run);
 #pragma unroll
-                for (int ct = 0; ct < 2; ++ct) {
-                    if (h == 0) store_part2(ws, mine + 2 * (cw + 32 * ct + c32), m_run[ct], l_run[ct]);
-#pragma unroll
-                    for (int i = 0; i < 4 * DT; ++i) {
-                        const f32x16& x = o[ct][i >> 2];
-                        const int e = 4 * (i & 3);
-                        store_part(ws, at(mine, ct, i), f32x4{x[e], x[e + 1], x[e + 2], x[e + 3]});
-                    }
+                for (int i = 0; i < 4 * DT; ++i) {
+                    const f32x16& x = o[i >> 2];
+                    const int e = 4 * (i & 3);
+                    store_part(ws, at(mine, i), f32x4{x[e], x[e + 1], x[e + 2], x[e + 3]});
                 }
             }
             __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0): this wave's stores are performed
@@ -1139,40 +1086,30 @@ __global__ __launch_bounds__(256, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
             lds_barrier();
             if (arrived == wb - wa) {  // the last one in joins the parts, in their order
                 if (cw < cols) {
+                    m_run = -INFINITY, l_run = 0.f;
 #pragma unroll
-                    for (int ct = 0; ct < 2; ++ct) {
-                        m_run[ct] = -INFINITY, l_run[ct] = 0.f;
+                    for (int d = 0; d < DT; ++d)
 #pragma unroll
-                        for (int d = 0; d < DT; ++d)
-#pragma unroll
-                            for (int e = 0; e < 16; ++e) o[ct][d][e] = 0.f;
-                    }
+                        for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
                     for (uint32_t i = wa; i <= wb; ++i) {
                         const int part = slot_at(i, i == wa);
-                        float2 ml[2];
-                        f32x4 x[2][4 * DT];
+                        const float2 ml = load_part2(ws, part + 2 * mycol);
+                        f32x4 x[4 * DT];
 #pragma unroll
-                        for (int ct = 0; ct < 2; ++ct) {
-                            ml[ct] = load_part2(ws, part + 2 * (cw + 32 * ct + c32));
-#pragma unroll
-                            for (int j = 0; j < 4 * DT; ++j) x[ct][j] = load_part(ws, at(part, ct, j));
-                        }
+                        for (int j = 0; j < 4 * DT; ++j) x[j] = load_part(ws, at(part, j));
                         __builtin_amdgcn_sched_barrier(0);  // (all under way before the first is waited for)
+                        const float mn = fmaxf(m_run, ml.x), mnc = mn == -INFINITY ? 0.f : mn * a.scale_log2;
+                        const float fo = __builtin_amdgcn_exp2f(m_run * a.scale_log2 - mnc);
+                        const float fn = __builtin_amdgcn_exp2f(ml.x * a.scale_log2 - mnc);
+                        l_run = l_run * fo + ml.y * fn;
+                        m_run = mn;
 #pragma unroll
-                        for (int ct = 0; ct < 2; ++ct) {
-                            const float mn = fmaxf(m_run[ct], ml[ct].x), mc = mn == -INFINITY ? 0.f : mn * a.scale_log2;
-                            const float fo = __builtin_amdgcn_exp2f(m_run[ct] * a.scale_log2 - mc);
-                            const float fn = __builtin_amdgcn_exp2f(ml[ct].x * a.scale_log2 - mc);
-                            l_run[ct] = l_run[ct] * fo + ml[ct].y * fn;
-                            m_run[ct] = mn;
+                        for (int j = 0; j < 4 * DT; ++j)
 #pragma unroll
-                            for (int j = 0; j < 4 * DT; ++j)
-#pragma unroll
-                                for (int q = 0; q < 4; ++q) {
-                                    const int e = 4 * (j & 3) + q;
-                                    o[ct][j >> 2][e] = o[ct][j >> 2][e] * fo + x[ct][j][q] * fn;
-                                }
-                        }
+                            for (int q = 0; q < 4; ++q) {
+                                const int e = 4 * (j & 3) + q;
+                                o[j >> 2][e] = o[j >> 2][e] * fo + x[j][q] * fn;
+                            }
                     }
                     write();
                 }
@@ -1286,7 +1223,7 @@ static void launch_attn(const uint32_t* w, void* const* p, hipStream_t s) {
     if (few_columns(w))
         hipLaunchKernelGGL((k_attn_rows<T, HD>), dim3(paged::kRowsGroups), dim3(256), 0, s, a, bytes, bytes);
     else
-        hipLaunchKernelGGL((k_attn_tiles<T, HD>), dim3(paged::kTileGroups), dim3(256), 0, s, a, bytes);
+        hipLaunchKernelGGL((k_attn_tiles<T, HD>), dim3(paged::kTileGroups), dim3(512), 0, s, a, bytes);
 }
 static void l_attn(const PreparedDispatch& pd, void* const* p, hipStream_t s) {
     const uint32_t* w = pd.words.data();
