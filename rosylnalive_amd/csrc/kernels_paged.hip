@@ -902,7 +902,19 @@ __global__ __launch_bounds__(512, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
             for (int e = 1; e < 16; ++e) m = fmaxf(m, s[e]);
             return join_halves(m);
         };
-        // hides what the columns do not see of the 32 keys, and moves the reference maxima where they are left behind
+        // the reference maximum moves where a column leaves it behind by more than 8 in the exponent
+        auto follow = [&](float mx) __attribute__((always_inline)) {
+            const bool grow = (mx - m_run) * a.scale_log2 > 8.0f;  // false for NaN (both -inf)
+            if (__any(grow)) {
+                const float alpha = grow ? __builtin_amdgcn_exp2f((m_run - mx) * a.scale_log2) : 1.0f;
+                m_run = grow ? mx : m_run;
+                mc = m_run == -INFINITY ? 0.f : m_run * a.scale_log2;
+                l_run *= alpha;
+#pragma unroll
+                for (int d = 0; d < DT; ++d) o[d] *= alpha;
+            }
+        };
+        // hides what the columns do not see of the 32 keys first
         auto settle = [&](int j, int kt, uint32_t bad, f32x16& s, float mx) __attribute__((always_inline)) {
             const int kb = (j0 + j) * KB + 32 * kt;
             if (j >= nbw) {  // behind the last block: nothing to see
@@ -914,20 +926,10 @@ __global__ __launch_bounds__(512, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
                     if (16 * (e >> 3) + (e & 7) >= lim || (bad >> (2 * kt + (e >> 3)) & 1u)) s[e] = -INFINITY;
                 mx = maximum(s);
             }
-            const bool grow = (mx - m_run) * a.scale_log2 > 8.0f;  // false for NaN (both -inf)
-            if (__any(grow)) {
-                const float alpha = grow ? __builtin_amdgcn_exp2f((m_run - mx) * a.scale_log2) : 1.0f;
-                m_run = grow ? mx : m_run;
-                mc = m_run == -INFINITY ? 0.f : m_run * a.scale_log2;
-                l_run *= alpha;
-#pragma unroll
-                for (int d = 0; d < DT; ++d) o[d] *= alpha;
-            }
+            follow(mx);
         };
         // 32 keys: the scores of the next 32 (matrix core) under the weights of these (VALU), then their products under the
-        // last of the weights and the next ones' maxima, a matrix instruction and its share of the VALU's work at a time: the
-        // scheduling barriers keep that order (without them all the instructions of one kind follow each other, and either
-        // unit waits for the other), with each operand read two ahead.
+        // last of the weights and the next ones' maxima, each operand read two instructions ahead.
         u32x4 kp[2];  // the first two operands of the next scores, read under the products before them
         auto half = [&](int kslot, int nkt, f32x16& nxt, int vslot, int kt, f32x16& cur, int pslot, int pkt,
                         auto&& side) __attribute__((always_inline)) {
@@ -953,7 +955,6 @@ __global__ __launch_bounds__(512, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
 #pragma unroll
             for (int e = 0; e < 16; ++e) nxt[e] = 0.f;
             kf[0] = kp[0], kf[1] = kp[1];
-            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
                 if (s + 2 < KS) kf[s + 2] = read_k(s + 2);
@@ -962,7 +963,6 @@ __global__ __launch_bounds__(512, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
                 nxt = M::m32(kf[s], qf[s], nxt);
 #pragma unroll
                 for (int p = EARLY * s / KS; p < EARLY * (s + 1) / KS; ++p) weigh(p);
-                __builtin_amdgcn_sched_barrier(0);
             }
             float m = -INFINITY;
 #pragma unroll
@@ -977,7 +977,6 @@ __global__ __launch_bounds__(512, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
 #pragma unroll
                 for (int p = i < 2 ? 0 : 8 * (i - 2) / (NV - 2); i >= 2 && p < 8 * (i - 1) / (NV - 2); ++p)
                     m = fmaxf(fmaxf(m, nxt[2 * p]), nxt[2 * p + 1]);  // (the last scores are two products old)
-                __builtin_amdgcn_sched_barrier(0);
             }
             return join_halves(m);
         };
@@ -1014,31 +1013,53 @@ __global__ __launch_bounds__(512, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
             for (int i = 0; i < 2; ++i) kp[i] = *reinterpret_cast<const u32x4*>(lds + 32 * KR + kbase + 32 * i);
         }
         int kslot = 0;  // n % 3
-        for (int n = 0; n < nb; ++n) {
-            const int kslot1 = kslot == 2 ? 0 : kslot + 1, kslot2 = kslot1 == 2 ? 0 : kslot1 + 1;
+        // one store or load of a K or V chunk: 4 LPB of them shared out over the parts of a half
+        auto move = [&](int ks, int vs, int sk, int sv, int part, int parts) __attribute__((always_inline)) {
+#pragma unroll
+            for (int x = 4 * LPB * part / parts; x < 4 * LPB * (part + 1) / parts; ++x) {
+                const int i = x >> 2;
+                if ((x & 3) == 0) *reinterpret_cast<u32x4*>(lds + ks * KBLK + kst[i]) = rk[i];
+                if ((x & 3) == 1) rk[i] = __builtin_amdgcn_raw_buffer_load_b128(k_rsrc, 16 * lane + 1024 * i, sk, 0);
+                if ((x & 3) == 2) store_v(vs, i);
+                if ((x & 3) == 3) rv[i] = __builtin_amdgcn_raw_buffer_load_b128(v_rsrc, 16 * lane + 1024 * i, sv, 0);
+            }
+        };
+        auto none = [](int, int) {};
+        int n = 0;
+        // while every column sees all of this block and the next, all have pages and more follow: nothing to ask
+        const int plain = no_page ? 0 : min(nb - 3, (rq.seen + row_first) / KB - 1 - j0);
+        for (; n < plain; ++n) {
+            const int kslot1 = kslot == 2 ? 0 : kslot + 1, kslot2 = kslot1 == 2 ? 0 : kslot1 + 1, vslot = n & 1;
+            if (n) lds_barrier();
+            locate(n + 3, s3, b3);
+            if (nbw > 0) {
+                follow(half(kslot, 1, sb, vslot, 0, sa, kslot1, 0, none));
+                follow(half(kslot1, 0, sa, vslot, 1, sb, kslot1, 1,
+                            [&](int part, int parts) { move(kslot2, 1 - vslot, s3, s2, part, parts); }));
+            } else {
+                move(kslot2, 1 - vslot, s3, s2, 0, 1);
+            }
+            s2 = s3, kslot = kslot1;
+            b0 = b1 = 0, b2 = b3;
+            if (no_page) {  // among the 16 blocks from n + 3 on
+                ++n;
+                break;
+            }
+        }
+        for (; n < nb; ++n) {
+            const int kslot1 = kslot == 2 ? 0 : kslot + 1, kslot2 = kslot1 == 2 ? 0 : kslot1 + 1, vslot = n & 1;
             if (n) lds_barrier();
             s3 = s2, b3 = b2;
             if (n + 3 < nb) locate(n + 3, s3, b3);
             if (n + 1 < nb) hide_v(n + 1, b1);
-            const int vslot = n & 1, vslot1 = 1 - vslot;
-            // one store or load of a K or V chunk: 4 LPB of them shared out over the parts of a half
-            auto move = [&](int part, int parts) __attribute__((always_inline)) {
-#pragma unroll
-                for (int x = 4 * LPB * part / parts; x < 4 * LPB * (part + 1) / parts; ++x) {
-                    const int i = x >> 2;
-                    if ((x & 3) == 0) *reinterpret_cast<u32x4*>(lds + kslot2 * KBLK + kst[i]) = rk[i];
-                    if ((x & 3) == 1) rk[i] = __builtin_amdgcn_raw_buffer_load_b128(k_rsrc, 16 * lane + 1024 * i, s3, 0);
-                    if ((x & 3) == 2) store_v(vslot1, i);
-                    if ((x & 3) == 3) rv[i] = __builtin_amdgcn_raw_buffer_load_b128(v_rsrc, 16 * lane + 1024 * i, s2, 0);
-                }
-            };
+            auto moves = [&](int part, int parts) { move(kslot2, 1 - vslot, s3, s2, part, parts); };
             if (n < nbw) {
-                float mx = half(kslot, 1, sb, vslot, 0, sa, kslot1, 0, [](int, int) {});
+                float mx = half(kslot, 1, sb, vslot, 0, sa, kslot1, 0, none);
                 settle(n, 1, b0, sb, mx);
-                mx = half(kslot1, 0, sa, vslot, 1, sb, kslot1, 1, move);  // (scores behind the last block: not used)
+                mx = half(kslot1, 0, sa, vslot, 1, sb, kslot1, 1, moves);  // (scores behind the last block: not used)
                 settle(n + 1, 0, b1, sa, mx);
             } else {
-                move(0, 1);
+                moves(0, 1);
             }
             s2 = s3, b0 = b1, b1 = b2, b2 = b3, kslot = kslot1;
         }
