@@ -368,18 +368,22 @@ struct Mfma<__bf16> {
 // an older line from the XCD's L2 (device scope), 16 or 8 bytes each and as many under way as there are registers (the
 // atomic loads of that scope are waited for one by one: a join of two parts took 25 us, of 32 parts 320).
 constexpr int kDeviceScope = 16;  // the sc1 bit of a buffer instruction
+template <int SCOPE = kDeviceScope>
 __device__ __forceinline__ void store_part(__amdgpu_buffer_rsrc_t r, int word, f32x4 v) {
-    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), r, word * 4, 0, kDeviceScope);
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), r, word * 4, 0, SCOPE);
 }
+template <int SCOPE = kDeviceScope>
 __device__ __forceinline__ f32x4 load_part(__amdgpu_buffer_rsrc_t r, int word) {
-    return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, word * 4, 0, kDeviceScope));
+    return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, word * 4, 0, SCOPE));
 }
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+template <int SCOPE = kDeviceScope>
 __device__ __forceinline__ void store_part2(__amdgpu_buffer_rsrc_t r, int word, float a, float b) {
-    __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(a), __float_as_uint(b)}, r, word * 4, 0, kDeviceScope);
+    __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(a), __float_as_uint(b)}, r, word * 4, 0, SCOPE);
 }
+template <int SCOPE = kDeviceScope>
 __device__ __forceinline__ float2 load_part2(__amdgpu_buffer_rsrc_t r, int word) {
-    const u32x2 v = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, word * 4, 0, kDeviceScope));
+    const u32x2 v = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, word * 4, 0, SCOPE));
     return make_float2(__uint_as_float(v[0]), __uint_as_float(v[1]));
 }
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
@@ -620,7 +624,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(AttnArgs a, uint32_t k_byt
                     float m = -INFINITY, sum = 0.f;
                     f32x4 v = {0.f, 0.f, 0.f, 0.f};
                     if (e < lanes && k < share) {
-                        constexpr int PF = 4;
+                        constexpr int PF = 6;
                         for (uint32_t i = wa + k; i <= wb; i += PF * share) {
                             float2 ml[PF];
                             f32x4 x[PF];
@@ -710,7 +714,13 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(AttnArgs a, uint32_t k_byt
 
 // sum over i < n of floor((b + i step) / 64) (Euclid's way down the two slopes), for sums below 2^31
 __device__ __forceinline__ uint32_t floor_sum64(uint32_t n, uint32_t step, uint32_t b) {
-    uint32_t m = 64, sum = 0;
+    // the first step, whose divisor is known
+    uint32_t sum = uint32_t(uint64_t(n) * (n - 1) / 2) * (step / 64) + n * (b / 64), m = 64;
+    step %= 64, b %= 64;
+    const uint32_t y0 = step * n + b;
+    n = y0 / 64, b = y0 % 64;
+    const uint32_t s0 = step;
+    step = m, m = s0;
     while (n) {
         sum += uint32_t(uint64_t(n) * (n - 1) / 2) * (step / m) + n * (b / m);
         step %= m, b %= m;
@@ -741,7 +751,8 @@ __global__ __launch_bounds__(512, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
     __shared__ __attribute__((aligned(16))) uint8_t lds[3 * KBLK + 2 * BLK];  // K blocks n % 3, then V blocks n % 2
     __shared__ uint32_t ends[paged::kMaxRequests];
     __shared__ uint32_t red[8];
-    __shared__ uint32_t arrived;
+    __shared__ uint32_t units_of_tile[paged::kTileGroups];
+    __shared__ int chosen[3];
     const int t = threadIdx.x, lane = t & 63, wv = uniform(t >> 6), c32 = lane & 31, h = lane >> 5;
     const int group = int(a.qh / a.kvh), kvh = int(a.kvh), TR = int(paged::kTileCols) / group;
 
@@ -760,45 +771,109 @@ __global__ __launch_bounds__(512, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
         return sum;
     };
     auto tiles_of = [&](const Request& q) { return (q.rows + TR - 1) / TR; };
-    {
+    // ends[r] = the sum of f over the requests up to and with r
+    auto scan_requests = [&](auto&& f) {
         const uint32_t per = (a.requests + 511) / 512, r0 = min(t * per, a.requests), r1 = min(r0 + per, a.requests);
         uint32_t sum = 0;
         for (uint32_t r = r0; r < r1; ++r) {
             const Request q = request_of(a, r);
-            if (q.rows > 0) sum += first_units(q, tiles_of(q)) * uint32_t(kvh);
+            if (q.rows > 0) sum += f(q);
             ends[r] = sum;
         }
         const uint32_t before = scan_sat(sum, red) - sum;
         for (uint32_t r = r0; r < r1; ++r) ends[r] += before;
         __syncthreads();
-    }
-    const uint32_t total = ends[a.requests - 1], G = min(uint32_t(gridDim.x), total);
-    // workgroups of one XCD (every eighth) take neighbouring units, which share a KV head's blocks in its L2
-    const uint32_t w = G == paged::kTileGroups ? (blockIdx.x % 8) * (paged::kTileGroups / 8) + blockIdx.x / 8 : blockIdx.x;
-    if (w >= G) return;
-    auto first_unit = [&](uint32_t i) { return uint32_t(uint64_t(total) * i / G); };
-    auto group_of = [&](uint32_t u) { return uint32_t(((uint64_t(u) + 1) * G - 1) / total); };
-    const uint32_t u0 = first_unit(w), u1 = first_unit(w + 1);
-
-    const __amdgpu_buffer_rsrc_t k_rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(a.kc), 0, bytes, 0x00020000);
-    const __amdgpu_buffer_rsrc_t v_rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(a.vc), 0, bytes, 0x00020000);
-    // this wave moves keys 8 wv .. + 7 of a block, 16 bytes per lane and load: both caches hold them in one piece
-    int kst[LPB];  // where a K chunk goes in its block
-#pragma unroll
-    for (int i = 0; i < LPB; ++i) {
-        const int p = 64 * i + lane, row = p / CH, ch = p % CH;  // row of the wave's 8, place in the row
-        kst[i] = (8 * wv + row) * KR + ch * 16;
-    }
-    // operand reads: K row of matrix row c32 is key 16 (c32 / 16) + 8 (c32 / 4 % 2) + 4 (c32 / 8 % 2) + c32 % 4
-    const int krow = (c32 & 19) | ((c32 & 4) << 1) | ((c32 & 8) >> 1);
-    const int kbase = krow * KR + 16 * h, vbase = 3 * KBLK + h * (8 * RB) + c32 * 16;
-
+    };
     Request rq{};
-    int r = uniform(first_above(ends, int(a.requests), u0));
-    int hk = 0, tile = 0, kfirst = 0;
-    {
+    auto enter = [&](int r) {
         rq = request_of(a, uint32_t(r));
         rq.row0 = uniform(rq.row0), rq.rows = uniform(rq.rows), rq.seen = uniform(rq.seen);
+    };
+    int r = 0, hk = 0, tile = 0, kfirst = 0;
+    uint32_t u0 = 0, u1 = 0, total = 0, G = 0, w = blockIdx.x;  // (units of all items; not used where each has its own workgroups)
+    int parts = 0, mine = 0, lead = 0;                          // of an item with workgroups of its own
+    // what the join has to know of a split item: written by the workgroup that begins it, by the others as none
+    auto describe = [&](int parts, int base, int stride, int first, const Request& q, int row_first, int cols, int hk) {
+        if (t != 0) return;
+        u32x4* d = reinterpret_cast<u32x4*>(a.ws + paged::kGroups) + 2 * w;
+        d[0] = u32x4{uint32_t(parts), uint32_t(base), uint32_t(stride), uint32_t(first)};
+        d[1] = u32x4{uint32_t(q.row0 + row_first), uint32_t(cols), uint32_t(hk), 0u};
+    };
+    auto describe_none = [&]() { describe(0, 0, 0, 0, Request{}, 0, 0, 0); };
+    scan_requests([&](const Request& q) { return uint32_t(tiles_of(q)); });
+    const uint32_t tiles_all = ends[a.requests - 1];
+    if (tiles_all == 0) {
+        describe_none();
+        return;
+    }
+    const bool apart = uint64_t(tiles_all) * kvh <= paged::kTileGroups;
+    if (apart) {
+        // No more items than workgroups: each gets ceil(units / q) of its own, q the least that fits, so no workgroup starts
+        // more than one piece (a start takes 4 us, the time of two units). More parts than the square root of half the
+        // longest item's units are not worth their join (about 1 us a part). All heads of a tile split alike; neighbouring
+        // workgroups, which run on different XCDs, take different heads.
+        if (uint32_t(t) < tiles_all) {
+            const int i = first_above(ends, int(a.requests), uint32_t(t));
+            units_of_tile[t] = uint32_t(tile_units(request_of(a, uint32_t(i)), t - int(i ? ends[i - 1] : 0)));
+        }
+        __syncthreads();
+        uint32_t n[4];
+        const int held = int(tiles_all + 63) / 64;  // tiles of a lane
+        float sum = 0.f, most = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            n[j] = uint32_t(lane + 64 * j) < tiles_all ? units_of_tile[lane + 64 * j] : 0u;
+            sum += float(n[j]);
+            most = fmaxf(most, float(n[j]));
+        }
+        const uint32_t room = paged::kTileGroups / uint32_t(kvh);
+        uint32_t hi = uint32_t(uniform(int(wave_max(most)))), lo = uint32_t(uniform(int(wave_sum(sum)))) / room;
+        lo = min(max(max(lo, 1u), uint32_t(sqrtf(0.5f * float(hi)))), hi);
+        while (lo < hi) {
+            const uint32_t q = (lo + hi) >> 1;
+            float need = 0.f;  // (a sum up to 2^24: exact; beyond, too many either way)
+            const float by = 1.0f / float(q);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (j >= held) continue;
+                uint32_t c = uint32_t(float(n[j]) * by);  // n / q but for the last place
+                c += uint32_t(c * q < n[j]), c -= uint32_t(c > 0 && (c - 1) * q >= n[j]);
+                need += float(c);
+            }
+            if (uint32_t(uniform(int(wave_sum(need)))) <= room)
+                hi = q;
+            else
+                lo = q + 1;
+        }
+        const uint32_t own = uint32_t(t) < tiles_all ? (units_of_tile[t] + hi - 1) / hi : 0u, end = scan_sat(own, red);
+        hk = int(w) % kvh;
+        const uint32_t place = w / uint32_t(kvh);
+        if (t == 0) chosen[0] = -1;
+        __syncthreads();
+        if (place < end && place >= end - own) chosen[0] = t, chosen[1] = int(own), chosen[2] = int(end - own);
+        __syncthreads();
+        const int at = uniform(chosen[0]);
+        if (at < 0) {
+            describe_none();
+            return;
+        }
+        parts = uniform(chosen[1]), mine = int(place) - uniform(chosen[2]), lead = uniform(chosen[2]) * kvh + hk;
+        r = uniform(first_above(ends, int(a.requests), uint32_t(at)));
+        tile = at - uniform(r ? int(ends[r - 1]) : 0);
+        enter(r);
+    } else {
+        __syncthreads();
+        scan_requests([&](const Request& q) { return first_units(q, tiles_of(q)) * uint32_t(kvh); });
+        total = ends[a.requests - 1], G = min(uint32_t(gridDim.x), total);
+        // workgroups of one XCD (every eighth) take neighbouring units, which share a KV head's blocks in its L2
+        if (G == paged::kTileGroups) w = (blockIdx.x % 8) * (paged::kTileGroups / 8) + blockIdx.x / 8;
+        if (w >= G) {
+            describe_none();
+            return;
+        }
+        u0 = uint32_t(uint64_t(total) * w / G), u1 = uint32_t(uint64_t(total) * (w + 1) / G);
+        r = uniform(first_above(ends, int(a.requests), u0));
+        enter(r);
         uint32_t in = u0 - (r ? uint32_t(uniform(int(ends[r - 1]))) : 0u);
         const int tiles = tiles_of(rq);
         const uint32_t per_head = uint32_t(uniform(int(first_units(rq, tiles))));
@@ -813,15 +888,30 @@ __global__ __launch_bounds__(512, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
         }
         tile = uniform(lo), kfirst = uniform(int(in - first_units(rq, lo)));
     }
-    constexpr int SW = int(paged::slot_words(paged::kTileCols, HD));
-    const __amdgpu_buffer_rsrc_t ws = __builtin_amdgcn_make_buffer_rsrc(
-        a.ws, 0, int(4 * (paged::kGroups + 2 * paged::kTileGroups * SW)), 0x00020000);
-    auto slot_at = [&](uint32_t i, bool begins) { return int(paged::kGroups) + int(2 * i + (begins ? 1 : 0)) * SW; };
 
-    for (uint32_t u = u0; u < u1;) {
+    const __amdgpu_buffer_rsrc_t k_rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(a.kc), 0, bytes, 0x00020000);
+    const __amdgpu_buffer_rsrc_t v_rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(a.vc), 0, bytes, 0x00020000);
+    // this wave moves keys 8 wv .. + 7 of a block, 16 bytes per lane and load: both caches hold them in one piece
+    int kst[LPB];  // where a K chunk goes in its block
+#pragma unroll
+    for (int i = 0; i < LPB; ++i) {
+        const int p = 64 * i + lane, row = p / CH, ch = p % CH;  // row of the wave's 8, place in the row
+        kst[i] = (8 * wv + row) * KR + ch * 16;
+    }
+    // operand reads: K row of matrix row c32 is key 16 (c32 / 16) + 8 (c32 / 4 % 2) + 4 (c32 / 8 % 2) + c32 % 4
+    const int krow = (c32 & 19) | ((c32 & 4) << 1) | ((c32 & 8) >> 1);
+    const int kbase = krow * KR + 16 * h, vbase = 3 * KBLK + h * (8 * RB) + c32 * 16;
+
+    constexpr int SW = int(paged::slot_words(paged::kTileCols, HD));
+    const __amdgpu_buffer_rsrc_t ws =
+        __builtin_amdgcn_make_buffer_rsrc(a.ws, 0, int(4 * (paged::kTileSlots + 2 * paged::kTileGroups * SW)), 0x00020000);
+    bool described = false;
+
+    for (uint32_t u = u0; apart || u < u1;) {
         // ---- a piece: blocks j0 .. j0 + nb - 1 of a tile
-        const int units = tile_units(rq, tile), keys = tile_keys(rq, tile), j0 = kfirst;
-        const int nb = min(units - j0, int(u1 - u));
+        const int units = tile_units(rq, tile), keys = tile_keys(rq, tile);
+        const int j0 = apart ? int(uint64_t(uint32_t(units)) * mine / parts) : kfirst;
+        const int nb = apart ? int(uint64_t(uint32_t(units)) * (mine + 1) / parts) - j0 : min(units - j0, int(u1 - u));
         const int row_first = tile * TR, cols = min(TR, rq.rows - row_first) * group;
         const int cw = 32 * wv;  // this wave's first column
         // blocks that some column of the wave sees
@@ -858,20 +948,22 @@ __global__ __launch_bounds__(512, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
             const uint32_t off = uint32_t((j0 + j) * KB + 8 * wv) & ((1u << a.page_log2) - 1);
             soff = id < a.pages ? int((((id * uint32_t(kvh) + hk) << a.page_log2) + off) * RB) : 0;
         };
-        u32x4 rk[LPB], rv[LPB];
-        auto load_k = [&](int soff) __attribute__((always_inline)) {
-#pragma unroll
-            for (int i = 0; i < LPB; ++i) rk[i] = __builtin_amdgcn_raw_buffer_load_b128(k_rsrc, 16 * lane + 1024 * i, soff, 0);
+        // the chunks of this wave on their way to LDS: two blocks of each cache
+        u32x4 rk[2][LPB], rv[2][LPB];
+        auto load_k = [&](auto set, int i, int soff) __attribute__((always_inline)) {
+            rk[decltype(set)::value][i] = __builtin_amdgcn_raw_buffer_load_b128(k_rsrc, 16 * lane + 1024 * i, soff, 0);
         };
-        auto load_v = [&](int soff) __attribute__((always_inline)) {
-#pragma unroll
-            for (int i = 0; i < LPB; ++i) rv[i] = __builtin_amdgcn_raw_buffer_load_b128(v_rsrc, 16 * lane + 1024 * i, soff, 0);
+        auto load_v = [&](auto set, int i, int soff) __attribute__((always_inline)) {
+            rv[decltype(set)::value][i] = __builtin_amdgcn_raw_buffer_load_b128(v_rsrc, 16 * lane + 1024 * i, soff, 0);
         };
-        auto store_k = [&](int slot) __attribute__((always_inline)) {
-#pragma unroll
-            for (int i = 0; i < LPB; ++i) *reinterpret_cast<u32x4*>(lds + slot * KBLK + kst[i]) = rk[i];
+        auto store_k = [&](auto set, int i, int slot) __attribute__((always_inline)) {
+            *reinterpret_cast<u32x4*>(lds + slot * KBLK + kst[i]) = rk[decltype(set)::value][i];
         };
-        auto hide_v = [&](int j, uint32_t bad) __attribute__((always_inline)) {
+        auto store_v = [&](auto set, int i, int slot) __attribute__((always_inline)) {
+            *reinterpret_cast<u32x4*>(lds + 3 * KBLK + slot * BLK + 1024 * (LPB * wv + i) + 16 * lane) =
+                rv[decltype(set)::value][i];
+        };
+        auto hide_v = [&](auto set, int j, uint32_t bad) __attribute__((always_inline)) {
             const int left = keys - (j0 + j) * KB;  // keys of the block that any column sees
             if (left < KB || bad) {  // uniform: what is hidden may be anything, and zero times NaN is NaN
 #pragma unroll
@@ -879,12 +971,9 @@ __global__ __launch_bounds__(512, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
                     const int in = (bad >> (wv >> 1) & 1u) ? 0 : left - 8 * wv;
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        rv[i][e] &= (2 * e < in ? 0x0000FFFFu : 0u) | (2 * e + 1 < in ? 0xFFFF0000u : 0u);
+                        rv[decltype(set)::value][i][e] &= (2 * e < in ? 0x0000FFFFu : 0u) | (2 * e + 1 < in ? 0xFFFF0000u : 0u);
                 }
             }
-        };
-        auto store_v = [&](int slot, int i) __attribute__((always_inline)) {
-            *reinterpret_cast<u32x4*>(lds + 3 * KBLK + slot * BLK + 1024 * (LPB * wv + i) + 16 * lane) = rv[i];
         };
         f32x16 sa, sb, o[DT];  // scores of a block's first and last 32 keys; products, [dim tile]
         float m_run = -INFINITY, mc = 0.f, l_run = 0.f;  // reference maximum, the same in the exponent (0: none yet), sum
@@ -981,27 +1070,37 @@ __global__ __launch_bounds__(512, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
             return join_halves(m);
         };
 
-        // Step n stores K(n + 2) and V(n + 1), loaded by step n - 1, under its second half, and loads K(n + 3) and V(n + 2) into
-        // the registers that this frees (behind the last block: the last one again, never read).
-        int s1, s2, s3;
-        uint32_t b0, b1, b2, b3;
+        // Step n stores K(n + 2) and V(n + 1) under its second half, loaded by step n - 2 (a block that is not in the XCD's L2
+        // takes about a step to arrive), and loads K(n + 4) and V(n + 3) into the registers that this frees (behind the last
+        // block: the last one again, never read).
+        using A0 = std::integral_constant<int, 0>;
+        using A1 = std::integral_constant<int, 1>;
+        int s1, s2, s3, s4;
+        uint32_t b0, b1, b2, b3, b4;
         locate(0, s1, b0);
-        load_k(s1);
-        load_v(s1);
+#pragma unroll
+        for (int i = 0; i < LPB; ++i) load_k(A0{}, i, s1), load_v(A0{}, i, s1);
         locate(min(1, nb - 1), s1, b1);
-        u32x4 r1[LPB];  // K(1), beside K(0)
 #pragma unroll
-        for (int i = 0; i < LPB; ++i) r1[i] = __builtin_amdgcn_raw_buffer_load_b128(k_rsrc, 16 * lane + 1024 * i, s1, 0);
+        for (int i = 0; i < LPB; ++i) load_k(A1{}, i, s1);
         locate(min(2, nb - 1), s2, b2);
+        locate(min(3, nb - 1), s3, b3);
         lds_barrier();  // the blocks of the piece before this one are read
-        store_k(0);
-        hide_v(0, b0);
+        hide_v(A0{}, 0, b0);
 #pragma unroll
-        for (int i = 0; i < LPB; ++i) store_v(0, i);
-        load_k(s2);
-        load_v(s1);
+        for (int i = 0; i < LPB; ++i) {
+            store_k(A0{}, i, 0);
+            load_k(A0{}, i, s2);
+            store_v(A0{}, i, 0);
+            load_v(A0{}, i, s1);
+        }
 #pragma unroll
-        for (int i = 0; i < LPB; ++i) *reinterpret_cast<u32x4*>(lds + KBLK + kst[i]) = r1[i];
+        for (int i = 0; i < LPB; ++i) {
+            store_k(A1{}, i, 1);
+            load_k(A1{}, i, s3);
+            load_v(A1{}, i, s2);
+        }
+        s4 = s3, b4 = b3;
         lds_barrier();
         if (nbw > 0) {
 #pragma unroll
@@ -1012,56 +1111,52 @@ __global__ __launch_bounds__(512, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
 #pragma unroll
             for (int i = 0; i < 2; ++i) kp[i] = *reinterpret_cast<const u32x4*>(lds + 32 * KR + kbase + 32 * i);
         }
-        int kslot = 0;  // n % 3
-        // one store or load of a K or V chunk: 4 LPB of them shared out over the parts of a half
-        auto move = [&](int ks, int vs, int sk, int sv, int part, int parts) __attribute__((always_inline)) {
-#pragma unroll
-            for (int x = 4 * LPB * part / parts; x < 4 * LPB * (part + 1) / parts; ++x) {
-                const int i = x >> 2;
-                if ((x & 3) == 0) *reinterpret_cast<u32x4*>(lds + ks * KBLK + kst[i]) = rk[i];
-                if ((x & 3) == 1) rk[i] = __builtin_amdgcn_raw_buffer_load_b128(k_rsrc, 16 * lane + 1024 * i, sk, 0);
-                if ((x & 3) == 2) store_v(vs, i);
-                if ((x & 3) == 3) rv[i] = __builtin_amdgcn_raw_buffer_load_b128(v_rsrc, 16 * lane + 1024 * i, sv, 0);
-            }
-        };
+        int kslot = 0, n = 0;  // kslot = n % 3
         auto none = [](int, int) {};
-        int n = 0;
-        // while every column sees all of this block and the next, all have pages and more follow: nothing to ask
-        const int plain = no_page ? 0 : min(nb - 3, (rq.seen + row_first) / KB - 1 - j0);
-        for (; n < plain; ++n) {
+        // PLAIN: every column sees all of this block and the next, all have pages, and more follow: nothing to ask
+        auto step = [&](auto set, auto plain) __attribute__((always_inline)) {
+            constexpr bool PLAIN = decltype(plain)::value;
             const int kslot1 = kslot == 2 ? 0 : kslot + 1, kslot2 = kslot1 == 2 ? 0 : kslot1 + 1, vslot = n & 1;
             if (n) lds_barrier();
-            locate(n + 3, s3, b3);
-            if (nbw > 0) {
-                follow(half(kslot, 1, sb, vslot, 0, sa, kslot1, 0, none));
-                follow(half(kslot1, 0, sa, vslot, 1, sb, kslot1, 1,
-                            [&](int part, int parts) { move(kslot2, 1 - vslot, s3, s2, part, parts); }));
-            } else {
-                move(kslot2, 1 - vslot, s3, s2, 0, 1);
-            }
-            s2 = s3, kslot = kslot1;
-            b0 = b1 = 0, b2 = b3;
-            if (no_page) {  // among the 16 blocks from n + 3 on
-                ++n;
-                break;
-            }
-        }
-        for (; n < nb; ++n) {
-            const int kslot1 = kslot == 2 ? 0 : kslot + 1, kslot2 = kslot1 == 2 ? 0 : kslot1 + 1, vslot = n & 1;
-            if (n) lds_barrier();
-            s3 = s2, b3 = b2;
-            if (n + 3 < nb) locate(n + 3, s3, b3);
-            if (n + 1 < nb) hide_v(n + 1, b1);
-            auto moves = [&](int part, int parts) { move(kslot2, 1 - vslot, s3, s2, part, parts); };
-            if (n < nbw) {
+            if (PLAIN || n + 4 < nb) locate(n + 4, s4, b4);
+            if (!PLAIN && n + 1 < nb) hide_v(set, n + 1, b1);
+            // one store or load of a chunk: 4 LPB of them shared out over the parts of a half
+            auto moves = [&](int part, int parts) __attribute__((always_inline)) {
+#pragma unroll
+                for (int x = 4 * LPB * part / parts; x < 4 * LPB * (part + 1) / parts; ++x) {
+                    const int i = x >> 2;
+                    if ((x & 3) == 0) store_k(set, i, kslot2);
+                    if ((x & 3) == 1) load_k(set, i, s4);
+                    if ((x & 3) == 2) store_v(set, i, 1 - vslot);
+                    if ((x & 3) == 3) load_v(set, i, s3);
+                }
+            };
+            if (PLAIN ? nbw > 0 : n < nbw) {
                 float mx = half(kslot, 1, sb, vslot, 0, sa, kslot1, 0, none);
-                settle(n, 1, b0, sb, mx);
+                if constexpr (PLAIN)
+                    follow(mx);
+                else
+                    settle(n, 1, b0, sb, mx);
                 mx = half(kslot1, 0, sa, vslot, 1, sb, kslot1, 1, moves);  // (scores behind the last block: not used)
-                settle(n + 1, 0, b1, sa, mx);
+                if constexpr (PLAIN)
+                    follow(mx);
+                else
+                    settle(n + 1, 0, b1, sa, mx);
             } else {
                 moves(0, 1);
             }
-            s2 = s3, b0 = b1, b1 = b2, b2 = b3, kslot = kslot1;
+            s3 = s4, b0 = b1, b1 = b2, b2 = b3, b3 = b4, kslot = kslot1, ++n;
+        };
+        const int plain = (b0 | b1 | b2 | b3) || no_page ? 0 : min(nb - 4, (rq.seen + row_first) / KB - 1 - j0);
+        while (n + 1 < plain && !no_page) {  // (no_page: among the 16 blocks from n + 3 on)
+            step(A0{}, std::true_type{});
+            step(A1{}, std::true_type{});
+        }
+        for (;;) {
+            step(A0{}, std::false_type{});
+            if (n >= nb) break;
+            step(A1{}, std::false_type{});
+            if (n >= nb) break;
         }
         {
             const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(l_run), __float_as_uint(l_run), false, false);
@@ -1081,62 +1176,34 @@ __global__ __launch_bounds__(512, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
                                        pack<T>(o[d][4 * e + 2] * inv, o[d][4 * e + 3] * inv));
             }
         };
-        const uint32_t begin = u - uint32_t(j0), end = begin + uint32_t(units);
-        if (begin >= u0 && end <= u1) {
+        // the item's parts: part i in slot base + i stride (+ 1 for the first, which its workgroup begins)
+        int base = 2 * lead, stride = 2 * kvh, first = 0;
+        if (!apart) {
+            const uint32_t begin = u - uint32_t(j0), end = begin + uint32_t(units);
+            auto group_of = [&](uint32_t x) { return int(((uint64_t(x) + 1) * G - 1) / total); };
+            lead = group_of(begin), parts = group_of(end - 1) - lead + 1, mine = int(w) - lead;
+            base = 2 * lead, stride = 2, first = 1;
+        }
+        if (parts == 1) {
             write();
         } else {
-            const uint32_t wa = group_of(begin), wb = group_of(end - 1);
-            // 16 bytes i of lane l: (4 DT wave + i) 64 + l, after the maxima and sums
-            auto at = [&](int slot, int i) {
-                return slot + 2 * int(paged::kTileCols) + ((wv * 4 * DT + i) * 64 + lane) * 4;
-            };
-            if (cw < cols) {
-                const int mine = slot_at(w, begin >= u0);
-                if (h == 0) store_part2(ws, mine + 2 * mycol, m_run, l_run);
+            if (mine == 0) {
+                describe(parts, base, stride, first, rq, row_first, cols, hk);
+                described = true;
+            }
+            if (cw < cols) {  // 16 bytes i of lane l: (4 DT wave + i) 64 + l, after the maxima and sums
+                const int slot = int(paged::kTileSlots) + (base + mine * stride + (mine ? 0 : first)) * SW;
+                if (h == 0) store_part2(ws, slot + 2 * mycol, m_run, l_run);
 #pragma unroll
                 for (int i = 0; i < 4 * DT; ++i) {
                     const f32x16& x = o[i >> 2];
                     const int e = 4 * (i & 3);
-                    store_part(ws, at(mine, i), f32x4{x[e], x[e + 1], x[e + 2], x[e + 3]});
+                    store_part(ws, slot + 2 * int(paged::kTileCols) + ((wv * 4 * DT + i) * 64 + lane) * 4,
+                               f32x4{x[e], x[e + 1], x[e + 2], x[e + 3]});
                 }
-            }
-            __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0): this wave's stores are performed
-            lds_barrier();
-            uint32_t* counter = a.ws + wa;
-            if (t == 0) arrived = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            lds_barrier();
-            if (arrived == wb - wa) {  // the last one in joins the parts, in their order
-                if (cw < cols) {
-                    m_run = -INFINITY, l_run = 0.f;
-#pragma unroll
-                    for (int d = 0; d < DT; ++d)
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
-                    for (uint32_t i = wa; i <= wb; ++i) {
-                        const int part = slot_at(i, i == wa);
-                        const float2 ml = load_part2(ws, part + 2 * mycol);
-                        f32x4 x[4 * DT];
-#pragma unroll
-                        for (int j = 0; j < 4 * DT; ++j) x[j] = load_part(ws, at(part, j));
-                        __builtin_amdgcn_sched_barrier(0);  // (all under way before the first is waited for)
-                        const float mn = fmaxf(m_run, ml.x), mnc = mn == -INFINITY ? 0.f : mn * a.scale_log2;
-                        const float fo = __builtin_amdgcn_exp2f(m_run * a.scale_log2 - mnc);
-                        const float fn = __builtin_amdgcn_exp2f(ml.x * a.scale_log2 - mnc);
-                        l_run = l_run * fo + ml.y * fn;
-                        m_run = mn;
-#pragma unroll
-                        for (int j = 0; j < 4 * DT; ++j)
-#pragma unroll
-                            for (int q = 0; q < 4; ++q) {
-                                const int e = 4 * (j & 3) + q;
-                                o[j >> 2][e] = o[j >> 2][e] * fo + x[j][q] * fn;
-                            }
-                    }
-                    write();
-                }
-                if (t == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             }
         }
+        if (apart) break;
         // ---- the next piece
         u += uint32_t(nb);
         kfirst = 0;
@@ -1146,10 +1213,74 @@ __global__ __launch_bounds__(512, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
                 hk = 0;
                 ++r;
                 while (r < int(a.requests) - 1 && uniform(int(ends[r])) == uniform(int(ends[r - 1]))) ++r;
-                rq = request_of(a, uint32_t(r));
-                rq.row0 = uniform(rq.row0), rq.rows = uniform(rq.rows), rq.seen = uniform(rq.seen);
+                enter(r);
             }
         }
+    }
+    if (!described) describe_none();
+}
+
+// The join of k_attn_tiles' split items: y = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i over an item's parts, in their
+// order. A launch of its own, for all CUs: the last workgroup of an item to end, if it joined them, would read 128 KiB a
+// part alone (1.5 us each, 12 us for the eight parts of a 512-row chunk at 8K). Block (item, wave of the tile): its four
+// waves take a quarter of each column's dims each.
+template <typename T, int HD>
+__global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {
+    constexpr int DT = HD / 32, N = DT;  // 16 bytes per lane and part
+    constexpr int SW = int(paged::slot_words(paged::kTileCols, HD));
+    const int lead = blockIdx.x >> 3, wv = blockIdx.x & 7, t = threadIdx.x, lane = t & 63, part_d = t >> 6, c32 = lane & 31;
+    const u32x4* d = reinterpret_cast<const u32x4*>(a.ws + paged::kGroups) + 2 * lead;
+    const u32x4 d0 = d[0], d1 = d[1];
+    const int parts = int(d0[0]), base = int(d0[1]), stride = int(d0[2]), first = int(d0[3]);
+    const int row0 = int(d1[0]), cols = int(d1[1]), hk = int(d1[2]), col = 32 * wv + c32;
+    if (parts == 0 || 32 * wv >= cols) return;
+    const __amdgpu_buffer_rsrc_t ws =
+        __builtin_amdgcn_make_buffer_rsrc(a.ws, 0, int(4 * (paged::kTileSlots + 2 * paged::kTileGroups * SW)), 0x00020000);
+    auto slot_at = [&](int i) { return int(paged::kTileSlots) + (base + i * stride + (i ? 0 : first)) * SW; };
+    constexpr int PF = 8;
+    float top = -INFINITY;
+    for (int i = 0; i < parts; i += PF) {
+        float2 ml[PF];
+#pragma unroll
+        for (int q = 0; q < PF; ++q) ml[q] = load_part2<0>(ws, slot_at(min(i + q, parts - 1)) + 2 * col);
+#pragma unroll
+        for (int q = 0; q < PF; ++q) top = fmaxf(top, ml[q].x);
+    }
+    const float tc = top == -INFINITY ? 0.f : top * a.scale_log2;
+    float l = 0.f, sum[4 * N];
+#pragma unroll
+    for (int e = 0; e < 4 * N; ++e) sum[e] = 0.f;
+    for (int i = 0; i < parts; i += PF) {
+        float2 ml[PF];
+        f32x4 x[PF][N];
+#pragma unroll
+        for (int q = 0; q < PF; ++q) {
+            const int slot = slot_at(min(i + q, parts - 1));
+            ml[q] = load_part2<0>(ws, slot + 2 * col);
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                x[q][j] = load_part<0>(ws, slot + 2 * int(paged::kTileCols) + ((wv * 4 * DT + part_d * N + j) * 64 + lane) * 4);
+        }
+        __builtin_amdgcn_sched_barrier(0);  // (all under way before the first is waited for)
+#pragma unroll
+        for (int q = 0; q < PF; ++q) {
+            const float f = i + q < parts ? __builtin_amdgcn_exp2f(ml[q].x * a.scale_log2 - tc) : 0.f;
+            if (i + q < parts) {
+                l += ml[q].y * f;
+#pragma unroll
+                for (int e = 0; e < 4 * N; ++e) sum[e] += x[q][e >> 2][e & 3] * f;
+            }
+        }
+    }
+    if (col >= cols) return;
+    const int group = int(a.qh / a.kvh);
+    const float inv = l != 0.f ? 1.0f / l : 0.f;  // no key at all: zeros
+    T* y = static_cast<T*>(a.y) + (size_t(row0 + col / group) * a.qh + hk * group + col % group) * HD + 4 * (lane >> 5);
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const int i = part_d * N + j;  // dims 32 (i / 4) + 8 (i % 4) + 4 h ..
+        *reinterpret_cast<uint2*>(y + 32 * (i >> 2) + 8 * (i & 3)) =
+            make_uint2(pack<T>(sum[4 * j] * inv, sum[4 * j + 1] * inv), pack<T>(sum[4 * j + 2] * inv, sum[4 * j + 3] * inv));
     }
 }
 
@@ -1243,8 +1374,10 @@ static void launch_attn(const uint32_t* w, void* const* p, hipStream_t s) {
     const uint32_t bytes = uint32_t(uint64_t(w[17]) * w[16] * w[13] * HD * 2);  // of each cache
     if (few_columns(w))
         hipLaunchKernelGGL((k_attn_rows<T, HD>), dim3(paged::kRowsGroups), dim3(256), 0, s, a, bytes, bytes);
-    else
+    else {
         hipLaunchKernelGGL((k_attn_tiles<T, HD>), dim3(paged::kTileGroups), dim3(512), 0, s, a, bytes);
+        hipLaunchKernelGGL((k_attn_join<T, HD>), dim3(paged::kTileGroups * 8), dim3(256), 0, s, a);
+    }
 }
 static void l_attn(const PreparedDispatch& pd, void* const* p, hipStream_t s) {
     const uint32_t* w = pd.words.data();

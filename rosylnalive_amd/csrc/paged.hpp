@@ -22,16 +22,19 @@ constexpr uint32_t kMaxRequests = 4096;
 
 inline bool page_ok(uint32_t page) { return page >= 16 && page <= 256 && (page & (page - 1)) == 0; }
 
-// attention_paged shares its work out in units, a block of keys of one item (query columns of one request on one KV head):
-// workgroup w of G takes the units [w units / G, (w + 1) units / G) of all items in order, whatever the lengths are. An item
-// that ends in another workgroup than it began in is joined from partials in the workspace. Word w counts the partials of
-// the item that workgroup w begins and does not end (zero between launches); after the kGroups counters, slot 2 w holds the
-// part of the item that w finds begun, slot 2 w + 1 the part of the one that it begins and does not end.
+// attention_paged shares its work out in units, a block of keys of one item (query columns of one request on one KV head).
+// Either every item has workgroups of its own, or workgroup w of G takes the units [w units / G, (w + 1) units / G) of all
+// items in order; both follow the lengths on the device. An item of several workgroups is joined from partials in the
+// workspace, two slots per workgroup: 2 w for the part of an item that w finds begun (or the part of its own), 2 w + 1 for
+// the part of the one that it begins and does not end. Before them stand kGroups words, in which the items of few columns
+// count their parts in (word w for the one that w begins; zero between launches), and for the items of many columns what
+// their join has to know, eight words per workgroup.
 constexpr uint32_t kGroups = 512;  // the most workgroups of a launch
 // Items of few columns (a request's rows x the heads of a group up to 16): two workgroups per CU, units of 128 keys.
 constexpr uint32_t kRowsGroups = 512, kRowsKeys = 128, kRowsCols = 16;
 // Items of many columns: one workgroup per CU, tiles of up to 256 columns, units of 64 keys.
 constexpr uint32_t kTileGroups = 256, kTileKeys = 64, kTileCols = 256;
+constexpr uint32_t kTileSlots = kGroups + 8 * kTileGroups;  // the word of the first slot
 // a slot: per column its maximum, its sum and its products
 constexpr uint64_t slot_words(uint64_t cols, uint64_t head_dim) { return cols * (2 + head_dim); }
 
@@ -41,7 +44,7 @@ inline uint64_t workspace_words(uint64_t requests, uint64_t tokens, uint64_t q_h
                                 uint64_t head_dim) {
     (void)requests;
     const uint64_t rows = kGroups + 2 * kRowsGroups * slot_words(kRowsCols, head_dim);
-    const uint64_t tiles = kGroups + 2 * kTileGroups * slot_words(kTileCols, head_dim);
+    const uint64_t tiles = kTileSlots + 2 * kTileGroups * slot_words(kTileCols, head_dim);
     return kv_heads && tokens * (q_heads / kv_heads) <= kRowsCols ? rows : (tiles > rows ? tiles : rows);
 }
 
