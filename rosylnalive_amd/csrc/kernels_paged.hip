@@ -388,6 +388,41 @@ __device__ __forceinline__ float2 load_part2(__amdgpu_buffer_rsrc_t r, int word)
 }
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
+// Values that are no finite numbers, at keys that one column of a tile sees and another does not: zero times such a value is
+// NaN, so they are taken out of the product and added to the columns that see them alone. A second product with 0 / 1
+// weights counts them: infinity as 1, minus infinity as 128, NaN as both; fewer than 128 keys, so float32 holds the counts.
+template <typename T>
+constexpr uint32_t kExponent = std::is_same_v<T, __bf16> ? 0x7F80u : 0x7C00u;
+template <typename T>
+__device__ __forceinline__ bool take_odd(u32x4& v) {  // zeroes them; whether there were any
+    constexpr uint32_t lo = kExponent<T>, hi = lo << 16;
+    bool any = false;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const bool l = (v[e] & lo) == lo, h = (v[e] & hi) == hi;
+        v[e] &= (l ? 0u : 0x0000FFFFu) | (h ? 0u : 0xFFFF0000u);
+        any = any || l || h;
+    }
+    return any;
+}
+template <typename T>
+__device__ __forceinline__ u32x4 odd_codes(u32x4 v) {
+    constexpr uint32_t exp = kExponent<T>;
+    auto code = [](uint32_t x) {
+        return (x & exp) != exp ? 0.f : (x & (0x7FFFu ^ exp)) ? 129.f : (x & 0x8000u) ? 128.f : 1.f;
+    };
+    u32x4 c;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c[e] = pack<T>(code(v[e] & 0xFFFFu), code(v[e] >> 16));
+    return c;
+}
+__device__ __forceinline__ float add_odd(float o, float count) {
+    const uint32_t n = uint32_t(count);
+    if (n & 127u) o += INFINITY;
+    if (n >> 7) o -= INFINITY;
+    return o;
+}
+
 // Rows of few query columns: up to 16 per request and KV head (column c = row c / group, head c % group of the KV head's).
 // Bound by the cache's bytes, so every wave streams its own keys straight into the registers that the matrix
 // instruction reads (no LDS, no barrier), two units in flight, and the four waves of a workgroup meet once per item.
@@ -520,6 +555,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(AttnArgs a, uint32_t k_byt
             s0 = M::m16(kr[S][s], qf[s], s0);
             s1 = M::m16(kr[S][KS + s], qf[s], s1);
         }
+        bool odd = false;  // some value that not all columns see is no finite number
         float sc[8];  // keys kb + 8 g ..
 #pragma unroll
         for (int e = 0; e < 4; ++e) sc[e] = s0[e], sc[4 + e] = s1[e];
@@ -535,6 +571,14 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(AttnArgs a, uint32_t k_byt
                     keep[e] = (2 * e < left ? 0x0000FFFFu : 0u) | (2 * e + 1 < left ? 0xFFFF0000u : 0u);
 #pragma unroll
                 for (int d = 0; d < DT; ++d) vr[S][d] &= keep;
+            }
+            if (p.keys > p.seen) {
+#pragma unroll
+                for (int d = 0; d < DT; ++d) {
+                    u32x4 x = vr[S][d];
+                    odd |= take_odd<T>(x);
+                }
+                odd = __any(odd);
             }
         }
         float mx = fmaxf(fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3])), fmaxf(fmaxf(sc[4], sc[5]), fmaxf(sc[6], sc[7])));
@@ -557,7 +601,19 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(AttnArgs a, uint32_t k_byt
         // the weights go into the product rounded to the cache's type, as its values are; their sum stays float32
         const u32x4 pb = {pack<T>(sc[0], sc[1]), pack<T>(sc[2], sc[3]), pack<T>(sc[4], sc[5]), pack<T>(sc[6], sc[7])};
 #pragma unroll
-        for (int d = 0; d < DT; ++d) o[d] = M::m16(vr[S][d], pb, o[d]);
+        for (int d = 0; d < DT; ++d) {
+            if (odd) {
+                const int lim = p.seen + c16 / group - kb - 8 * g;
+                u32x4 sees;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sees[e] = pack<T>(2 * e < lim ? 1.f : 0.f, 2 * e + 1 < lim ? 1.f : 0.f);
+                const f32x4 counts = M::m16(odd_codes<T>(vr[S][d]), sees, f32x4{0.f, 0.f, 0.f, 0.f});
+                take_odd<T>(vr[S][d]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[d][e] = add_odd(o[d][e], counts[e]);
+            }
+            o[d] = M::m16(vr[S][d], pb, o[d]);
+        }
     };
 
     // ---- the end of an item here: the waves' parts meet in LDS, then y, or a partial and the join
@@ -753,6 +809,7 @@ __global__ __launch_bounds__(512, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
     __shared__ uint32_t red[8];
     __shared__ uint32_t units_of_tile[paged::kTileGroups];
     __shared__ int chosen[3];
+    __shared__ uint32_t odd;  // the first unit of the last piece that held values to take out
     const int t = threadIdx.x, lane = t & 63, wv = uniform(t >> 6), c32 = lane & 31, h = lane >> 5;
     const int group = int(a.qh / a.kvh), kvh = int(a.kvh), TR = int(paged::kTileCols) / group;
 
@@ -784,6 +841,7 @@ __global__ __launch_bounds__(512, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
         for (uint32_t r = r0; r < r1; ++r) ends[r] += before;
         __syncthreads();
     };
+    if (t == 0) odd = ~0u;
     Request rq{};
     auto enter = [&](int r) {
         rq = request_of(a, uint32_t(r));
@@ -963,6 +1021,7 @@ __global__ __launch_bounds__(512, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
             *reinterpret_cast<u32x4*>(lds + 3 * KBLK + slot * BLK + 1024 * (LPB * wv + i) + 16 * lane) =
                 rv[decltype(set)::value][i];
         };
+        const int tile_seen = rq.seen + row_first;  // keys that the tile's first row sees: all of its columns do
         auto hide_v = [&](auto set, int j, uint32_t bad) __attribute__((always_inline)) {
             const int left = keys - (j0 + j) * KB;  // keys of the block that any column sees
             if (left < KB || bad) {  // uniform: what is hidden may be anything, and zero times NaN is NaN
@@ -973,6 +1032,12 @@ __global__ __launch_bounds__(512, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
                     for (int e = 0; e < 4; ++e)
                         rv[decltype(set)::value][i][e] &= (2 * e < in ? 0x0000FFFFu : 0u) | (2 * e + 1 < in ? 0xFFFF0000u : 0u);
                 }
+            }
+            if ((j0 + j + 1) * KB > tile_seen) {
+                bool any = false;
+#pragma unroll
+                for (int i = 0; i < LPB; ++i) any |= take_odd<T>(rv[decltype(set)::value][i]);
+                if (any) odd = u;
             }
         };
         f32x16 sa, sb, o[DT];  // scores of a block's first and last 32 keys; products, [dim tile]
@@ -1161,6 +1226,31 @@ __global__ __launch_bounds__(512, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
         {
             const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(l_run), __float_as_uint(l_run), false, false);
             l_run = __uint_as_float(x[0]) + __uint_as_float(x[1]);
+        }
+
+        if (uint32_t(uniform(int(odd))) == u) {  // adds the values that hide_v has taken out, from the cache once more
+            const int end = min((j0 + nb) * KB, keys);
+#pragma unroll 1
+            for (int k = max(j0 * KB, tile_seen / KB * KB); k < end; k += 16) {
+                const uint32_t id = uint32_t(uniform(int(trow[min(uint32_t(k) >> a.page_log2, a.blocks - 1)])));
+                if (id >= a.pages) continue;
+                const int soff = int((((id * uint32_t(kvh) + hk) << a.page_log2) + (uint32_t(k) & ((1u << a.page_log2) - 1))) * RB);
+                const int lim = vis - k - 8 * h;
+                u32x4 sees;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sees[e] = pack<T>(2 * e < lim ? 1.f : 0.f, 2 * e + 1 < lim ? 1.f : 0.f);
+#pragma unroll
+                for (int d = 0; d < DT; ++d) {
+                    f32x16 counts;
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) counts[e] = 0.f;
+                    const u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(v_rsrc, 8 * RB * h + 512 * d + 16 * c32, soff, 0);
+                    counts = M::m32(odd_codes<T>(x), sees, counts);
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) o[d][e] = add_odd(o[d][e], counts[e]);
+                    __builtin_amdgcn_sched_barrier(0);  // (one tile of counts at a time)
+                }
+            }
         }
 
         auto write = [&]() __attribute__((always_inline)) {

@@ -200,7 +200,7 @@ def test_append_extreme_values():
 # ---------------------------------------------------------------- attention
 
 def _attn_case(dtype, qh, kvh, hd, page, lens, *, pad=0, max_fresh=0, context=None, spoil=None, std=1.0, seed=0, spare=3,
-               scale=None, values=None, twice=True):
+               scale=None, values=None, twice=True, check=True):
     """lens: (cached, new) of each request. Every position that no request may read (spare pages, the end of the last page)
     holds NaN. spoil(table, pages): changes the table's entries. values(q, kc, vc, table): changes the inputs."""
     r = np.random.default_rng([seed, len(lens), hd, qh])
@@ -251,6 +251,8 @@ def _attn_case(dtype, qh, kvh, hd, page, lens, *, pad=0, max_fresh=0, context=No
     finally:
         s.close()
     assert all(x.tobytes() == runs[0].tobytes() for x in runs)
+    if not check:
+        return f(dtype, runs[0])
     want, bound = O.attention(f(dtype, qb), f(dtype, kb), f(dtype, vb), table, starts, ctx, qh, kvh, hd, page, pages, blocks, T,
                               max_fresh or T, float(np.float32(sc)), dtype, np.zeros(y0.shape))
     mine = bound >= 0
@@ -384,6 +386,61 @@ def test_attention_scores(dtype, fresh):
         _attn_case(d, 4, 2, 128, 16, lens, values=change)
     _attn_case(d, 4, 2, 64, 16, lens, scale=30.0, seed=2)
     _attn_case(d, 4, 2, 64, 16, lens, scale=1e-4, seed=2)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("lens", [[(40, 2), (0, 3), (130, 4)], [(300, 90), (0, 77), (63, 5)], [(1900, 129), (5, 20)],
+                                  [(100, 200)] * 40], ids=["few", "chunks", "long", "many"])
+def test_attention_values_that_are_not_finite(dtype, hd, lens):
+    """Infinities and NaN among a chunk's own values reach the rows that see them, in their dim of their head, and change no
+    bit of any other row: what a row gives does not depend on the tokens after it."""
+    qh, kvh, page, at = 4, 2, 16, []
+    r = np.random.default_rng(5)
+    for i, (past, new) in enumerate(lens):
+        for j in {0, 1, new // 2, new - 1}:
+            for x in (np.inf, -np.inf, np.nan):
+                at.append((i, past + j, int(r.integers(kvh)), int(r.integers(hd)), x))
+        at.append((i, past + new - 1, 0, at[-1][3], np.inf))
+
+    def put(odd):
+        def change(q, kc, vc, table):
+            for i, pos, h, d, x in at:
+                vc[table[i, pos // page], h, pos % page // 8, d, pos % 8] = x if odd else 0.0
+        return change
+
+    d = DT[dtype]
+    plain = _attn_case(d, qh, kvh, hd, page, lens, std=0.3, values=put(False), twice=False)
+    got = _attn_case(d, qh, kvh, hd, page, lens, std=0.3, values=put(True), check=False)
+    add = np.zeros(plain.shape)
+    first = np.concatenate([[0], np.cumsum([n for _, n in lens])])
+    last = {(i, pos, h, dim): x for i, pos, h, dim, x in at}  # (a later entry takes the place of an earlier one)
+    with np.errstate(invalid="ignore"):
+        for (i, pos, h, dim), x in last.items():
+            for g in range(2 * h, 2 * h + 2):
+                add[first[i] + pos - lens[i][0]:first[i + 1], g * hd + dim] += x
+    want = np.where(add == 0, plain, add)
+    assert np.array_equal(got, want, equal_nan=True), np.argwhere(~((got == want) | (np.isnan(got) & np.isnan(want))))[:5]
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("lens", [[(40, 2), (0, 3), (130, 4)], [(300, 90), (0, 77), (1900, 129)]], ids=["few", "chunks"])
+@pytest.mark.parametrize("x", [np.nan, np.inf])
+def test_attention_keys_that_are_not_finite(dtype, lens, x):
+    """A chunk's last key, if it is NaN or infinite, changes no bit of the rows before it."""
+    def put(x):
+        def change(q, kc, vc, table):
+            for i, (past, new) in enumerate(lens):
+                pos = past + new - 1
+                kc[table[i, pos // 16], :, pos % 16] = x
+        return change
+
+    d = DT[dtype]
+    plain = _attn_case(d, 4, 2, 128, 16, lens, values=put(0.0), twice=False)
+    got = _attn_case(d, 4, 2, 128, 16, lens, values=put(x), check=False)
+    ends = np.cumsum([n for _, n in lens])
+    before = np.setdiff1d(np.arange(ends[-1]), ends - 1)
+    assert np.array_equal(got[before], plain[before])
 
 
 def test_attention_replayed_with_other_lengths():
