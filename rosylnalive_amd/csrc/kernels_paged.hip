@@ -864,12 +864,15 @@ __global__ __launch_bounds__(512, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
         describe_none();
         return;
     }
-    const bool apart = uint64_t(tiles_all) * kvh <= paged::kTileGroups;
+    bool apart = uint64_t(tiles_all) * kvh <= paged::kTileGroups;
+    uint32_t q = 0;
     if (apart) {
         // No more items than workgroups: each gets ceil(units / q) of its own, q the least that fits, so no workgroup starts
-        // more than one piece (a start takes 4 us, the time of two units). More parts than the square root of half the
-        // longest item's units are not worth their join (about 1 us a part). All heads of a tile split alike; neighbouring
-        // workgroups, which run on different XCDs, take different heads.
+        // more than one piece (a start takes 4 us, the time of two units at head_dim 128). More parts than the square root of
+        // half the longest item's units are not worth their join. All heads of a tile split alike; neighbouring workgroups,
+        // which run on different XCDs, take different heads. Where whole workgroups fit the lengths badly, q far above the
+        // mean, units shared out evenly are faster in spite of the second start: measured 171 us apart and 129 even at
+        // q / mean = 1.85, 68 and 68 at 1.5, 88 and 94 at 1.67, 47 and 58 at 1.3.
         if (uint32_t(t) < tiles_all) {
             const int i = first_above(ends, int(a.requests), uint32_t(t));
             units_of_tile[t] = uint32_t(tile_units(request_of(a, uint32_t(i)), t - int(i ? ends[i - 1] : 0)));
@@ -886,6 +889,7 @@ __global__ __launch_bounds__(512, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
         }
         const uint32_t room = paged::kTileGroups / uint32_t(kvh);
         uint32_t hi = uint32_t(uniform(int(wave_max(most)))), lo = uint32_t(uniform(int(wave_sum(sum)))) / room;
+        const uint32_t even = lo;
         lo = min(max(max(lo, 1u), uint32_t(sqrtf(0.5f * float(hi)))), hi);
         while (lo < hi) {
             const uint32_t q = (lo + hi) >> 1;
@@ -903,7 +907,11 @@ __global__ __launch_bounds__(512, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
             else
                 lo = q + 1;
         }
-        const uint32_t own = uint32_t(t) < tiles_all ? (units_of_tile[t] + hi - 1) / hi : 0u, end = scan_sat(own, red);
+        q = hi;
+        apart = 4 * q <= 7 * even + 12;
+    }
+    if (apart) {
+        const uint32_t own = uint32_t(t) < tiles_all ? (units_of_tile[t] + q - 1) / q : 0u, end = scan_sat(own, red);
         hk = int(w) % kvh;
         const uint32_t place = w / uint32_t(kvh);
         if (t == 0) chosen[0] = -1;
@@ -1321,13 +1329,13 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {
     const int lead = blockIdx.x >> 3, wv = blockIdx.x & 7, t = threadIdx.x, lane = t & 63, part_d = t >> 6, c32 = lane & 31;
     const u32x4* d = reinterpret_cast<const u32x4*>(a.ws + paged::kGroups) + 2 * lead;
     const u32x4 d0 = d[0], d1 = d[1];
-    const int parts = int(d0[0]), base = int(d0[1]), stride = int(d0[2]), first = int(d0[3]);
+    const int parts = uniform(int(d0[0])), base = uniform(int(d0[1])), stride = uniform(int(d0[2])), first = uniform(int(d0[3]));
     const int row0 = int(d1[0]), cols = int(d1[1]), hk = int(d1[2]), col = 32 * wv + c32;
     if (parts == 0 || 32 * wv >= cols) return;
     const __amdgpu_buffer_rsrc_t ws =
         __builtin_amdgcn_make_buffer_rsrc(a.ws, 0, int(4 * (paged::kTileSlots + 2 * paged::kTileGroups * SW)), 0x00020000);
     auto slot_at = [&](int i) { return int(paged::kTileSlots) + (base + i * stride + (i ? 0 : first)) * SW; };
-    constexpr int PF = 8;
+    constexpr int PF = 6;
     float top = -INFINITY;
     for (int i = 0; i < parts; i += PF) {
         float2 ml[PF];
@@ -1345,7 +1353,8 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {
         f32x4 x[PF][N];
 #pragma unroll
         for (int q = 0; q < PF; ++q) {
-            const int slot = slot_at(min(i + q, parts - 1));
+            if (i + q >= parts) break;
+            const int slot = slot_at(i + q);
             ml[q] = load_part2<0>(ws, slot + 2 * col);
 #pragma unroll
             for (int j = 0; j < N; ++j)
@@ -1354,12 +1363,11 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {
         __builtin_amdgcn_sched_barrier(0);  // (all under way before the first is waited for)
 #pragma unroll
         for (int q = 0; q < PF; ++q) {
-            const float f = i + q < parts ? __builtin_amdgcn_exp2f(ml[q].x * a.scale_log2 - tc) : 0.f;
-            if (i + q < parts) {
-                l += ml[q].y * f;
+            if (i + q >= parts) break;
+            const float f = __builtin_amdgcn_exp2f(ml[q].x * a.scale_log2 - tc);
+            l += ml[q].y * f;
 #pragma unroll
-                for (int e = 0; e < 4 * N; ++e) sum[e] += x[q][e >> 2][e & 3] * f;
-            }
+            for (int e = 0; e < 4 * N; ++e) sum[e] += x[q][e >> 2][e & 3] * f;
         }
     }
     if (col >= cols) return;

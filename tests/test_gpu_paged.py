@@ -314,6 +314,12 @@ def test_attention_request_limits(requests):
     _attn_case(F16, 1, 1, 64, 16, [(i % 5, i % 2) for i in range(1, requests + 1)], pad=1)
 
 
+@pytest.mark.parametrize("short", [9, 24])
+def test_attention_uneven_requests(short):
+    """Few items of very different lengths: with workgroups of their own each, and with too few left for the long ones."""
+    _attn_case(F16, 8, 8, 64, 32, [(3 * i, 2) for i in range(short)] + [(4000, 30), (3900, 17), (4100, 1)], pad=3)
+
+
 def test_attention_rows_without_keys():
     """A context shorter than the new rows: the first of them see nothing and give zeros; a request with no context; a
     context past the table."""
