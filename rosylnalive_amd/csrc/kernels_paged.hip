@@ -898,8 +898,8 @@ __global__ __launch_bounds__(512, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 if (j >= held) continue;
-                uint32_t c = uint32_t(float(n[j]) * by);  // n / q but for the last place
-                c += uint32_t(c * q < n[j]), c -= uint32_t(c > 0 && (c - 1) * q >= n[j]);
+                uint32_t c = uint32_t(float(n[j]) * by);  // n / q but for one (n is below 2^24 + 1)
+                c += uint32_t(c * q < n[j]), c += uint32_t(c * q < n[j]), c -= uint32_t(c > 0 && (c - 1) * q >= n[j]);
                 need += float(c);
             }
             if (uint32_t(uniform(int(wave_sum(need)))) <= room)
