@@ -813,19 +813,21 @@ __global__ __launch_bounds__(512, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
     const int t = threadIdx.x, lane = t & 63, wv = uniform(t >> 6), c32 = lane & 31, h = lane >> 5;
     const int group = int(a.qh / a.kvh), kvh = int(a.kvh), TR = int(paged::kTileCols) / group;
 
+    constexpr int kStart = int(paged::kTileStart);
     // ---- the units of every request, and this workgroup's
     // blocks of 64 keys of a request's first n tiles on one KV head: tile i's last row sees seen + min((i + 1) TR, rows) - 1
-    // keys, at least one block. All full tiles but the clamped ones follow a slope.
+    // keys, at least one block. All full tiles but the clamped ones follow a slope. In even shares a tile weighs kStart units
+    // more than it has, for its start.
     auto tile_keys = [&](const Request& q, int i) { return max(0, q.seen + min((i + 1) * TR, q.rows) - 1); };
     auto tile_units = [&](const Request& q, int i) { return max(1, (tile_keys(q, i) + KB - 1) / KB); };
-    auto first_units = [&](const Request& q, int n) {
+    auto first_weight = [&](const Request& q, int n) {
         const int full = min(n, q.rows / TR);
         // tiles of one block: seen + (i + 1) TR - 1 <= 64
         const int ones = min(full, max(0, (KB + 1 - q.seen) / TR));
         uint32_t sum = uint32_t(ones);
         if (full > ones) sum += floor_sum64(uint32_t(full - ones), uint32_t(TR), uint32_t(q.seen + (ones + 1) * TR - 1 + KB - 1));
         if (n > full) sum += uint32_t(tile_units(q, full));
-        return sum;
+        return sum + uint32_t(n * kStart);
     };
     auto tiles_of = [&](const Request& q) { return (q.rows + TR - 1) / TR; };
     // ends[r] = the sum of f over the requests up to and with r
@@ -848,7 +850,8 @@ __global__ __launch_bounds__(512, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
         rq.row0 = uniform(rq.row0), rq.rows = uniform(rq.rows), rq.seen = uniform(rq.seen);
     };
     int r = 0, hk = 0, tile = 0, kfirst = 0;
-    uint32_t u0 = 0, u1 = 0, total = 0, G = 0, w = blockIdx.x;  // (units of all items; not used where each has its own workgroups)
+    uint32_t u1 = 0, total = 0, G = 0, w = blockIdx.x;  // (weights of all items; not used where each has its own workgroups)
+    uint32_t begin = 0;                                 // the weight before the item under way
     int parts = 0, mine = 0, lead = 0;                          // of an item with workgroups of its own
     // what the join has to know of a split item: written by the workgroup that begins it, by the others as none
     auto describe = [&](int parts, int base, int stride, int first, const Request& q, int row_first, int cols, int hk) {
@@ -929,7 +932,7 @@ __global__ __launch_bounds__(512, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
         enter(r);
     } else {
         __syncthreads();
-        scan_requests([&](const Request& q) { return first_units(q, tiles_of(q)) * uint32_t(kvh); });
+        scan_requests([&](const Request& q) { return first_weight(q, tiles_of(q)) * uint32_t(kvh); });
         total = ends[a.requests - 1], G = min(uint32_t(gridDim.x), total);
         // workgroups of one XCD (every eighth) take neighbouring units, which share a KV head's blocks in its L2
         if (G == paged::kTileGroups) w = (blockIdx.x % 8) * (paged::kTileGroups / 8) + blockIdx.x / 8;
@@ -937,22 +940,24 @@ __global__ __launch_bounds__(512, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
             describe_none();
             return;
         }
-        u0 = uint32_t(uint64_t(total) * w / G), u1 = uint32_t(uint64_t(total) * (w + 1) / G);
+        const uint32_t u0 = uint32_t(uint64_t(total) * w / G);
+        u1 = uint32_t(uint64_t(total) * (w + 1) / G);
         r = uniform(first_above(ends, int(a.requests), u0));
         enter(r);
         uint32_t in = u0 - (r ? uint32_t(uniform(int(ends[r - 1]))) : 0u);
         const int tiles = tiles_of(rq);
-        const uint32_t per_head = uint32_t(uniform(int(first_units(rq, tiles))));
+        const uint32_t per_head = uint32_t(uniform(int(first_weight(rq, tiles))));
         hk = int(in / per_head), in %= per_head;
         int lo = 0, hi = tiles - 1;  // the last tile whose first unit is at or before `in`
         while (lo < hi) {
             const int m = (lo + hi + 1) >> 1;
-            if (first_units(rq, m) <= in)
+            if (first_weight(rq, m) <= in)
                 lo = m;
             else
                 hi = m - 1;
         }
-        tile = uniform(lo), kfirst = uniform(int(in - first_units(rq, lo)));
+        in = uint32_t(uniform(int(in - first_weight(rq, lo))));
+        tile = uniform(lo), kfirst = max(0, int(in) - kStart), begin = u0 - in;
     }
 
     const __amdgpu_buffer_rsrc_t k_rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(a.kc), 0, bytes, 0x00020000);
@@ -973,11 +978,12 @@ __global__ __launch_bounds__(512, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
         __builtin_amdgcn_make_buffer_rsrc(a.ws, 0, int(4 * (paged::kTileSlots + 2 * paged::kTileGroups * SW)), 0x00020000);
     bool described = false;
 
-    for (uint32_t u = u0; apart || u < u1;) {
+    for (;;) {
         // ---- a piece: blocks j0 .. j0 + nb - 1 of a tile
         const int units = tile_units(rq, tile), keys = tile_keys(rq, tile);
         const int j0 = apart ? int(uint64_t(uint32_t(units)) * mine / parts) : kfirst;
-        const int nb = apart ? int(uint64_t(uint32_t(units)) * (mine + 1) / parts) - j0 : min(units - j0, int(u1 - u));
+        const int nb = apart ? int(uint64_t(uint32_t(units)) * (mine + 1) / parts) - j0 : min(units, int(u1 - begin) - kStart) - j0;
+        if (nb <= 0) break;  // (the start of an item, and none of its units)
         const int row_first = tile * TR, cols = min(TR, rq.rows - row_first) * group;
         const int cw = 32 * wv;  // this wave's first column
         // blocks that some column of the wave sees
@@ -1045,7 +1051,7 @@ __global__ __launch_bounds__(512, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
                 bool any = false;
 #pragma unroll
                 for (int i = 0; i < LPB; ++i) any |= take_odd<T>(rv[decltype(set)::value][i]);
-                if (any) odd = u;
+                if (any) odd = begin;
             }
         };
         f32x16 sa, sb, o[DT];  // scores of a block's first and last 32 keys; products, [dim tile]
@@ -1236,7 +1242,7 @@ __global__ __launch_bounds__(512, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
             l_run = __uint_as_float(x[0]) + __uint_as_float(x[1]);
         }
 
-        if (uint32_t(uniform(int(odd))) == u) {  // adds the values that hide_v has taken out, from the cache once more
+        if (uint32_t(uniform(int(odd))) == begin) {  // adds the values that hide_v has taken out, from the cache once more
             const int end = min((j0 + nb) * KB, keys);
 #pragma unroll 1
             for (int k = max(j0 * KB, tile_seen / KB * KB); k < end; k += 16) {
@@ -1277,9 +1283,9 @@ __global__ __launch_bounds__(512, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
         // the item's parts: part i in slot base + i stride (+ 1 for the first, which its workgroup begins)
         int base = 2 * lead, stride = 2 * kvh, first = 0;
         if (!apart) {
-            const uint32_t begin = u - uint32_t(j0), end = begin + uint32_t(units);
+            const uint32_t unit0 = begin + uint32_t(kStart);
             auto group_of = [&](uint32_t x) { return int(((uint64_t(x) + 1) * G - 1) / total); };
-            lead = group_of(begin), parts = group_of(end - 1) - lead + 1, mine = int(w) - lead;
+            lead = group_of(unit0), parts = group_of(unit0 + uint32_t(units) - 1) - lead + 1, mine = int(w) - lead;
             base = 2 * lead, stride = 2, first = 1;
         }
         if (parts == 1) {
@@ -1303,9 +1309,10 @@ __global__ __launch_bounds__(512, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
         }
         if (apart) break;
         // ---- the next piece
-        u += uint32_t(nb);
+        begin += uint32_t(kStart + units);
         kfirst = 0;
-        if (u < u1 && ++tile >= tiles_of(rq)) {
+        if (begin + uint32_t(kStart) >= u1) break;
+        if (++tile >= tiles_of(rq)) {
             tile = 0;
             if (++hk >= kvh) {
                 hk = 0;
@@ -1630,7 +1637,8 @@ std::vector<KernelSpec> paged_catalog() {
                          contract_fail("%s: at most %u query heads per KV head", n, paged::kTileCols);
                      // units: a tile of a request's rows (at least one a request) x the blocks of keys, on every KV head
                      const uint64_t tiles = R + uint64_t(T) / (paged::kTileCols / (qh / kvh));
-                     if (times(few_columns(w) ? R : tiles, kvh, uint64_t(blocks) * page / paged::kTileKeys + 1) > 1ull << 31)
+                     if (times(few_columns(w) ? R : tiles, kvh,
+                               uint64_t(blocks) * page / paged::kTileKeys + 1 + paged::kTileStart) > 1ull << 31)
                          contract_fail("%s: rows * kv_heads * blocks * page are more than one dispatch shares out", n);
                      need(c, 0, times(T, qh, hd), n, "q");
                      need(c, 1, times(uint64_t(pages) * page, kvh, hd), n, "k_cache");
