@@ -135,10 +135,39 @@ int lrm_hip_contains(lrm_hip_device *d, uint32_t kernel); /* 1 or 0 */
 int lrm_hip_debug_gemm_stamps(lrm_hip_device *d, uint32_t kind, uint64_t *dst, uint64_t words);
 int lrm_hip_denormal_probe(lrm_hip_device *d, int *mode, uint32_t results[7]);
 
-/* The paged key/value cache (ids 47 paged_plan, 48 qk_norm_rope_append_paged, 49 attention_paged; no counterpart in the
- * reference, whose cache is one sequence's rows): u32 words of attention_paged's workspace for dispatches of up to that many
- * requests and tokens. The workspace's words must be zero before the first launch (a new heap's are); every launch leaves
- * the ones that it counts in at zero. Dispatches that may overlap need a workspace each. */
+/* The paged key/value cache (ids 47 paged_plan, 48 qk_norm_rope_append_paged, 49 attention_paged, in the fast set; no
+ * counterpart in the reference, whose cache is one sequence's rows). A page holds `page` positions (a power of two, 16 to
+ * 256) of every KV head, head_dim 64 or 128, fp16 or bf16:
+ *   k_cache [pages][kv_heads][page][head_dim], v_cache [pages][kv_heads][page / 8][head_dim][8] (8 positions innermost; as a
+ *   table row of rank 4, its last dimension is 8 head_dim);
+ *   table [requests][blocks]: the page of each `page` positions of a request; 0xFFFFFFFF (any id >= pages) is none;
+ *   starts [requests + 1]: request r's new rows are starts[r] .. starts[r + 1] - 1 of the batch's `tokens` rows (not
+ *   decreasing); context [requests]: its positions, the new ones included.
+ * Lengths are device memory: one recorded list serves every step, padded to `tokens` rows and `requests` requests (a request
+ * of no new rows costs nothing). Rows behind the last request's are left as they were. requests is at most 4096, blocks *
+ * page at most 2^30. Indices from device memory that point nowhere are skipped, never followed.
+ *
+ * 47 paged_plan: past, fresh [requests] (cached and new positions), free [free_count] (page ids, taken in order), table
+ *   (read and completed), then starts, context, positions [tokens], slots [tokens] (page id * page + offset, 0xFFFFFFFF where a
+ *   row has none) and counts [3]: rows, pages taken (both of what was asked for), and bits 1 more rows than `tokens`, 2 a
+ *   request longer than blocks * page, 4 the free pages ran out. Sums of lengths saturate at 2^32 - 1. Entries of the table
+ *   that hold no new position are not written; where the free pages end, entries and slots are none. The plan of a request
+ *   that bit 1, 2 or 4 speaks of does not hold (its context counts positions that have no row or no page): the step is planned
+ *   again with fewer rows, or its rows are not used.
+ * 48 qk_norm_rope_append_paged: qkv [tokens][(q_heads + 2 kv_heads) head_dim] (float32, or the cache's type), q_norm and k_norm
+ *   [head_dim], cos_table and sin_table [max_pos][head_dim / 2]: per head x w / sqrt(mean x^2 + eps), rotated by the row's
+ *   position, q [tokens][q_heads head_dim] and the caches' entries at the row's slot; values as they are. Rows of the batch
+ *   are the first starts[requests]. A row whose position is not below max_pos gives zeros and appends nothing; one without a
+ *   slot gives q and appends nothing. Slots are distinct: where two rows name one, it is not said whose parts stay.
+ * 49 attention_paged: y = softmax(scale q k^T) v of the new rows, causal (row i of a request sees context - new + i + 1
+ *   positions; positions whose page is none are left out; a row that sees none gives zeros), any number of rows per request in
+ *   one dispatch. max_fresh: 0, or the most rows of a request: with max_fresh * q_heads / kv_heads <= 16 the form for single
+ *   tokens runs (rows past max_fresh are left as they were). q_heads / kv_heads is at most 256. The same lengths give the same
+ *   bits. What a row gives does not depend on the tokens behind it, whatever they hold.
+ *
+ * u32 words of attention_paged's workspace for dispatches of up to that many requests and tokens. The workspace's words must
+ * be zero before the first launch (a new heap's are); every launch leaves the ones that it counts in at zero, so lists with
+ * other lengths, tokens or max_fresh may share it one after the other. Dispatches that may overlap need a workspace each. */
 int lrm_attention_paged_workspace(uint32_t requests, uint32_t tokens, uint32_t q_heads, uint32_t kv_heads,
                                   uint32_t head_dim, uint64_t *words);
 

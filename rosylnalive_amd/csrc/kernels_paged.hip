@@ -60,7 +60,8 @@ __device__ __forceinline__ int first_above(const uint32_t* ends, int n, uint32_t
 // page) pages off the free list, after those of the requests before it; row j of its fresh ones has position past + j and
 // the slot of that position. Every workgroup scans the R lengths itself (two scans in LDS, at most 16 requests a thread)
 // and then finds its rows' requests by bisection, so one launch does it: what bounds it is the latency of the lengths'
-// load, the scans and the table's load one after the other.
+// load, the scans and the table's load one after the other (64 requests of one token 3.3 us, 700 requests with 25,600 rows
+// 6.0 us).
 __global__ __launch_bounds__(256) void k_paged_plan(const uint32_t* past, const uint32_t* fresh, const uint32_t* free,
                                                     uint32_t* table, uint32_t* starts, uint32_t* context,
                                                     uint32_t* positions, uint32_t* slots, uint32_t* counts, uint32_t R,
@@ -208,7 +209,9 @@ __device__ __forceinline__ float sum_lanes(float v) {
 }
 
 // ---------------------------------------------------------------- 48 qk_norm_rope_append_paged
-// Bound by the projections' bytes. Queries and keys: a head is 4 to 16 lanes with 16 bytes of its lower and of its upper
+// n = w x / sqrt(mean x^2 + eps) over a head, (a, b) its halves: (a cos - b sin, b cos + a sin) at the row's position; values
+// as they are. Everything is float32 until the one rounding to the cache's type (nearest even) at the stores.
+// Bound by the projections' bytes (9,200 rows of 32 + 8 + 8 heads of 128 in bf16: 47 us, 5.2 TB/s; 512 rows 5.2 us). Queries and keys: a head is 4 to 16 lanes with 16 bytes of its lower and of its upper
 // half each, so a lane holds the pairs that the rotation turns, the sum of squares is a few DPP adds, and a wave takes 4 to
 // 16 heads of a row at a time; the row's rotation and the norm weights are loaded once per wave. Values: a wave takes the
 // runs of rows that begin in its 8 rows, a run being rows whose slots follow each other in one tile of 8 positions; a
@@ -424,8 +427,13 @@ __device__ __forceinline__ float add_odd(float o, float count) {
 }
 
 // Rows of few query columns: up to 16 per request and KV head (column c = row c / group, head c % group of the KV head's).
+// y = sum_k 2^((s_k - m) c) v_k / sum_k 2^((s_k - m) c) over the keys that a column sees, c the scale times log2 e, in one pass
+// with a running reference m.
 // Bound by the cache's bytes, so every wave streams its own keys straight into the registers that the matrix
-// instruction reads (no LDS, no barrier), two units in flight, and the four waves of a workgroup meet once per item.
+// instruction reads (no LDS, no barrier), two units in flight, and the four waves of a workgroup meet once per item. All
+// units are shared out evenly over 512 workgroups, so a long context spreads over the GPU and a batch of uneven ones leaves no
+// CU behind; the last part of an item to arrive joins its partials. Measured: 200 requests of up to 4000 positions 262 us, 16
+// of 8192 88 us (both 6.1 TB/s), one of 65,701 47 us (5.7 TB/s), one of 700 8.6 us alone.
 //
 // A unit is 128 keys of an item, 32 per wave. S^T = K Q^T on 16 x 16 x 32 tiles: the two tiles' rows i hold the keys
 // 8 (i / 4) + 4 tile + i % 4, so that lane group g = lane / 16 gets the scores of the eight keys 8 g .. 8 g + 7 of its column:
@@ -791,12 +799,18 @@ __device__ __forceinline__ uint32_t floor_sum64(uint32_t n, uint32_t step, uint3
 
 // Rows of many query columns, on 32 x 32 x 16 tiles. A tile of an item is up to 256 columns (whole rows of the request: 256 /
 // group of them), 32 per wave, eight waves: two per SIMD, so that one's VALU work runs beside the other's matrix
-// instructions. K and V blocks of 64 keys go from the pages
-// through registers into LDS (three K blocks, two V blocks), loaded a step before they are stored; one barrier per block.
-// V's layout in the cache is already the order in which it is read.
+// instructions (four waves of 64 columns would read half as much from LDS, but past 256 registers every product's result
+// has to come out of the accumulation file first: 1317 us where this form takes 992). K and V blocks of 64 keys go from the
+// pages through registers into LDS (three K blocks, two V blocks), loaded two steps before they are stored; one barrier per
+// block. (Loads straight into LDS made the compiler wait for all of them before every LDS read.) V's layout in the cache is
+// already the order in which it is read.
 // Step n: the scores of block n + 1 (matrix core) under the exponentials of block n (VALU), then block n's products
 // under the maxima of block n + 1. The rows of S^T's tiles hold the keys in the order in which P^T wants them (bits 2 and 3
-// of the row exchanged), so weights never cross lanes.
+// of the row exchanged), so weights never cross lanes. They are rounded to the cache's type for the product, as its values
+// are, at most 2^8 above the reference maximum; scores, sums and products are float32.
+// Measured: 4096 rows on 28,672 positions (16 / 8 heads of 128, fp16) 938 us, 1100 TFLOP/s: the card's power limit, at which
+// a library product of 8192^3 reaches 1159; matrix cores busy 55 % of the cycles. A prompt of 2048 30 us (570 TFLOP/s): 4 us
+// to start, 11 blocks of 1.9 us, 2 to store, 8 for the join.
 template <typename T, int HD>
 __global__ __launch_bounds__(512, 1) void k_attn_tiles(AttnArgs a, uint32_t bytes) {
     using M = Mfma<T>;
@@ -1419,15 +1433,16 @@ static void l_plan(const PreparedDispatch& pd, void* const* p, hipStream_t s) {
 // qkv, q_norm, k_norm, cos_table, sin_table, starts, positions, slots, q, k_cache, v_cache, requests, tokens, q_heads,
 // kv_heads, head_dim, max_pos, page, pages, eps
 // The grid of 48: waves of queries and keys, then waves of values. A wave takes 1024 elements of a row's query and key heads,
-// or, from 2048 rows on, which fill the GPU so, all of them (the row's rotation is then loaded once); 8 rows x 128
-// elements of the value heads.
+// or, from 4096 rows on, all of them, so that the row's rotation is loaded once (2048 rows: 8.8 us in parts, 9.9 whole; 4096:
+// 15.8 and 16.0; 9,200 rows of 40 heads in bf16 49.4 and 47.0, of 24 in float32 46.1 and 48.4); 8 rows x 128 elements of the
+// value heads.
 struct AppendGrid {
     uint32_t parts, qk_blocks, v_chunks, v_blocks;
 };
 static AppendGrid append_grid(const uint32_t* w) {
     const uint64_t T = w[13];
     AppendGrid g;
-    g.parts = T >= 2048 ? 1 : uint32_t(((uint64_t(w[14]) + w[15]) * w[16] + 1023) / 1024);
+    g.parts = T >= 4096 ? 1 : uint32_t(((uint64_t(w[14]) + w[15]) * w[16] + 1023) / 1024);
     g.qk_blocks = uint32_t((T * g.parts + 3) / 4);
     g.v_chunks = uint32_t((uint64_t(w[15]) * w[16] + 127) / 128);
     g.v_blocks = uint32_t(((T + 7) / 8 * g.v_chunks + 3) / 4);
@@ -1468,6 +1483,8 @@ static void l_append(const PreparedDispatch& pd, void* const* p, hipStream_t s) 
 // blocks, page, pages, scale
 // the most new rows of a request in the dispatch, and whether every item's columns fit the kernel for few
 static uint32_t most_fresh(const uint32_t* w) { return w[11] ? std::min(w[11], w[10]) : w[10]; }
+// (the kernel for few against the tiles at 16 columns: 16 requests of 4 rows on 2000 positions 23 us and 32, 64 of one row 86
+// and 101; past 16 a second tile of columns would double its registers)
 static bool few_columns(const uint32_t* w) {
     return w[13] && uint64_t(most_fresh(w)) * (w[12] / w[13]) <= paged::kRowsCols;
 }
@@ -1614,7 +1631,8 @@ std::vector<KernelSpec> paged_catalog() {
                      same_dtype("qk_norm_rope_append_paged", t, {8, 9, 10});
                      if (t[0].row.dtype() != F32) same_dtype("qk_norm_rope_append_paged", t, {0, 8});
                  }});
-    // 49 attention_paged
+    // 49 attention_paged (the catalog's thread count is that of the kernel for few columns; the tiles' has 512, and a second
+    // launch joins their split items)
     c.push_back({"attention_paged", "paged", {256, 1, 1}, false,
                  [](const uint32_t* w) {
                      return Grid3{int64_t(few_columns(w) ? paged::kRowsGroups : paged::kTileGroups), 1, 1};

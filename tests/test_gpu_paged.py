@@ -314,6 +314,13 @@ def test_attention_request_limits(requests):
     _attn_case(F16, 1, 1, 64, 16, [(i % 5, i % 2) for i in range(1, requests + 1)], pad=1)
 
 
+@pytest.mark.parametrize("qh,kvh,hd", [(256, 1, 64), (100, 1, 128), (34, 2, 64), (17, 1, 128)])
+def test_attention_large_groups(qh, kvh, hd):
+    """Query heads per KV head that fill a tile with one row, leave columns over, and just miss the form for few."""
+    _attn_case(F16, qh, kvh, hd, 16, [(50, 1), (0, 5), (130, 3)], pad=1)
+    _attn_case(BF16, qh, kvh, hd, 32, [(70, 1), (0, 1)], max_fresh=1)
+
+
 @pytest.mark.parametrize("short", [9, 24])
 def test_attention_uneven_requests(short):
     """Few items of very different lengths: with workgroups of their own each, and with too few left for the long ones."""
@@ -485,6 +492,133 @@ def test_attention_replayed_with_other_lengths():
     finally:
         cl.release()
         s.close()
+
+
+def _batch(seed, lens, qh, kvh, hd, page, outputs, workspaces, tokens):
+    """A session with one ragged batch in it and as many results and workspaces, and the dispatch's fields for each form."""
+    r = np.random.default_rng(seed)
+    past, fresh = (np.array(x) for x in zip(*lens))
+    R, blocks = len(lens), int((past + fresh).max()) // page + 1
+    pages = R * blocks
+    kb, vb = O.to_bits(F16, r.standard_normal((pages, kvh, page, hd))), O.to_bits(F16, r.standard_normal((pages, kvh, page // 8, hd, 8)))
+    u = lambda a: (U32, np.shape(a), 0, np.asarray(a, np.uint32))  # noqa: E731
+    words = attention_paged_workspace_words(R, tokens, qh, kvh, hd)
+    q = O.to_bits(F16, r.standard_normal((tokens, qh * hd)))
+    s = Session({"q": (F16, q.shape, 0, q), "k_cache": (F16, kb.shape, RO, kb), "v_cache": (F16, _rank4(vb), RO, vb),
+                 "table": u(r.permutation(pages).reshape(R, blocks)), "starts": u(np.concatenate([[0], np.cumsum(fresh)])),
+                 "context": u(past + fresh), **{f"y{i}": (F16, q.shape, 0, None) for i in range(outputs)},
+                 **{f"ws{i}": u(np.zeros(words)) for i in range(workspaces)}})
+    common = ("q", "k_cache", "v_cache", "table", "starts", "context")
+
+    def fields(y, ws, max_fresh):
+        return s.fields("attention_paged", **{n: n for n in common}, y=y, workspace=ws, requests=R, tokens=tokens,
+                        max_fresh=max_fresh, q_heads=qh, kv_heads=kvh, head_dim=hd, blocks=blocks, page=page, pages=pages,
+                        scale=hd ** -0.5)
+    return s, fields
+
+
+def _eager(s, fields, *args):
+    cl = s.backend.begin()
+    cl.dispatch("attention_paged", fields(*args))
+    s.backend.wait(s.backend.submit(cl))
+    cl.release()
+    return s.read(args[0])
+
+
+@pytest.mark.parametrize("count", [2, 10])
+def test_attention_forms_take_turns_in_one_workspace(count):
+    """A reusable list of few dispatches (launched one by one) and of many (a captured graph) in which the form for single
+    tokens and the tiles use one workspace in turn, replayed with eager work and other lists between: every replay gives the
+    eager dispatch's bits."""
+    lens = [(700, 1), (0, 1), (1500, 1), (63, 1), (64, 1), (2000, 1)]
+    s, fields = _batch(3, lens, 4, 2, 128, 16, count, 1, 40)
+    cl, other = s.backend.begin(reusable=True), s.backend.begin(reusable=True)
+    try:
+        want = [_eager(s, fields, "y0", "ws0", f) for f in (1, 0)]
+        for i in range(count):
+            cl.dispatch("attention_paged", fields(f"y{i}", "ws0", 1 - i % 2))
+        other.dispatch("attention_paged", fields("y0", "ws0", 0))
+        for replay in range(4):
+            for i in range(count):
+                s.write(f"y{i}", s.poison(f"y{i}"))
+            s.backend.wait(s.backend.submit(cl, repeat=1 + replay % 2))
+            for i in range(count):
+                assert s.read(f"y{i}").tobytes() == want[i % 2].tobytes(), (replay, i)
+            s.backend.wait(s.backend.submit(other))
+            assert s.read("y0").tobytes() == want[1].tobytes()
+    finally:
+        cl.release()
+        other.release()
+        s.close()
+
+
+@pytest.mark.parametrize("first,second", [(1, 1), (1, 0), (0, 0)])
+def test_attention_overlapped(first, second):
+    """Two dispatches that may run at once, each with a workspace of its own."""
+    s, fields = _batch(4, [(1200, 1), (300, 1), (5, 1)], 8, 4, 64, 32, 2, 2, 20)
+    try:
+        want = [_eager(s, fields, "y0", "ws0", f) for f in (first, second)]
+        for _ in range(3):
+            for n in ("y0", "y1"):
+                s.write(n, s.poison(n))
+            cl = s.backend.begin()
+            cl.dispatch_overlapped("attention_paged", fields("y0", "ws0", first))
+            cl.dispatch("attention_paged", fields("y1", "ws1", second))
+            cl.barrier()
+            s.backend.wait(s.backend.submit(cl))
+            cl.release()
+            assert [s.read(n).tobytes() for n in ("y0", "y1")] == [w.tobytes() for w in want]
+    finally:
+        s.close()
+
+
+def test_attention_pages_missing_far_back():
+    """Pages that are none in the middle of long contexts, in some groups of sixteen blocks and not in others."""
+    def spoil(table, pages):
+        r = np.random.default_rng(2)
+        for i in range(len(table)):
+            table[i, r.integers(0, 3000 // 16, 4)] = [PAGED_NONE, pages, pages + 7, PAGED_NONE]
+
+    for lens in ([(3000, 40), (2900, 100)], [(3000, 1)] * 3 + [(2990, 2)]):
+        _attn_case(F16, 4, 2, 128, 16, lens, spoil=spoil)
+        _attn_case(BF16, 2, 2, 64, 16, lens, spoil=spoil)
+
+
+def test_append_two_rows_of_one_slot():
+    """Two rows that name one slot: each part of the entry is one row's or the other's, and nothing else changes."""
+    r = np.random.default_rng(6)
+    qh, kvh, hd, page, pages, T = 2, 2, 64, 16, 3, 4
+    qkv = r.standard_normal((T, (qh + 2 * kvh) * hd)).astype(np.float32)
+    ones, cos = O.to_bits(BF16, np.ones(hd)), np.ones((9, hd // 2), np.float32)
+    kc, vc = (np.full(n, POISON_16, np.uint16) for n in ((pages, kvh, page, hd), (pages, kvh, page // 8, hd, 8)))
+    u = lambda a: (U32, np.shape(a), 0, np.asarray(a, np.uint32))  # noqa: E731
+    s = Session({"qkv": (F32, qkv.shape, RO, qkv), "q_norm": (BF16, (hd,), RO, ones), "k_norm": (BF16, (hd,), RO, ones),
+                 "cos_table": (F32, cos.shape, RO, cos), "sin_table": (F32, cos.shape, RO, cos * 0), "starts": u([0, T]),
+                 "positions": u([1, 2, 3, 4]), "slots": u([5, 21, 5, 21]), "q": (F16, (T, qh * hd), 0, None),
+                 "k_cache": (F16, kc.shape, 0, kc), "v_cache": (F16, _rank4(vc), 0, vc)})
+    try:
+        cl = s.backend.begin()
+        cl.dispatch("qk_norm_rope_append_paged", s.fields(
+            "qk_norm_rope_append_paged", **{n: n for n in s.spec}, requests=1, tokens=T, q_heads=qh, kv_heads=kvh, head_dim=hd,
+            max_pos=9, page=page, pages=pages, eps=0.0))
+        s.backend.wait(s.backend.submit(cl))
+        cl.release()
+        gk, gv = s.read("k_cache"), s.read("v_cache").reshape(vc.shape)
+    finally:
+        s.close()
+    x = qkv.reshape(T, qh + 2 * kvh, hd)
+    v = O.to_bits(F16, x[:, qh + kvh:])
+    k = x[:, qh:qh + kvh].astype(np.float64)
+    k = k / np.sqrt((k * k).mean(-1, keepdims=True))
+    touched_k, touched_v = np.zeros(kc.shape, bool), np.zeros(vc.shape, bool)
+    for slot, rows in ((5, (0, 2)), (21, (1, 3))):
+        at, off = divmod(slot, page)
+        touched_k[at, :, off], touched_v[at, :, off // 8, :, off % 8] = True, True
+        g = O.from_bits(F16, gk[at, :, off])
+        # float32's sum of squares, root and products, then half a step of fp16
+        assert np.all(np.min([np.abs(g - k[t]) - (2.0 ** -11 + 16 * O.U24) * np.abs(k[t]) for t in rows], axis=0) <= 2.0 ** -25)
+        assert np.all((gv[at, :, off // 8, :, off % 8] == v[rows[0]]) | (gv[at, :, off // 8, :, off % 8] == v[rows[1]]))
+    assert np.all(gk[~touched_k] == POISON_16) and np.all(gv[~touched_v] == POISON_16)
 
 
 # ---------------------------------------------------------------- together
