@@ -1357,16 +1357,7 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {
         __builtin_amdgcn_make_buffer_rsrc(a.ws, 0, int(4 * (paged::kTileSlots + 2 * paged::kTileGroups * SW)), 0x00020000);
     auto slot_at = [&](int i) { return int(paged::kTileSlots) + (base + i * stride + (i ? 0 : first)) * SW; };
     constexpr int PF = 6;
-    float top = -INFINITY;
-    for (int i = 0; i < parts; i += PF) {
-        float2 ml[PF];
-#pragma unroll
-        for (int q = 0; q < PF; ++q) ml[q] = load_part2<0>(ws, slot_at(min(i + q, parts - 1)) + 2 * col);
-#pragma unroll
-        for (int q = 0; q < PF; ++q) top = fmaxf(top, ml[q].x);
-    }
-    const float tc = top == -INFINITY ? 0.f : top * a.scale_log2;
-    float l = 0.f, sum[4 * N];
+    float top = -INFINITY, l = 0.f, sum[4 * N];
 #pragma unroll
     for (int e = 0; e < 4 * N; ++e) sum[e] = 0.f;
     for (int i = 0; i < parts; i += PF) {
@@ -1382,6 +1373,18 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {
                 x[q][j] = load_part<0>(ws, slot + 2 * int(paged::kTileCols) + ((wv * 4 * DT + part_d * N + j) * 64 + lane) * 4);
         }
         __builtin_amdgcn_sched_barrier(0);  // (all under way before the first is waited for)
+        float most = top;
+#pragma unroll
+        for (int q = 0; q < PF; ++q) {
+            if (i + q >= parts) break;
+            most = fmaxf(most, ml[q].x);
+        }
+        const float tc = most == -INFINITY ? 0.f : most * a.scale_log2;
+        const float back = __builtin_amdgcn_exp2f(top * a.scale_log2 - tc);
+        top = most;
+        l *= back;
+#pragma unroll
+        for (int e = 0; e < 4 * N; ++e) sum[e] *= back;
 #pragma unroll
         for (int q = 0; q < PF; ++q) {
             if (i + q >= parts) break;
