@@ -258,7 +258,7 @@ class Device {
         uint64_t fence;
         hipEvent_t event;
     };
-    static constexpr int64_t kMarkNs = 20000;
+    static constexpr int64_t kMarkNs = 50000;
     void mark(uint64_t fence);
     void reach(uint64_t fence);  // waits until every submission up to `fence` has completed
     std::deque<Mark> marks_;

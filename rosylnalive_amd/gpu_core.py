@@ -391,6 +391,12 @@ class HipBackend:
         self.info = _info(s)
         self.heap: Optional[HipHeap] = None
         self.shader_set_hash: Optional[bytes] = None
+        self._results()
+
+    def _results(self):
+        """Where submit and wait find their results: a call of each per step, from one thread at a time."""
+        self._fence, self._dispatches, self._timers = C.c_uint64(), C.c_int(), C.c_int()
+        self._refs = C.byref(self._fence), C.byref(self._dispatches), C.byref(self._timers)
 
     @classmethod
     def _wrap(cls, handle) -> "HipBackend":
@@ -402,6 +408,7 @@ class HipBackend:
         b.heap = None
         b.shader_set_hash = None
         b._borrowed = True
+        b._results()
         return b
 
     @property
@@ -440,20 +447,23 @@ class HipBackend:
         return HipCommandList(self, l, reusable)
 
     def submit(self, commands: "HipCommandList", repeat: int = 1) -> Submission:
-        f = C.c_uint64()
-        check(lib().lrm_hip_submit(self._h, commands._h, repeat, C.byref(f)))
-        return Submission(f.value)
+        rc = lib().lrm_hip_submit(self._h, commands._h, repeat, self._refs[0])
+        if rc:
+            check(rc)
+        return Submission(self._fence.value)
 
     def wait(self, submission: int) -> Completion:
-        nd, nt = C.c_int(), C.c_int()
-        check(lib().lrm_hip_wait(self._h, int(submission), C.byref(nd), C.byref(nt)))
-        timers = []
-        for i in range(nt.value):
+        _, nd, nt = self._refs
+        rc = lib().lrm_hip_wait(self._h, int(submission), nd, nt)
+        if rc:
+            check(rc)
+        timers, dispatches = [], self._dispatches.value
+        for i in range(self._timers.value):
             name = C.create_string_buffer(128)
             st, du = C.c_int64(), C.c_int64()
             check(lib().lrm_hip_timer(self._h, int(submission), i, name, 128, C.byref(st), C.byref(du)))
             timers.append(TimerResult(name.value.decode(), st.value, du.value))
-        return Completion(int(submission), nd.value, timers)
+        return Completion(int(submission), dispatches, timers)
 
     def close(self):
         if getattr(self, "_h", None) and not getattr(self, "_borrowed", False):
