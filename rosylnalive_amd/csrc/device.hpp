@@ -171,8 +171,8 @@ class Device {
     // IKernelSet. Two kernel sets, each its own ExecutionClass (its own shader-set hash), since they make different
     // bit-identity claims:
     //   Reference: the reference's catalog, ids 0 .. fast_first_id() - 1, and the fused fp32 kernels, ids kFusedFirstId ..
-    //     kPagedFirstId - 1, which keeps the BatchInvariance contract (a row alone equals the row in any batch; prefill equals decode and
-    //     any chunked prefill);
+    //     kPagedFirstId - 1, which keeps the BatchInvariance contract (a row alone equals the row in any batch; prefill equals
+    //     decode and any chunked prefill);
     //   Fast: every id (the reference's catalog and the fast path), which only claims that the same work on the same
     //     inputs gives the same bits: its k-split and attention-split choices depend on the row count, and its
     //     prefill and decode kernels sum in different orders.
@@ -221,7 +221,7 @@ class Device {
     void join_side();                             // the main stream waits for the side stream
     static bool graphs_enabled();
     // A graph's launch takes 17 us of host time on MI355X whatever it holds, a kernel's 2.6: lists of up to this many
-    // launches and nothing else are launched one by one.
+    // dispatches (most are one launch) and nothing else are launched one by one.
     static constexpr size_t kDirectLaunches = 6;
     void run_probe();
     DeviceInfo info_{};

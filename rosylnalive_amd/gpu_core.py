@@ -20,7 +20,8 @@ from ._native import Fp16RangeError, GpuContractException, HipDeviceError, LrmEr
 __all__ = [
     "Fp16RangeError", "GpuContractException", "HipDeviceError", "LrmError", "Heap", "DType", "Arena", "TensorFlags", "Catalog",
     "KernelSpec", "ArgBlock", "HeapLayout", "HeapPlanner", "TensorTable", "SealedTable", "HipBackendProvider",
-    "HipBackend", "HipHeap", "HeapView", "HipCommandList", "Submission", "Completion", "TimerResult", "prepare", "grid_physical",
+    "HipBackend", "HipHeap", "HeapView", "HipCommandList", "Submission", "Completion", "TimerResult", "prepare",
+    "grid_physical", "PAGED_NONE", "attention_paged_workspace_words",
 ]
 
 
@@ -519,9 +520,9 @@ class HeapView:
     """A heap tensor to other libraries that use this GPU in the process, without a copy (`__cuda_array_interface__`: torch,
     cupy). bf16 and u32, which the interface lacks or few libraries take, come as the int16 and int32 that hold their
     bits. Both sides have to use one HIP runtime: a program that uses torch imports it before this package loads its library,
-    which then finds torch's. It keeps the backend object alive, not its memory: nothing may use it after HipBackend.close. Nothing orders
-    the other library's work with the backend's stream: wait for a submission before reading what it wrote, and
-    synchronise the other library before submitting what reads its writes."""
+    which then finds torch's. It keeps the backend object alive, not its memory: nothing may use it after HipBackend.close.
+    Nothing orders the other library's work with the backend's stream: wait for a submission before reading what it wrote,
+    and synchronise the other library before submitting what reads its writes."""
 
     TYPESTR = {DType.F32: "<f4", DType.BF16: "<i2", DType.F16: "<f2", DType.I32: "<i4", DType.U32: "<i4", DType.U8: "|u1",
                DType.F64: "<f8", DType.I64: "<i8"}
