@@ -797,8 +797,8 @@ __device__ __forceinline__ uint32_t floor_sum64(uint32_t n, uint32_t step, uint3
     return sum;
 }
 
-// Rows of many query columns, on 32 x 32 x 16 tiles. A tile of an item is up to 256 columns (whole rows of the request: 256 /
-// group of them), 32 per wave, eight waves: two per SIMD, so that one's VALU work runs beside the other's matrix
+// Rows of many query columns, on 32 x 32 x 16 tiles. A tile of an item is up to 32 columns per wave (whole rows of the request),
+// eight waves or two workgroups of four per CU: two waves per SIMD, so that one's VALU work runs beside the other's matrix
 // instructions (four waves of 64 columns would read half as much from LDS, but past 256 registers every product's result
 // has to come out of the accumulation file first: 1317 us where this form takes 992). K and V blocks of 64 keys go from the
 // pages through registers into LDS (three K blocks, two V blocks), loaded two steps before they are stored; one barrier per
@@ -811,21 +811,23 @@ __device__ __forceinline__ uint32_t floor_sum64(uint32_t n, uint32_t step, uint3
 // Measured: 4096 rows on 28,672 positions (16 / 8 heads of 128, fp16) 938 us, 1100 TFLOP/s: the card's power limit, at which
 // a library product of 8192^3 reaches 1159; matrix cores busy 55 % of the cycles. A prompt of 2048 30 us (570 TFLOP/s): 4 us
 // to start, 11 blocks of 1.9 us, 2 to store, 8 for the join.
-template <typename T, int HD>
-__global__ __launch_bounds__(512, 1) void k_attn_tiles(AttnArgs a, uint32_t bytes) {
+template <typename T, int HD, int NW>
+__global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void k_attn_tiles(AttnArgs a, uint32_t bytes) {
     using M = Mfma<T>;
     constexpr int KB = int(paged::kTileKeys), KS = HD / 16, DT = HD / 32, RB = HD * 2, BLK = KB * RB;
     constexpr int KR = RB + 16, KBLK = KB * KR;  // a K row in LDS is padded by 16 bytes: 16 rows lie in different banks
     constexpr int CH = RB / 16;            // 16-byte chunks of a K row
-    constexpr int LPB = BLK / 8192;        // loads of a block per wave and of 1 KB each: 8 keys
+    constexpr int WK = KB / NW;            // keys of a block that a wave moves
+    constexpr int LPB = WK * RB / 1024;    // its loads, of 1 KB each
+    constexpr uint32_t GROUPS = paged::tile_groups(NW), COLS = paged::tile_cols(NW), SLOTS = paged::tile_slots(NW);
     __shared__ __attribute__((aligned(16))) uint8_t lds[3 * KBLK + 2 * BLK];  // K blocks n % 3, then V blocks n % 2
     __shared__ uint32_t ends[paged::kMaxRequests];
     __shared__ uint32_t red[8];
-    __shared__ uint32_t units_of_tile[paged::kTileGroups];
+    __shared__ uint32_t units_of_tile[64 * NW];
     __shared__ int chosen[3];
     __shared__ uint32_t odd;  // the first unit of the last piece that held values to take out
     const int t = threadIdx.x, lane = t & 63, wv = uniform(t >> 6), c32 = lane & 31, h = lane >> 5;
-    const int group = int(a.qh / a.kvh), kvh = int(a.kvh), TR = int(paged::kTileCols) / group;
+    const int group = int(a.qh / a.kvh), kvh = int(a.kvh), TR = int(COLS) / group;
 
     constexpr int kStart = int(paged::kTileStart);
     // ---- the units of every request, and this workgroup's
@@ -846,7 +848,7 @@ __global__ __launch_bounds__(512, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
     auto tiles_of = [&](const Request& q) { return (q.rows + TR - 1) / TR; };
     // ends[r] = the sum of f over the requests up to and with r
     auto scan_requests = [&](auto&& f) {
-        const uint32_t per = (a.requests + 511) / 512, r0 = min(t * per, a.requests), r1 = min(r0 + per, a.requests);
+        const uint32_t per = (a.requests + 64 * NW - 1) / (64 * NW), r0 = min(t * per, a.requests), r1 = min(r0 + per, a.requests);
         uint32_t sum = 0;
         for (uint32_t r = r0; r < r1; ++r) {
             const Request q = request_of(a, r);
@@ -881,7 +883,7 @@ __global__ __launch_bounds__(512, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
         describe_none();
         return;
     }
-    bool apart = uint64_t(tiles_all) * kvh <= paged::kTileGroups;
+    bool apart = uint64_t(tiles_all) * kvh <= GROUPS && tiles_all <= 256;
     uint32_t q = 0;
     if (apart) {
         // No more items than workgroups: each gets ceil(units / q) of its own, q the least that fits, so no workgroup starts
@@ -904,7 +906,7 @@ __global__ __launch_bounds__(512, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
             sum += float(n[j]);
             most = fmaxf(most, float(n[j]));
         }
-        const uint32_t room = paged::kTileGroups / uint32_t(kvh);
+        const uint32_t room = GROUPS / uint32_t(kvh);
         uint32_t hi = uint32_t(uniform(int(wave_max(most)))), lo = uint32_t(uniform(int(wave_sum(sum)))) / room;
         const uint32_t even = lo;
         lo = min(max(max(lo, 1u), uint32_t(sqrtf(0.5f * float(hi)))), hi);
@@ -949,7 +951,7 @@ __global__ __launch_bounds__(512, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
         scan_requests([&](const Request& q) { return first_weight(q, tiles_of(q)) * uint32_t(kvh); });
         total = ends[a.requests - 1], G = min(uint32_t(gridDim.x), total);
         // workgroups of one XCD (every eighth) take neighbouring units, which share a KV head's blocks in its L2
-        if (G == paged::kTileGroups) w = (blockIdx.x % 8) * (paged::kTileGroups / 8) + blockIdx.x / 8;
+        if (G == GROUPS) w = (blockIdx.x % 8) * (GROUPS / 8) + blockIdx.x / 8;
         if (w >= G) {
             describe_none();
             return;
@@ -981,15 +983,15 @@ __global__ __launch_bounds__(512, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
 #pragma unroll
     for (int i = 0; i < LPB; ++i) {
         const int p = 64 * i + lane, row = p / CH, ch = p % CH;  // row of the wave's 8, place in the row
-        kst[i] = (8 * wv + row) * KR + ch * 16;
+        kst[i] = (WK * wv + row) * KR + ch * 16;
     }
     // operand reads: K row of matrix row c32 is key 16 (c32 / 16) + 8 (c32 / 4 % 2) + 4 (c32 / 8 % 2) + c32 % 4
     const int krow = (c32 & 19) | ((c32 & 4) << 1) | ((c32 & 8) >> 1);
     const int kbase = krow * KR + 16 * h, vbase = 3 * KBLK + h * (8 * RB) + c32 * 16;
 
-    constexpr int SW = int(paged::slot_words(paged::kTileCols, HD));
+    constexpr int SW = int(paged::slot_words(COLS, HD));
     const __amdgpu_buffer_rsrc_t ws =
-        __builtin_amdgcn_make_buffer_rsrc(a.ws, 0, int(4 * (paged::kTileSlots + 2 * paged::kTileGroups * SW)), 0x00020000);
+        __builtin_amdgcn_make_buffer_rsrc(a.ws, 0, int(4 * (SLOTS + 2 * GROUPS * SW)), 0x00020000);
     bool described = false;
 
     for (;;) {
@@ -1030,8 +1032,8 @@ __global__ __launch_bounds__(512, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
                 no_page = __ballot(ids >= a.pages);
             }
             bad = uint32_t(no_page >> (4 * (j & 15))) & 15u;
-            const uint32_t id = uint32_t(__builtin_amdgcn_readlane(int(ids), 4 * (j & 15) + (wv >> 1)));
-            const uint32_t off = uint32_t((j0 + j) * KB + 8 * wv) & ((1u << a.page_log2) - 1);
+            const uint32_t id = uint32_t(__builtin_amdgcn_readlane(int(ids), 4 * (j & 15) + (WK * wv >> 4)));
+            const uint32_t off = uint32_t((j0 + j) * KB + WK * wv) & ((1u << a.page_log2) - 1);
             soff = id < a.pages ? int((((id * uint32_t(kvh) + hk) << a.page_log2) + off) * RB) : 0;
         };
         // the chunks of this wave on their way to LDS: two blocks of each cache
@@ -1055,7 +1057,7 @@ __global__ __launch_bounds__(512, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
             if (left < KB || bad) {  // uniform: what is hidden may be anything, and zero times NaN is NaN
 #pragma unroll
                 for (int i = 0; i < LPB; ++i) {
-                    const int in = (bad >> (wv >> 1) & 1u) ? 0 : left - 8 * wv;
+                    const int in = (bad >> (WK * wv >> 4) & 1u) ? 0 : left - WK * wv - i * 1024 / (8 * RB) * 8;
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
                         rv[decltype(set)::value][i][e] &= (2 * e < in ? 0x0000FFFFu : 0u) | (2 * e + 1 < in ? 0xFFFF0000u : 0u);
@@ -1310,13 +1312,13 @@ __global__ __launch_bounds__(512, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
                 described = true;
             }
             if (cw < cols) {  // 16 bytes i of lane l: (4 DT wave + i) 64 + l, after the maxima and sums
-                const int slot = int(paged::kTileSlots) + (base + mine * stride + (mine ? 0 : first)) * SW;
+                const int slot = int(SLOTS) + (base + mine * stride + (mine ? 0 : first)) * SW;
                 if (h == 0) store_part2(ws, slot + 2 * mycol, m_run, l_run);
 #pragma unroll
                 for (int i = 0; i < 4 * DT; ++i) {
                     const f32x16& x = o[i >> 2];
                     const int e = 4 * (i & 3);
-                    store_part(ws, slot + 2 * int(paged::kTileCols) + ((wv * 4 * DT + i) * 64 + lane) * 4,
+                    store_part(ws, slot + 2 * int(COLS) + ((wv * 4 * DT + i) * 64 + lane) * 4,
                                f32x4{x[e], x[e + 1], x[e + 2], x[e + 3]});
                 }
             }
@@ -1343,19 +1345,20 @@ __global__ __launch_bounds__(512, 1) void k_attn_tiles(AttnArgs a, uint32_t byte
 // order. A launch of its own, for all CUs: the last workgroup of an item to end, if it joined them, would read 128 KiB a
 // part alone (1.5 us each, 12 us for the eight parts of a 512-row chunk at 8K). Block (item, wave of the tile): its four
 // waves take a quarter of each column's dims each.
-template <typename T, int HD>
+template <typename T, int HD, int NW>
 __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {
+    constexpr uint32_t GROUPS = paged::tile_groups(NW), COLS = paged::tile_cols(NW), SLOTS = paged::tile_slots(NW);
     constexpr int DT = HD / 32, N = DT;  // 16 bytes per lane and part
-    constexpr int SW = int(paged::slot_words(paged::kTileCols, HD));
-    const int lead = blockIdx.x >> 3, wv = blockIdx.x & 7, t = threadIdx.x, lane = t & 63, part_d = t >> 6, c32 = lane & 31;
+    constexpr int SW = int(paged::slot_words(COLS, HD));
+    const int lead = blockIdx.x / NW, wv = blockIdx.x % NW, t = threadIdx.x, lane = t & 63, part_d = t >> 6, c32 = lane & 31;
     const u32x4* d = reinterpret_cast<const u32x4*>(a.ws + paged::kGroups) + 2 * lead;
     const u32x4 d0 = d[0], d1 = d[1];
     const int parts = uniform(int(d0[0])), base = uniform(int(d0[1])), stride = uniform(int(d0[2])), first = uniform(int(d0[3]));
     const int row0 = int(d1[0]), cols = int(d1[1]), hk = int(d1[2]), col = 32 * wv + c32;
     if (parts == 0 || 32 * wv >= cols) return;
     const __amdgpu_buffer_rsrc_t ws =
-        __builtin_amdgcn_make_buffer_rsrc(a.ws, 0, int(4 * (paged::kTileSlots + 2 * paged::kTileGroups * SW)), 0x00020000);
-    auto slot_at = [&](int i) { return int(paged::kTileSlots) + (base + i * stride + (i ? 0 : first)) * SW; };
+        __builtin_amdgcn_make_buffer_rsrc(a.ws, 0, int(4 * (SLOTS + 2 * GROUPS * SW)), 0x00020000);
+    auto slot_at = [&](int i) { return int(SLOTS) + (base + i * stride + (i ? 0 : first)) * SW; };
     constexpr int PF = 6;
     float top = -INFINITY, l = 0.f, sum[4 * N];
 #pragma unroll
@@ -1370,7 +1373,7 @@ __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {
             ml[q] = load_part2<0>(ws, slot + 2 * col);
 #pragma unroll
             for (int j = 0; j < N; ++j)
-                x[q][j] = load_part<0>(ws, slot + 2 * int(paged::kTileCols) + ((wv * 4 * DT + part_d * N + j) * 64 + lane) * 4);
+                x[q][j] = load_part<0>(ws, slot + 2 * int(COLS) + ((wv * 4 * DT + part_d * N + j) * 64 + lane) * 4);
         }
         __builtin_amdgcn_sched_barrier(0);  // (all under way before the first is waited for)
         float most = top;
@@ -1491,6 +1494,13 @@ static uint32_t most_fresh(const uint32_t* w) { return w[11] ? std::min(w[11], w
 static bool few_columns(const uint32_t* w) {
     return w[13] && uint64_t(most_fresh(w)) * (w[12] / w[13]) <= paged::kRowsCols;
 }
+static uint32_t tile_waves_of(const uint32_t* w) { return paged::tile_waves(w[14], w[13] ? w[12] / w[13] : 0); }
+template <typename T, int HD, int NW>
+static void launch_tiles(const AttnArgs& a, uint32_t bytes, hipStream_t s) {
+    constexpr uint32_t groups = paged::tile_groups(NW);
+    hipLaunchKernelGGL((k_attn_tiles<T, HD, NW>), dim3(groups), dim3(64 * NW), 0, s, a, bytes);
+    hipLaunchKernelGGL((k_attn_join<T, HD, NW>), dim3(groups * NW), dim3(256), 0, s, a);
+}
 template <typename T, int HD>
 static void launch_attn(const uint32_t* w, void* const* p, hipStream_t s) {
     const float scale_log2 = f32_of(w[18]) * 1.4426950408889634f;
@@ -1499,10 +1509,10 @@ static void launch_attn(const uint32_t* w, void* const* p, hipStream_t s) {
     const uint32_t bytes = uint32_t(uint64_t(w[17]) * w[16] * w[13] * HD * 2);  // of each cache
     if (few_columns(w))
         hipLaunchKernelGGL((k_attn_rows<T, HD>), dim3(paged::kRowsGroups), dim3(256), 0, s, a, bytes, bytes);
-    else {
-        hipLaunchKernelGGL((k_attn_tiles<T, HD>), dim3(paged::kTileGroups), dim3(512), 0, s, a, bytes);
-        hipLaunchKernelGGL((k_attn_join<T, HD>), dim3(paged::kTileGroups * 8), dim3(256), 0, s, a);
-    }
+    else if (tile_waves_of(w) == 8)
+        launch_tiles<T, HD, 8>(a, bytes, s);
+    else if constexpr (HD == 64)
+        launch_tiles<T, HD, 4>(a, bytes, s);
 }
 static void l_attn(const PreparedDispatch& pd, void* const* p, hipStream_t s) {
     const uint32_t* w = pd.words.data();
@@ -1634,11 +1644,11 @@ std::vector<KernelSpec> paged_catalog() {
                      same_dtype("qk_norm_rope_append_paged", t, {8, 9, 10});
                      if (t[0].row.dtype() != F32) same_dtype("qk_norm_rope_append_paged", t, {0, 8});
                  }});
-    // 49 attention_paged (the catalog's thread count is that of the kernel for few columns; the tiles' has 512, and a second
-    // launch joins their split items)
+    // 49 attention_paged (the catalog's thread count is that of the kernel for few columns; the tiles' have 256 or 512, and a
+    // second launch joins their split items)
     c.push_back({"attention_paged", "paged", {256, 1, 1}, false,
                  [](const uint32_t* w) {
-                     return Grid3{int64_t(few_columns(w) ? paged::kRowsGroups : paged::kTileGroups), 1, 1};
+                     return Grid3{int64_t(few_columns(w) ? paged::kRowsGroups : paged::tile_groups(tile_waves_of(w))), 1, 1};
                  },
                  {TOK_R("q", H), TOK_R("k_cache", H), TOK_R("v_cache", H), TOK_R("table", U), TOK_R("starts", U),
                   TOK_R("context", U), TOK_W("y", H), TOK_RW("workspace", U), U32F("requests"), U32F("tokens"),
@@ -1654,10 +1664,10 @@ std::vector<KernelSpec> paged_catalog() {
                      need_table(n, blocks, page);
                      const float scale = f32_of(w[18]);
                      if (!(scale > 0.f) || std::isinf(scale)) contract_fail("%s: scale must be positive and finite", n);
-                     if (qh / kvh > paged::kTileCols)
-                         contract_fail("%s: at most %u query heads per KV head", n, paged::kTileCols);
+                     if (qh / kvh > paged::kMaxTileCols)
+                         contract_fail("%s: at most %u query heads per KV head", n, paged::kMaxTileCols);
                      // units: a tile of a request's rows (at least one a request) x the blocks of keys, on every KV head
-                     const uint64_t tiles = R + uint64_t(T) / (paged::kTileCols / (qh / kvh));
+                     const uint64_t tiles = R + uint64_t(T) / (paged::tile_cols(tile_waves_of(w)) / (qh / kvh));
                      if (times(few_columns(w) ? R : tiles, kvh,
                                uint64_t(blocks) * page / paged::kTileKeys + 1 + paged::kTileStart) > 1ull << 31)
                          contract_fail("%s: rows * kv_heads * blocks * page are more than one dispatch shares out", n);
