@@ -820,8 +820,13 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void k_attn_tiles(AttnArg
     constexpr int WK = KB / NW;            // keys of a block that a wave moves
     constexpr int LPB = WK * RB / 1024;    // its loads, of 1 KB each
     constexpr uint32_t GROUPS = paged::tile_groups(NW), COLS = paged::tile_cols(NW), SLOTS = paged::tile_slots(NW);
-    __shared__ __attribute__((aligned(16))) uint8_t lds[3 * KBLK + 2 * BLK];  // K blocks n % 3, then V blocks n % 2
-    __shared__ uint32_t ends[paged::kMaxRequests];
+    // Where two workgroups share a CU, heads of 128 leave room for two K blocks: a block's place is free for the one after the
+    // next only when all waves have its scores, one more barrier a step. And for one set of registers on the way to LDS.
+    constexpr bool TIGHT = HD == 128 && NW == 4;
+    constexpr int KN = TIGHT ? 2 : 3, SETS = TIGHT ? 1 : 2;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[KN * KBLK + 2 * BLK];  // K blocks n % KN, then V blocks n % 2
+    uint32_t* const ends = reinterpret_cast<uint32_t*>(lds);                 // until the first block takes its place
+    static_assert(sizeof(lds) >= 4 * paged::kMaxRequests);
     __shared__ uint32_t red[8];
     __shared__ uint32_t units_of_tile[64 * NW];
     __shared__ int chosen[3];
@@ -987,7 +992,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void k_attn_tiles(AttnArg
     }
     // operand reads: K row of matrix row c32 is key 16 (c32 / 16) + 8 (c32 / 4 % 2) + 4 (c32 / 8 % 2) + c32 % 4
     const int krow = (c32 & 19) | ((c32 & 4) << 1) | ((c32 & 8) >> 1);
-    const int kbase = krow * KR + 16 * h, vbase = 3 * KBLK + h * (8 * RB) + c32 * 16;
+    const int kbase = krow * KR + 16 * h, vbase = KN * KBLK + h * (8 * RB) + c32 * 16;
 
     constexpr int SW = int(paged::slot_words(COLS, HD));
     const __amdgpu_buffer_rsrc_t ws =
@@ -1037,19 +1042,19 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void k_attn_tiles(AttnArg
             soff = id < a.pages ? int((((id * uint32_t(kvh) + hk) << a.page_log2) + off) * RB) : 0;
         };
         // the chunks of this wave on their way to LDS: two blocks of each cache
-        u32x4 rk[2][LPB], rv[2][LPB];
+        u32x4 rk[SETS][LPB], rv[SETS][LPB];
         auto load_k = [&](auto set, int i, int soff) __attribute__((always_inline)) {
-            rk[decltype(set)::value][i] = __builtin_amdgcn_raw_buffer_load_b128(k_rsrc, 16 * lane + 1024 * i, soff, 0);
+            rk[decltype(set)::value % SETS][i] = __builtin_amdgcn_raw_buffer_load_b128(k_rsrc, 16 * lane + 1024 * i, soff, 0);
         };
         auto load_v = [&](auto set, int i, int soff) __attribute__((always_inline)) {
-            rv[decltype(set)::value][i] = __builtin_amdgcn_raw_buffer_load_b128(v_rsrc, 16 * lane + 1024 * i, soff, 0);
+            rv[decltype(set)::value % SETS][i] = __builtin_amdgcn_raw_buffer_load_b128(v_rsrc, 16 * lane + 1024 * i, soff, 0);
         };
         auto store_k = [&](auto set, int i, int slot) __attribute__((always_inline)) {
-            *reinterpret_cast<u32x4*>(lds + slot * KBLK + kst[i]) = rk[decltype(set)::value][i];
+            *reinterpret_cast<u32x4*>(lds + slot * KBLK + kst[i]) = rk[decltype(set)::value % SETS][i];
         };
         auto store_v = [&](auto set, int i, int slot) __attribute__((always_inline)) {
-            *reinterpret_cast<u32x4*>(lds + 3 * KBLK + slot * BLK + 1024 * (LPB * wv + i) + 16 * lane) =
-                rv[decltype(set)::value][i];
+            *reinterpret_cast<u32x4*>(lds + KN * KBLK + slot * BLK + 1024 * (LPB * wv + i) + 16 * lane) =
+                rv[decltype(set)::value % SETS][i];
         };
         const int tile_seen = rq.seen + row_first;  // keys that the tile's first row sees: all of its columns do
         auto hide_v = [&](auto set, int j, uint32_t bad) __attribute__((always_inline)) {
@@ -1060,13 +1065,13 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void k_attn_tiles(AttnArg
                     const int in = (bad >> (WK * wv >> 4) & 1u) ? 0 : left - WK * wv - i * 1024 / (8 * RB) * 8;
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        rv[decltype(set)::value][i][e] &= (2 * e < in ? 0x0000FFFFu : 0u) | (2 * e + 1 < in ? 0xFFFF0000u : 0u);
+                        rv[decltype(set)::value % SETS][i][e] &= (2 * e < in ? 0x0000FFFFu : 0u) | (2 * e + 1 < in ? 0xFFFF0000u : 0u);
                 }
             }
             if ((j0 + j + 1) * KB > tile_seen) {
                 bool any = false;
 #pragma unroll
-                for (int i = 0; i < LPB; ++i) any |= take_odd<T>(rv[decltype(set)::value][i]);
+                for (int i = 0; i < LPB; ++i) any |= take_odd<T>(rv[decltype(set)::value % SETS][i]);
                 if (any) odd = begin;
             }
         };
@@ -1176,8 +1181,9 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void k_attn_tiles(AttnArg
 #pragma unroll
         for (int i = 0; i < LPB; ++i) load_k(A0{}, i, s1), load_v(A0{}, i, s1);
         locate(min(1, nb - 1), s1, b1);
+        if constexpr (SETS == 2)
 #pragma unroll
-        for (int i = 0; i < LPB; ++i) load_k(A1{}, i, s1);
+            for (int i = 0; i < LPB; ++i) load_k(A1{}, i, s1);
         locate(min(2, nb - 1), s2, b2);
         locate(min(3, nb - 1), s3, b3);
         lds_barrier();  // the blocks of the piece before this one are read
@@ -1185,15 +1191,15 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void k_attn_tiles(AttnArg
 #pragma unroll
         for (int i = 0; i < LPB; ++i) {
             store_k(A0{}, i, 0);
-            load_k(A0{}, i, s2);
+            load_k(A0{}, i, SETS == 2 ? s2 : s1);
             store_v(A0{}, i, 0);
             load_v(A0{}, i, s1);
         }
 #pragma unroll
         for (int i = 0; i < LPB; ++i) {
             store_k(A1{}, i, 1);
-            load_k(A1{}, i, s3);
-            load_v(A1{}, i, s2);
+            load_k(A1{}, i, SETS == 2 ? s3 : s2);
+            if constexpr (SETS == 2) load_v(A1{}, i, s2);
         }
         s4 = s3, b4 = b3;
         lds_barrier();
@@ -1211,7 +1217,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void k_attn_tiles(AttnArg
         // PLAIN: every column sees all of this block and the next, all have pages, and more follow: nothing to ask
         auto step = [&](auto set, auto plain) __attribute__((always_inline)) {
             constexpr bool PLAIN = decltype(plain)::value;
-            const int kslot1 = kslot == 2 ? 0 : kslot + 1, kslot2 = kslot1 == 2 ? 0 : kslot1 + 1, vslot = n & 1;
+            const int kslot1 = kslot == KN - 1 ? 0 : kslot + 1, kslot2 = kslot1 == KN - 1 ? 0 : kslot1 + 1, vslot = n & 1;
             if (n) lds_barrier();
             if (PLAIN || n + 4 < nb) locate(n + 4, s4, b4);
             if (!PLAIN && n + 1 < nb) hide_v(set, n + 1, b1);
@@ -1221,26 +1227,40 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void k_attn_tiles(AttnArg
                 for (int x = 4 * LPB * part / parts; x < 4 * LPB * (part + 1) / parts; ++x) {
                     const int i = x >> 2;
                     if ((x & 3) == 0) store_k(set, i, kslot2);
-                    if ((x & 3) == 1) load_k(set, i, s4);
+                    if ((x & 3) == 1) load_k(set, i, SETS == 2 ? s4 : s3);
                     if ((x & 3) == 2) store_v(set, i, 1 - vslot);
-                    if ((x & 3) == 3) load_v(set, i, s3);
+                    if ((x & 3) == 3) load_v(set, i, SETS == 2 ? s3 : s2);
                 }
             };
-            if (PLAIN ? nbw > 0 : n < nbw) {
-                float mx = half(kslot, 1, sb, vslot, 0, sa, kslot1, 0, none);
+            const bool act = PLAIN ? nbw > 0 : n < nbw;
+            auto first_half = [&]() __attribute__((always_inline)) {
+                const float mx = half(kslot, 1, sb, vslot, 0, sa, kslot1, 0, none);
                 if constexpr (PLAIN)
                     follow(mx);
                 else
                     settle(n, 1, b0, sb, mx);
-                mx = half(kslot1, 0, sa, vslot, 1, sb, kslot1, 1, moves);  // (scores behind the last block: not used)
+            };
+            auto second_half = [&]() __attribute__((always_inline)) {
+                const float mx = half(kslot1, 0, sa, vslot, 1, sb, kslot1, 1, moves);  // (scores behind the last block: not used)
                 if constexpr (PLAIN)
                     follow(mx);
                 else
                     settle(n + 1, 0, b1, sa, mx);
+            };
+            if constexpr (TIGHT) {
+                if (act) first_half();
+                lds_barrier();
+                if (act)
+                    second_half();
+                else
+                    moves(0, 1);
+            } else if (act) {
+                first_half();
+                second_half();
             } else {
                 moves(0, 1);
             }
-            s3 = s4, b0 = b1, b1 = b2, b2 = b3, b3 = b4, kslot = kslot1, ++n;
+            s2 = s3, s3 = s4, b0 = b1, b1 = b2, b2 = b3, b3 = b4, kslot = kslot1, ++n;
         };
         const int plain = (b0 | b1 | b2 | b3) || no_page ? 0 : min(nb - 4, (rq.seen + row_first) / KB - 1 - j0);
         while (n + 1 < plain && !no_page) {  // (no_page: among the 16 blocks from n + 3 on)
@@ -1332,9 +1352,9 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void k_attn_tiles(AttnArg
             tile = 0;
             if (++hk >= kvh) {
                 hk = 0;
-                ++r;
-                while (r < int(a.requests) - 1 && uniform(int(ends[r])) == uniform(int(ends[r - 1]))) ++r;
-                enter(r);
+                do
+                    enter(++r);
+                while (rq.rows < 1 && r < int(a.requests) - 1);
             }
         }
     }
@@ -1494,7 +1514,7 @@ static uint32_t most_fresh(const uint32_t* w) { return w[11] ? std::min(w[11], w
 static bool few_columns(const uint32_t* w) {
     return w[13] && uint64_t(most_fresh(w)) * (w[12] / w[13]) <= paged::kRowsCols;
 }
-static uint32_t tile_waves_of(const uint32_t* w) { return paged::tile_waves(w[14], w[13] ? w[12] / w[13] : 0); }
+static uint32_t tile_waves_of(const uint32_t* w) { return paged::tile_waves(w[9], w[10], w[14], w[13] ? w[12] / w[13] : 0); }
 template <typename T, int HD, int NW>
 static void launch_tiles(const AttnArgs& a, uint32_t bytes, hipStream_t s) {
     constexpr uint32_t groups = paged::tile_groups(NW);
@@ -1511,7 +1531,7 @@ static void launch_attn(const uint32_t* w, void* const* p, hipStream_t s) {
         hipLaunchKernelGGL((k_attn_rows<T, HD>), dim3(paged::kRowsGroups), dim3(256), 0, s, a, bytes, bytes);
     else if (tile_waves_of(w) == 8)
         launch_tiles<T, HD, 8>(a, bytes, s);
-    else if constexpr (HD == 64)
+    else
         launch_tiles<T, HD, 4>(a, bytes, s);
 }
 static void l_attn(const PreparedDispatch& pd, void* const* p, hipStream_t s) {

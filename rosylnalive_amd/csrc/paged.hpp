@@ -32,12 +32,17 @@ inline bool page_ok(uint32_t page) { return page >= 16 && page <= 256 && (page &
 constexpr uint32_t kGroups = 512;  // the most workgroups of a launch
 // Items of few columns (a request's rows x the heads of a group up to 16): two workgroups per CU, units of 128 keys.
 constexpr uint32_t kRowsGroups = 512, kRowsKeys = 128, kRowsCols = 16;
-// Items of many columns: tiles of 32 columns per wave, units of 64 keys. Workgroups of four waves where two of them fit a CU and
-// a tile holds a row (heads of 64, up to 128 query heads per KV head), so that one's start, end and barriers run beside the
-// other's products (40 mixed requests with heads of 64: 31.6 us against 37.8 with eight waves, 3621 rows on 2581 positions 78.5
-// and 80.8); of eight otherwise. 2048 waves in all.
+// Items of many columns: tiles of 32 columns per wave, units of 64 keys, 2048 waves in all: workgroups of eight, one per CU, or of
+// four, two per CU, so that one's start, end and barriers run beside the other's products, and a single token among the
+// chunks holds half as much. Four for heads of 64 (40 mixed requests 31.6 us against 37.8, 3621 rows on 2581 positions 78.5 and
+// 80.8), and for heads of 128, whose blocks then have a place less in LDS, where most requests bring few rows (29 requests
+// with 3 chunks 24.6 us against 31.9, 48 of up to 8 rows 56.7 and 67.0, 16 21-row ones 31.0 and 31.5; but a prompt of 2048 31.7
+// and 29.9, 4096 rows on 28,672 positions 1009 and 954, and with fewer requests 14 of up to 30 rows 16.5 and 13.6). A row's heads
+// of a group have to fit a tile.
 constexpr uint32_t kTileKeys = 64, kMaxTileCols = 256;
-constexpr uint32_t tile_waves(uint64_t head_dim, uint64_t group) { return head_dim == 64 && group <= 128 ? 4 : 8; }
+constexpr uint32_t tile_waves(uint64_t requests, uint64_t tokens, uint64_t head_dim, uint64_t group) {
+    return group <= 128 && (head_dim == 64 || (requests >= 16 && tokens <= 64 * requests)) ? 4 : 8;
+}
 constexpr uint32_t tile_cols(uint32_t waves) { return 32 * waves; }
 constexpr uint32_t tile_groups(uint32_t waves) { return 2048 / waves; }
 // What the start of a tile weighs in even shares of the units, in units: its queries, its first blocks and the end of the tile
@@ -53,8 +58,11 @@ inline uint64_t workspace_words(uint64_t requests, uint64_t tokens, uint64_t q_h
                                 uint64_t head_dim) {
     (void)requests;
     const uint64_t rows = kGroups + 2 * kRowsGroups * slot_words(kRowsCols, head_dim);
-    const uint32_t waves = tile_waves(head_dim, kv_heads ? q_heads / kv_heads : 0);
-    const uint64_t tiles = tile_slots(waves) + 2 * tile_groups(waves) * slot_words(tile_cols(waves), head_dim);
+    uint64_t tiles = 0;
+    for (uint32_t waves : {4u, 8u}) {  // (which of them a dispatch of fewer requests or tokens takes is its own)
+        const uint64_t n = tile_slots(waves) + 2 * tile_groups(waves) * slot_words(tile_cols(waves), head_dim);
+        tiles = n > tiles ? n : tiles;
+    }
     return kv_heads && tokens * (q_heads / kv_heads) <= kRowsCols ? rows : (tiles > rows ? tiles : rows);
 }
 

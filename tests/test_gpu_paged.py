@@ -314,6 +314,16 @@ def test_attention_request_limits(requests):
     _attn_case(F16, 1, 1, 64, 16, [(i % 5, i % 2) for i in range(1, requests + 1)], pad=1)
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("qh,kvh,hd", [(16, 8, 128), (14, 2, 64), (200, 1, 64), (130, 1, 128), (24, 2, 128)])
+def test_attention_mixed_batches(dtype, qh, kvh, hd):
+    """Single tokens and chunks together: most requests with one row, of very different contexts, none that has rows first and
+    last."""
+    r = np.random.default_rng(12)
+    lens = [(30, 0)] + [(int(x), 1) for x in r.integers(0, 1500, 17)] + [(700, 90), (0, 40), (0, 0), (1000, 33), (64, 0)]
+    _attn_case(DT[dtype], qh, kvh, hd, 16, lens, pad=5)
+
+
 @pytest.mark.parametrize("qh,kvh,hd", [(256, 1, 64), (100, 1, 128), (34, 2, 64), (17, 1, 128)])
 def test_attention_large_groups(qh, kvh, hd):
     """Query heads per KV head that fill a tile with one row, leave columns over, and just miss the form for few."""
@@ -404,7 +414,8 @@ def test_attention_scores(dtype, fresh):
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("lens", [[(40, 2), (0, 3), (130, 4)], [(300, 90), (0, 77), (63, 5)], [(1900, 129), (5, 20)],
-                                  [(100, 200)] * 40], ids=["few", "chunks", "long", "many"])
+                                  [(100, 200)] * 40, [(500, 1)] * 17 + [(40, 90), (700, 150)]],
+                         ids=["few", "chunks", "long", "many", "mixed"])
 def test_attention_values_that_are_not_finite(dtype, hd, lens):
     """Infinities and NaN among a chunk's own values reach the rows that see them, in their dim of their head, and change no
     bit of any other row: what a row gives does not depend on the tokens after it."""
