@@ -812,7 +812,7 @@ __device__ __forceinline__ uint32_t floor_sum64(uint32_t n, uint32_t step, uint3
 // a library product of 8192^3 reaches 1159; matrix cores busy 55 % of the cycles. A prompt of 2048 30 us (570 TFLOP/s): 4 us
 // to start, 11 blocks of 1.9 us, 2 to store, 8 for the join.
 template <typename T, int HD, int NW>
-__global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void k_attn_tiles(AttnArgs a, uint32_t bytes) {
+__global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : HD == 64 ? 3 : 2) void k_attn_tiles(AttnArgs a, uint32_t bytes) {
     using M = Mfma<T>;
     constexpr int KB = int(paged::kTileKeys), KS = HD / 16, DT = HD / 32, RB = HD * 2, BLK = KB * RB;
     constexpr int KR = RB + 16, KBLK = KB * KR;  // a K row in LDS is padded by 16 bytes: 16 rows lie in different banks
@@ -820,10 +820,11 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void k_attn_tiles(AttnArg
     constexpr int WK = KB / NW;            // keys of a block that a wave moves
     constexpr int LPB = WK * RB / 1024;    // its loads, of 1 KB each
     constexpr uint32_t GROUPS = paged::tile_groups(NW), COLS = paged::tile_cols(NW), SLOTS = paged::tile_slots(NW);
-    // Where two workgroups share a CU, heads of 128 leave room for two K blocks: a block's place is free for the one after the
-    // next only when all waves have its scores, one more barrier a step. And for one set of registers on the way to LDS.
+    // Workgroups that share a CU have one set of registers on the way to LDS (for heads of 64 three of them fit then, from
+    // batches under way at once: 40 mixed requests 28.9 us against 31.1). Heads of 128 leave two of them room for two K
+    // blocks: a block's place is free for the one after the next only when all waves have its scores, one more barrier a step.
     constexpr bool TIGHT = HD == 128 && NW == 4;
-    constexpr int KN = TIGHT ? 2 : 3, SETS = TIGHT ? 1 : 2;
+    constexpr int KN = TIGHT ? 2 : 3, SETS = NW == 4 ? 1 : 2;
     __shared__ __attribute__((aligned(16))) uint8_t lds[KN * KBLK + 2 * BLK];  // K blocks n % KN, then V blocks n % 2
     uint32_t* const ends = reinterpret_cast<uint32_t*>(lds);                 // until the first block takes its place
     static_assert(sizeof(lds) >= 4 * paged::kMaxRequests);
