@@ -801,8 +801,8 @@ __device__ __forceinline__ uint32_t floor_sum64(uint32_t n, uint32_t step, uint3
 // eight waves or two workgroups of four per CU: two waves per SIMD, so that one's VALU work runs beside the other's matrix
 // instructions (four waves of 64 columns would read half as much from LDS, but past 256 registers every product's result
 // has to come out of the accumulation file first: 1317 us where this form takes 992). K and V blocks of 64 keys go from the
-// pages through registers into LDS (three K blocks, two V blocks), loaded two steps before they are stored; one barrier per
-// block. (Loads straight into LDS made the compiler wait for all of them before every LDS read.) V's layout in the cache is
+// pages through registers into LDS (three K blocks, two V blocks), loaded two steps before they are stored (one in workgroups
+// of four waves); one barrier per block. (Loads straight into LDS made the compiler wait for all of them before every LDS read.) V's layout in the cache is
 // already the order in which it is read.
 // Step n: the scores of block n + 1 (matrix core) under the exponentials of block n (VALU), then block n's products
 // under the maxima of block n + 1. The rows of S^T's tiles hold the keys in the order in which P^T wants them (bits 2 and 3
