@@ -324,6 +324,15 @@ def test_attention_mixed_batches(dtype, qh, kvh, hd):
     _attn_case(DT[dtype], qh, kvh, hd, 16, lens, pad=5)
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("qh,kvh,hd", [(16, 8, 128), (12, 12, 64), (32, 8, 128)])
+def test_attention_many_items(dtype, qh, kvh, hd):
+    """More items than workgroups: pieces of several, the parts of others, requests without rows between them."""
+    r = np.random.default_rng(13)
+    lens = [(int(x), int(f)) for x, f in zip(r.integers(0, 700, 90), r.choice([0, 1, 1, 1, 2, 20], 90))] + [(300, 150), (1400, 40)]
+    _attn_case(DT[dtype], qh, kvh, hd, 32, lens, pad=2)
+
+
 @pytest.mark.parametrize("qh,kvh,hd", [(256, 1, 64), (100, 1, 128), (34, 2, 64), (17, 1, 128)])
 def test_attention_large_groups(qh, kvh, hd):
     """Query heads per KV head that fill a tile with one row, leave columns over, and just miss the form for few."""
