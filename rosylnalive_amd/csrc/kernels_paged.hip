@@ -324,6 +324,7 @@ struct AttnArgs {
     void* y;
     uint32_t* ws;
     uint32_t requests, tokens, max_fresh, qh, kvh, blocks, page_log2, pages;
+    uint32_t join_here;  // the tiles' last workgroup of an item joins its parts
     float scale_log2;  // the scale times log2(e): weights are 2^(s scale_log2 - m scale_log2)
 };
 
@@ -797,6 +798,71 @@ __device__ __forceinline__ uint32_t floor_sum64(uint32_t n, uint32_t step, uint3
     return sum;
 }
 
+// The join of an item of the tiles: y = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i over its parts, in their order. This wave
+// takes a quarter part_d of the dims of its 32 columns of the tile.
+struct Split {
+    int parts, base, stride, first;  // part i in slot base + i stride (+ `first` for the first)
+    int row0, cols, hk;
+};
+template <typename T, int HD, int NW, int SCOPE>
+__device__ __forceinline__ void join_item(const AttnArgs& a, const Split& p, int wv, int part_d, int lane) {
+    constexpr int DT = HD / 32, N = DT;  // 16 bytes per lane and part
+    constexpr uint32_t GROUPS = paged::tile_groups(NW), COLS = paged::tile_cols(NW), SLOTS = paged::tile_slots(NW);
+    constexpr int SW = int(paged::slot_words(COLS, HD));
+    const int parts = p.parts, cols = p.cols, row0 = p.row0, hk = p.hk, col = 32 * wv + (lane & 31);
+    const __amdgpu_buffer_rsrc_t ws =
+        __builtin_amdgcn_make_buffer_rsrc(a.ws, 0, int(4 * (SLOTS + 2 * GROUPS * SW)), 0x00020000);
+    auto slot_at = [&](int i) { return int(SLOTS) + (p.base + i * p.stride + (i ? 0 : p.first)) * SW; };
+    constexpr int PF = SCOPE ? 2 : 6;  // parts under way (the tiles have fewer registers to spare)
+    float top = -INFINITY, l = 0.f, sum[4 * N];
+#pragma unroll
+    for (int e = 0; e < 4 * N; ++e) sum[e] = 0.f;
+    for (int i = 0; i < parts; i += PF) {
+        float2 ml[PF];
+        f32x4 x[PF][N];
+#pragma unroll
+        for (int q = 0; q < PF; ++q) {
+            if (i + q >= parts) break;
+            const int slot = slot_at(i + q);
+            ml[q] = load_part2<SCOPE>(ws, slot + 2 * col);
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                x[q][j] = load_part<SCOPE>(ws, slot + 2 * int(COLS) + ((wv * 4 * DT + part_d * N + j) * 64 + lane) * 4);
+        }
+        __builtin_amdgcn_sched_barrier(0);  // (all under way before the first is waited for)
+        float most = top;
+#pragma unroll
+        for (int q = 0; q < PF; ++q) {
+            if (i + q >= parts) break;
+            most = fmaxf(most, ml[q].x);
+        }
+        const float tc = most == -INFINITY ? 0.f : most * a.scale_log2;
+        const float back = __builtin_amdgcn_exp2f(top * a.scale_log2 - tc);
+        top = most;
+        l *= back;
+#pragma unroll
+        for (int e = 0; e < 4 * N; ++e) sum[e] *= back;
+#pragma unroll
+        for (int q = 0; q < PF; ++q) {
+            if (i + q >= parts) break;
+            const float f = __builtin_amdgcn_exp2f(ml[q].x * a.scale_log2 - tc);
+            l += ml[q].y * f;
+#pragma unroll
+            for (int e = 0; e < 4 * N; ++e) sum[e] += x[q][e >> 2][e & 3] * f;
+        }
+    }
+    if (col >= cols) return;
+    const int group = int(a.qh / a.kvh);
+    const float inv = l != 0.f ? 1.0f / l : 0.f;  // no key at all: zeros
+    T* y = static_cast<T*>(a.y) + (size_t(row0 + col / group) * a.qh + hk * group + col % group) * HD + 4 * (lane >> 5);
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const int i = part_d * N + j;  // dims 32 (i / 4) + 8 (i % 4) + 4 h ..
+        *reinterpret_cast<uint2*>(y + 32 * (i >> 2) + 8 * (i & 3)) =
+            make_uint2(pack<T>(sum[4 * j] * inv, sum[4 * j + 1] * inv), pack<T>(sum[4 * j + 2] * inv, sum[4 * j + 3] * inv));
+    }
+}
+
 // Rows of many query columns, on 32 x 32 x 16 tiles. A tile of an item is up to 32 columns per wave (whole rows of the request),
 // eight waves or two workgroups of four per CU: two waves per SIMD, so that one's VALU work runs beside the other's matrix
 // instructions (four waves of 64 columns would read half as much from LDS, but past 256 registers every product's result
@@ -831,6 +897,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : HD == 64 ? 3 : 2) void k_att
     __shared__ uint32_t red[8];
     __shared__ uint32_t units_of_tile[64 * NW];
     __shared__ int chosen[3];
+    __shared__ uint32_t arrived;
     __shared__ uint32_t odd;  // the first unit of the last piece that held values to take out
     const int t = threadIdx.x, lane = t & 63, wv = uniform(t >> 6), c32 = lane & 31, h = lane >> 5;
     const int group = int(a.qh / a.kvh), kvh = int(a.kvh), TR = int(COLS) / group;
@@ -877,7 +944,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : HD == 64 ? 3 : 2) void k_att
     int parts = 0, mine = 0, lead = 0;                          // of an item with workgroups of its own
     // what the join has to know of a split item: written by the workgroup that begins it, by the others as none
     auto describe = [&](int parts, int base, int stride, int first, const Request& q, int row_first, int cols, int hk) {
-        if (t != 0) return;
+        if (t != 0 || a.join_here) return;
         u32x4* d = reinterpret_cast<u32x4*>(a.ws + paged::kGroups) + 2 * w;
         d[0] = u32x4{uint32_t(parts), uint32_t(base), uint32_t(stride), uint32_t(first)};
         d[1] = u32x4{uint32_t(q.row0 + row_first), uint32_t(cols), uint32_t(hk), 0u};
@@ -1343,6 +1410,21 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : HD == 64 ? 3 : 2) void k_att
                                f32x4{x[e], x[e + 1], x[e + 2], x[e + 3]});
                 }
             }
+            if (a.join_here) {
+                __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0): this wave's stores are performed
+                lds_barrier();
+                uint32_t* const counter = a.ws + lead;
+                if (t == 0) arrived = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                lds_barrier();
+                if (uint32_t(uniform(int(arrived))) == uint32_t(parts - 1)) {
+                    if (cw < cols)
+#pragma unroll 1
+                        for (int d = 0; d < 4; ++d)
+                            join_item<T, HD, NW, kDeviceScope>(
+                                a, Split{parts, base, stride, first, rq.row0 + row_first, cols, hk}, wv, d, lane);
+                    if (t == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                }
+            }
         }
         if (apart) break;
         // ---- the next piece
@@ -1362,72 +1444,16 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : HD == 64 ? 3 : 2) void k_att
     if (!described) describe_none();
 }
 
-// The join of k_attn_tiles' split items: y = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i over an item's parts, in their
-// order. A launch of its own, for all CUs: the last workgroup of an item to end, if it joined them, would read 128 KiB a
-// part alone (1.5 us each, 12 us for the eight parts of a 512-row chunk at 8K). Block (item, wave of the tile): its four
-// waves take a quarter of each column's dims each.
+// The joins of k_attn_tiles' split items where they may have many parts, a launch of its own for all CUs (kJoinHere). Block
+// (item, wave of the tile): its four waves take a quarter of each column's dims each.
 template <typename T, int HD, int NW>
 __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {
-    constexpr uint32_t GROUPS = paged::tile_groups(NW), COLS = paged::tile_cols(NW), SLOTS = paged::tile_slots(NW);
-    constexpr int DT = HD / 32, N = DT;  // 16 bytes per lane and part
-    constexpr int SW = int(paged::slot_words(COLS, HD));
-    const int lead = blockIdx.x / NW, wv = blockIdx.x % NW, t = threadIdx.x, lane = t & 63, part_d = t >> 6, c32 = lane & 31;
+    const int lead = blockIdx.x / NW, wv = blockIdx.x % NW, t = threadIdx.x;
     const u32x4* d = reinterpret_cast<const u32x4*>(a.ws + paged::kGroups) + 2 * lead;
     const u32x4 d0 = d[0], d1 = d[1];
-    const int parts = uniform(int(d0[0])), base = uniform(int(d0[1])), stride = uniform(int(d0[2])), first = uniform(int(d0[3]));
-    const int row0 = int(d1[0]), cols = int(d1[1]), hk = int(d1[2]), col = 32 * wv + c32;
-    if (parts == 0 || 32 * wv >= cols) return;
-    const __amdgpu_buffer_rsrc_t ws =
-        __builtin_amdgcn_make_buffer_rsrc(a.ws, 0, int(4 * (SLOTS + 2 * GROUPS * SW)), 0x00020000);
-    auto slot_at = [&](int i) { return int(SLOTS) + (base + i * stride + (i ? 0 : first)) * SW; };
-    constexpr int PF = 6;
-    float top = -INFINITY, l = 0.f, sum[4 * N];
-#pragma unroll
-    for (int e = 0; e < 4 * N; ++e) sum[e] = 0.f;
-    for (int i = 0; i < parts; i += PF) {
-        float2 ml[PF];
-        f32x4 x[PF][N];
-#pragma unroll
-        for (int q = 0; q < PF; ++q) {
-            if (i + q >= parts) break;
-            const int slot = slot_at(i + q);
-            ml[q] = load_part2<0>(ws, slot + 2 * col);
-#pragma unroll
-            for (int j = 0; j < N; ++j)
-                x[q][j] = load_part<0>(ws, slot + 2 * int(COLS) + ((wv * 4 * DT + part_d * N + j) * 64 + lane) * 4);
-        }
-        __builtin_amdgcn_sched_barrier(0);  // (all under way before the first is waited for)
-        float most = top;
-#pragma unroll
-        for (int q = 0; q < PF; ++q) {
-            if (i + q >= parts) break;
-            most = fmaxf(most, ml[q].x);
-        }
-        const float tc = most == -INFINITY ? 0.f : most * a.scale_log2;
-        const float back = __builtin_amdgcn_exp2f(top * a.scale_log2 - tc);
-        top = most;
-        l *= back;
-#pragma unroll
-        for (int e = 0; e < 4 * N; ++e) sum[e] *= back;
-#pragma unroll
-        for (int q = 0; q < PF; ++q) {
-            if (i + q >= parts) break;
-            const float f = __builtin_amdgcn_exp2f(ml[q].x * a.scale_log2 - tc);
-            l += ml[q].y * f;
-#pragma unroll
-            for (int e = 0; e < 4 * N; ++e) sum[e] += x[q][e >> 2][e & 3] * f;
-        }
-    }
-    if (col >= cols) return;
-    const int group = int(a.qh / a.kvh);
-    const float inv = l != 0.f ? 1.0f / l : 0.f;  // no key at all: zeros
-    T* y = static_cast<T*>(a.y) + (size_t(row0 + col / group) * a.qh + hk * group + col % group) * HD + 4 * (lane >> 5);
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-        const int i = part_d * N + j;  // dims 32 (i / 4) + 8 (i % 4) + 4 h ..
-        *reinterpret_cast<uint2*>(y + 32 * (i >> 2) + 8 * (i & 3)) =
-            make_uint2(pack<T>(sum[4 * j] * inv, sum[4 * j + 1] * inv), pack<T>(sum[4 * j + 2] * inv, sum[4 * j + 3] * inv));
-    }
+    const Split p{uniform(int(d0[0])), uniform(int(d0[1])), uniform(int(d0[2])), uniform(int(d0[3])), int(d1[0]), int(d1[1]), int(d1[2])};
+    if (p.parts == 0 || 32 * wv >= p.cols) return;
+    join_item<T, HD, NW, 0>(a, p, wv, t >> 6, t & 63);
 }
 
 }  // namespace
@@ -1520,13 +1546,14 @@ template <typename T, int HD, int NW>
 static void launch_tiles(const AttnArgs& a, uint32_t bytes, hipStream_t s) {
     constexpr uint32_t groups = paged::tile_groups(NW);
     hipLaunchKernelGGL((k_attn_tiles<T, HD, NW>), dim3(groups), dim3(64 * NW), 0, s, a, bytes);
-    hipLaunchKernelGGL((k_attn_join<T, HD, NW>), dim3(groups * NW), dim3(256), 0, s, a);
+    if (!a.join_here) hipLaunchKernelGGL((k_attn_join<T, HD, NW>), dim3(groups * NW), dim3(256), 0, s, a);
 }
 template <typename T, int HD>
 static void launch_attn(const uint32_t* w, void* const* p, hipStream_t s) {
     const float scale_log2 = f32_of(w[18]) * 1.4426950408889634f;
     const AttnArgs a{p[0], p[1], p[2], (const uint32_t*)p[3], (const uint32_t*)p[4], (const uint32_t*)p[5], p[6],
-                     (uint32_t*)p[7], w[9], w[10], most_fresh(w), w[12], w[13], w[15], log2_of(w[16]), w[17], scale_log2};
+                     (uint32_t*)p[7], w[9], w[10], most_fresh(w), w[12], w[13], w[15], log2_of(w[16]), w[17], uint32_t(uint64_t(w[15]) * w[16] <= paged::kJoinHere),
+                     scale_log2};
     const uint32_t bytes = uint32_t(uint64_t(w[17]) * w[16] * w[13] * HD * 2);  // of each cache
     if (few_columns(w))
         hipLaunchKernelGGL((k_attn_rows<T, HD>), dim3(paged::kRowsGroups), dim3(256), 0, s, a, bytes, bytes);

@@ -26,9 +26,9 @@ inline bool page_ok(uint32_t page) { return page >= 16 && page <= 256 && (page &
 // Either every item has workgroups of its own, or workgroup w of G takes the units [w units / G, (w + 1) units / G) of all
 // items in order (for tiles weighted, kTileStart); both follow the lengths on the device. An item of several workgroups is joined from partials in the
 // workspace, two slots per workgroup: 2 w for the part of an item that w finds begun (or the part of its own), 2 w + 1 for
-// the part of the one that it begins and does not end. Before them stand kGroups words, in which the items of few columns
-// count their parts in (word w for the one that w begins; zero between launches), and for the items of many columns what
-// their join has to know, eight words per workgroup.
+// the part of the one that it begins and does not end. Before them stand kGroups words, in which the items count their parts
+// in where the last one to arrive joins them (word w for the one that w begins; zero between launches), and for the tiles what
+// a join in a launch of its own has to know, eight words per workgroup.
 constexpr uint32_t kGroups = 512;  // the most workgroups of a launch
 // Items of few columns (a request's rows x the heads of a group up to 16): two workgroups per CU, units of 128 keys.
 constexpr uint32_t kRowsGroups = 512, kRowsKeys = 128, kRowsCols = 16;
@@ -43,6 +43,11 @@ constexpr uint32_t kTileKeys = 64, kMaxTileCols = 256;
 constexpr uint32_t tile_waves(uint64_t requests, uint64_t tokens, uint64_t head_dim, uint64_t group) {
     return group <= 128 && (head_dim == 64 || (requests >= 16 && tokens <= 64 * requests)) ? 4 : 8;
 }
+// The tiles' split items are joined by their last workgroup where the table holds no more than this many positions, so that
+// parts are few, and by a second launch over all CUs otherwise (64-row prompts 5.5 us and 7.7, 41 rows among 24 requests of up
+// to 655 positions 15.3 and 17.1, a prompt of 2263 28.3 and 27.8; but 13 rows on 3576 positions 23.8 and 16.8, 24 on 11,275 74 and
+// 26: the last one reads the parts alone, 1.5 us each).
+constexpr uint32_t kJoinHere = 2048;
 constexpr uint32_t tile_cols(uint32_t waves) { return 32 * waves; }
 constexpr uint32_t tile_groups(uint32_t waves) { return 2048 / waves; }
 // What the start of a tile weighs in even shares of the units, in units: its queries, its first blocks and the end of the tile
