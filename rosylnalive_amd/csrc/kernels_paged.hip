@@ -1693,7 +1693,7 @@ std::vector<KernelSpec> paged_catalog() {
                      if (t[0].row.dtype() != F32) same_dtype("qk_norm_rope_append_paged", t, {0, 8});
                  }});
     // 49 attention_paged (the catalog's thread count is that of the kernel for few columns; the tiles' have 256 or 512, and a
-    // second launch joins their split items)
+    // second launch may join their split items)
     c.push_back({"attention_paged", "paged", {256, 1, 1}, false,
                  [](const uint32_t* w) {
                      return Grid3{int64_t(few_columns(w) ? paged::kRowsGroups : paged::tile_groups(tile_waves_of(w))), 1, 1};
