@@ -481,6 +481,8 @@ uint64_t Device::submit(CommandList* l, uint32_t repeat) {
     if (repeat < 1) contract_fail("a submission runs its list at least once");
     if (repeat > 1 && !l->reusable_) contract_fail("only a reusable list can be replayed");
     HIPC(hipSetDevice(index_));
+    const bool few = uint64_t(l->cmds_.size()) * repeat <= kDirectLaunches;
+    if (marked_ < next_fence_ - 1 && (!few || host_ns() - marked_ns_ >= kMarkNs)) mark(next_fence_ - 1);
     Pending pend{};
     pend.dispatches = l->dispatches_ * int(repeat);
     if (!l->reusable_) {
@@ -565,7 +567,7 @@ uint64_t Device::submit(CommandList* l, uint32_t repeat) {
     }
     uint64_t fence = next_fence_++;
     pending_[fence] = std::move(pend);
-    if (host_ns() - marked_ns_ >= kMarkNs) mark(fence);
+    if (!few || host_ns() - marked_ns_ >= kMarkNs) mark(fence);
     return fence;
 }
 
@@ -583,13 +585,14 @@ void Device::mark(uint64_t fence) {
         hip_check(r, "hipEventRecord");
     }
     marks_.push_back(Mark{fence, e});
+    marked_ = fence;
     marked_ns_ = host_ns();
 }
 
 void Device::reach(uint64_t fence) {
     if (fence <= reached_) return;
     HIPC(hipSetDevice(index_));
-    if (marks_.empty() || marks_.back().fence < fence) mark(next_fence_ - 1);
+    if (marked_ < fence) mark(next_fence_ - 1);
     while (marks_.front().fence < fence) {  // older ones are behind the one waited for
         spare_events_.push_back(marks_.front().event);
         marks_.pop_front();

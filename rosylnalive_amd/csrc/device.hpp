@@ -252,8 +252,10 @@ class Device {
     };
     std::map<uint64_t, Pending> pending_;
     // Completion of submissions: events on the stream, each for every submission up to its own, oldest first. Recording one
-    // costs 4 us of host time on MI355X, more than a kernel's launch (2.6 us), so submissions that follow each other within
-    // kMarkNs share one; a wait for a submission that has none behind it records one then.
+    // costs 4 us of host time on MI355X, more than a kernel's launch (2.6 us), so submissions of up to kDirectLaunches
+    // commands that follow each other within kMarkNs share one. Before anything else is launched behind a submission without
+    // an event (more commands, or kMarkNs later) it gets one, so no wait ever covers that later work; a wait for a submission
+    // that has none behind it yet records one then.
     struct Mark {
         uint64_t fence;
         hipEvent_t event;
@@ -263,7 +265,8 @@ class Device {
     void reach(uint64_t fence);  // waits until every submission up to `fence` has completed
     std::deque<Mark> marks_;
     std::vector<hipEvent_t> spare_events_;
-    int64_t marked_ns_ = 0;       // host clock at the last mark
+    uint64_t marked_ = 0;         // the last submission that was marked, and the host clock then
+    int64_t marked_ns_ = 0;
     uint64_t reached_ = 0;        // submissions up to this one have completed
     std::map<uint64_t, Completion> done_;  // the last kKeptCompletions waited on, by fence
 

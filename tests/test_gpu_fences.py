@@ -1,5 +1,7 @@
 """Submissions that share a completion event: short lists made right behind each other, waited for in any order; and replays of
 short reusable lists, which are launched again rather than captured, next to captured ones."""
+import time
+
 import numpy as np
 import pytest
 
@@ -90,3 +92,58 @@ def test_replays_of_short_and_long_lists(sess, launches):
     with pytest.raises(GpuContractException, match="timers"):
         sess.backend.submit(cl)
     cl.release()
+
+
+@pytest.fixture()
+def long():
+    """A session whose one launch over 32 million values takes about 60 us, and small tensors beside them."""
+    n = 1 << 25
+    s = Session({"big": (F32, (n,), 0, np.zeros(n, np.float32)), "x": (F32, (N,), 0, np.ones(N, np.float32)),
+                 "y": (F32, (N,), 0, None)})
+    s.n_big = n
+    yield s
+    s.close()
+
+
+def _long_list(s, launches, reusable):
+    cl = s.backend.begin(reusable=reusable)
+    for _ in range(launches):
+        cl.dispatch("scale_f32", s.fields("scale_f32", x="big", y="big", n=s.n_big, a=1.0))
+    return cl
+
+
+@pytest.mark.parametrize("form", ["direct", "captured", "one shot"])
+@pytest.mark.parametrize("pause", [0.0, 1e-3])
+def test_a_wait_does_not_cover_long_work_submitted_later(long, form, pause):
+    """Two short submissions right behind each other, so that the second has no completion event of its own, then a long one, at
+    once or a millisecond later: the wait for the second returns while the long one still runs, which the wait for that one
+    then shows."""
+    s = long
+    launches = {"direct": 4, "captured": 40, "one shot": 400}[form]
+    repeat = 400 // launches
+    short = s.backend.begin(reusable=True)
+    _scale(s, short, 2.0)
+    s.backend.wait(s.backend.submit(short))
+    late = _long_list(s, launches, form != "one shot")
+    if form != "one shot":
+        s.backend.wait(s.backend.submit(late))  # (the first submission captures)
+    good = 0
+    for _ in range(5):
+        time.sleep(1e-3)
+        a, b = s.backend.submit(short), s.backend.submit(short)
+        if pause:
+            s.backend.wait(a)
+            time.sleep(pause)
+        c = s.backend.submit(late, repeat if form != "one shot" else 1)
+        t0 = time.perf_counter()
+        s.backend.wait(b)
+        t1 = time.perf_counter()
+        s.backend.wait(c)
+        t2 = time.perf_counter()
+        good += t1 - t0 < t2 - t1
+        if form == "one shot":
+            late.release()
+            late = _long_list(s, launches, False)
+    assert good >= 4  # (the host may be held up once)
+    short.release()
+    late.release()
