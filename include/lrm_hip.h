@@ -142,7 +142,7 @@ int lrm_hip_denormal_probe(lrm_hip_device *d, int *mode, uint32_t results[7]);
  *   table row of rank 4, its last dimension is 8 head_dim);
  *   table [requests][blocks]: the page of each `page` positions of a request; 0xFFFFFFFF (any id >= pages) is none;
  *   starts [requests + 1]: request r's new rows are starts[r] .. starts[r + 1] - 1 of the batch's `tokens` rows (not
- *   decreasing); context [requests]: its positions, the new ones included.
+ *   decreasing: where they do, attention_paged computes no row); context [requests]: its positions, the new ones included.
  * Lengths are device memory: one recorded list serves every step, padded to `tokens` rows and `requests` requests (a request
  * of no new rows costs nothing). Rows behind the last request's are left as they were. requests is at most 4096, blocks *
  * page at most 2^30. Indices from device memory that point nowhere are skipped, never followed.

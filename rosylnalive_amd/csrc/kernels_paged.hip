@@ -340,6 +340,15 @@ __device__ __forceinline__ Request request_of(const AttnArgs& a, uint32_t r) {
     return Request{int(s0), min(fresh, int(a.max_fresh)), ctx - fresh + 1};
 }
 
+// The sums of a request's share of the work over the requests before it hold because their rows lie one after the other: at
+// most `tokens` in all, which is what a dispatch was checked for. Where starts decrease, the rows of several requests may
+// overlap and their sums pass 32 bits, so such a sum is kNoSum from there on (add_sat and scan_sat stay there) and nothing
+// is computed.
+constexpr uint32_t kNoSum = 0xFFFFFFFFu;
+__device__ __forceinline__ uint32_t add_share(const AttnArgs& a, uint32_t r, uint32_t sum, uint32_t share) {
+    return a.starts[r + 1] < a.starts[r] ? kNoSum : add_sat(sum, share);
+}
+
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 // words that no launch writes while it reads them, at uniform addresses: scalar loads
@@ -464,7 +473,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(AttnArgs a, uint32_t k_byt
         const uint32_t per = (a.requests + 255) / 256, r0 = min(t * per, a.requests), r1 = min(r0 + per, a.requests);
         uint32_t sum = 0;
         for (uint32_t r = r0; r < r1; ++r) {
-            sum += uint32_t(units_of(request_of(a, r)) * kvh);
+            sum = add_share(a, r, sum, uint32_t(units_of(request_of(a, r)) * kvh));
             ends[r] = sum;
         }
         const uint32_t before = scan_sat(sum, red) - sum;
@@ -472,7 +481,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(AttnArgs a, uint32_t k_byt
         __syncthreads();
     }
     const uint32_t total = ends[a.requests - 1], G = min(uint32_t(gridDim.x), total), w = blockIdx.x;
-    if (w >= G) return;
+    if (w >= G || total == kNoSum) return;
     auto first_unit = [&](uint32_t i) { return uint32_t(uint64_t(total) * i / G); };
     auto group_of = [&](uint32_t u) { return uint32_t(((uint64_t(u) + 1) * G - 1) / total); };
     const uint32_t u0 = first_unit(w), u1 = first_unit(w + 1);
@@ -925,7 +934,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : HD == 64 ? 3 : 2) void k_att
         uint32_t sum = 0;
         for (uint32_t r = r0; r < r1; ++r) {
             const Request q = request_of(a, r);
-            if (q.rows > 0) sum += f(q);
+            sum = add_share(a, r, sum, q.rows > 0 ? f(q) : 0u);
             ends[r] = sum;
         }
         const uint32_t before = scan_sat(sum, red) - sum;
@@ -952,7 +961,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : HD == 64 ? 3 : 2) void k_att
     auto describe_none = [&]() { describe(0, 0, 0, 0, Request{}, 0, 0, 0); };
     scan_requests([&](const Request& q) { return uint32_t(tiles_of(q)); });
     const uint32_t tiles_all = ends[a.requests - 1];
-    if (tiles_all == 0) {
+    if (tiles_all == 0 || tiles_all == kNoSum) {
         describe_none();
         return;
     }

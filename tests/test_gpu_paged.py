@@ -514,6 +514,58 @@ def test_attention_replayed_with_other_lengths():
         s.close()
 
 
+@pytest.mark.parametrize("hd,wide", [(128, 0), (64, 0), (128, 200)])
+def test_attention_starts_that_decrease(hd, wide):
+    """Starts that decrease somewhere (requests whose rows would overlap) compute nothing, in either form and however split
+    items are joined; the next dispatch with good ones finds the workspace as it has to be."""
+    qh, kvh, page, R, T = 4, 2, 16, 300, 90
+    r = np.random.default_rng(17)
+    past, fresh = r.integers(0, 60, R), np.zeros(R, np.int64)
+    fresh[r.permutation(R)[:45]] = 2
+    blocks, pages = 5 + wide, 99
+    good = np.concatenate([[0], np.cumsum(fresh)]).astype(np.uint32)
+    kb, vb = O.to_bits(F16, r.standard_normal((pages, kvh, page, hd))), O.to_bits(F16, r.standard_normal((pages, kvh, page // 8, hd, 8)))
+    qb = O.to_bits(F16, r.standard_normal((T, qh * hd)))
+    table = r.integers(0, pages, (R, blocks)).astype(np.uint32)
+    u = lambda a: (U32, np.shape(a), 0, np.asarray(a, np.uint32))  # noqa: E731
+    words = attention_paged_workspace_words(R, T, qh, kvh, hd)
+    s = Session({"q": (F16, qb.shape, RO, qb), "k_cache": (F16, kb.shape, RO, kb), "v_cache": (F16, _rank4(vb), RO, vb),
+                 "table": u(table), "starts": u(good), "context": u(past + fresh), "y": (F16, qb.shape, 0, None),
+                 "workspace": u(np.zeros(words))})
+    f = O.from_bits
+    want, bound = O.attention(f(F16, qb), f(F16, kb), f(F16, vb), table, good, past + fresh, qh, kvh, hd, page, pages, blocks, T, T,
+                              float(np.float32(hd ** -0.5)), F16, np.zeros(qb.shape))
+
+    def run(starts, most):
+        s.write("starts", starts.astype(np.uint32))
+        s.write("y", s.poison("y"))
+        cl = s.backend.begin()
+        cl.dispatch("attention_paged", s.fields(
+            "attention_paged", **{n: n for n in s.spec}, requests=R, tokens=T, max_fresh=most, q_heads=qh, kv_heads=kvh,
+            head_dim=hd, blocks=blocks, page=page, pages=pages, scale=hd ** -0.5))
+        s.backend.wait(s.backend.submit(cl))
+        cl.release()
+        return s.read("y")
+
+    turns = np.zeros(R + 1, np.int64)
+    turns[1::2] = T
+    last, first = good.copy(), good.copy()
+    last[R] = T - 1 - last[R] % 2
+    last[R - 1] = T
+    first[0] = 1
+    first[1] = 0
+    far = np.where(np.arange(R + 1) == 7, 0xFFFFFFFF, good)
+    try:
+        for most in (2, 0):
+            for starts in (turns, turns[::-1], last, first, far):
+                assert np.all(run(starts, most) == POISON_16)
+            assert np.all(s.read("workspace")[:512] == 0)
+            y = run(good, most)
+            assert np.all((np.abs(f(F16, y) - want) <= bound)[bound >= 0]) and np.all(y[bound < 0] == POISON_16)
+    finally:
+        s.close()
+
+
 def _batch(seed, lens, qh, kvh, hd, page, outputs, workspaces, tokens):
     """A session with one ragged batch in it and as many results and workspaces, and the dispatch's fields for each form."""
     r = np.random.default_rng(seed)
