@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes as C
 import struct
+import threading
 from dataclasses import dataclass, field
 from typing import Dict, List, Optional, Sequence, Tuple
 
@@ -381,8 +382,20 @@ class Submission(int):
     pass
 
 
+class _Results(threading.local):
+    """Where a thread's submits and waits find their results. ctypes lets other threads run during a call, so each has its
+    own; they are made once, since a step has a call of each."""
+
+    def __init__(self):
+        self.fence, self.dispatches, self.timers = C.c_uint64(), C.c_int(), C.c_int()
+        self.refs = C.byref(self.fence), C.byref(self.dispatches), C.byref(self.timers)
+
+
+_results = _Results()
+
+
 class HipBackend:
-    """IGpuBackend on one gfx950 device (Backend.fs:139-153)."""
+    """IGpuBackend on one gfx950 device (Backend.fs:139-153). Calls on one backend come from one thread at a time."""
 
     def __init__(self, index: int = 0, time_dispatches: bool = False):
         self._h = C.c_void_p()
@@ -392,12 +405,6 @@ class HipBackend:
         self.info = _info(s)
         self.heap: Optional[HipHeap] = None
         self.shader_set_hash: Optional[bytes] = None
-        self._results()
-
-    def _results(self):
-        """Where submit and wait find their results: a call of each per step, from one thread at a time."""
-        self._fence, self._dispatches, self._timers = C.c_uint64(), C.c_int(), C.c_int()
-        self._refs = C.byref(self._fence), C.byref(self._dispatches), C.byref(self._timers)
 
     @classmethod
     def _wrap(cls, handle) -> "HipBackend":
@@ -409,7 +416,6 @@ class HipBackend:
         b.heap = None
         b.shader_set_hash = None
         b._borrowed = True
-        b._results()
         return b
 
     @property
@@ -448,18 +454,20 @@ class HipBackend:
         return HipCommandList(self, l, reusable)
 
     def submit(self, commands: "HipCommandList", repeat: int = 1) -> Submission:
-        rc = lib().lrm_hip_submit(self._h, commands._h, repeat, self._refs[0])
+        r = _results
+        rc = lib().lrm_hip_submit(self._h, commands._h, repeat, r.refs[0])
         if rc:
             check(rc)
-        return Submission(self._fence.value)
+        return Submission(r.fence.value)
 
     def wait(self, submission: int) -> Completion:
-        _, nd, nt = self._refs
-        rc = lib().lrm_hip_wait(self._h, int(submission), nd, nt)
+        r = _results
+        rc = lib().lrm_hip_wait(self._h, int(submission), r.refs[1], r.refs[2])
         if rc:
             check(rc)
-        timers, dispatches = [], self._dispatches.value
-        for i in range(self._timers.value):
+        dispatches, n = r.dispatches.value, r.timers.value
+        timers = []
+        for i in range(n):
             name = C.create_string_buffer(128)
             st, du = C.c_int64(), C.c_int64()
             check(lib().lrm_hip_timer(self._h, int(submission), i, name, 128, C.byref(st), C.byref(du)))
