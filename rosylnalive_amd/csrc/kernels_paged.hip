@@ -401,6 +401,13 @@ __device__ __forceinline__ float2 load_part2(__amdgpu_buffer_rsrc_t r, int word)
 }
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
+// Weights go into their product with the values rounded to the cache's type, relative to a reference that the largest may
+// exceed by 2^8. fp16 ends at 2^-24, which tens of thousands of small weights behind a few large ones would fall below (64,000 of
+// 2^-25 together are 0.002 of the largest), so they are 2^kUp of what they are: at most 2^15, and lost below 2^-32.
+// Their sum is formed from the same, so the results are not changed otherwise.
+template <typename T>
+constexpr float kUp = std::is_same_v<T, _Float16> ? 7.f : 0.f;
+
 // Values that are no finite numbers, at keys that one column of a tile sees and another does not: zero times such a value is
 // NaN, so they are taken out of the product and added to the columns that see them alone. A second product with 0 / 1
 // weights counts them: infinity as 1, minus infinity as 128, NaN as both; fewer than 128 keys, so float32 holds the counts.
@@ -610,7 +617,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(AttnArgs a, uint32_t k_byt
 #pragma unroll
             for (int d = 0; d < DT; ++d) o[d] *= alpha;
         }
-        const float mc = m_run == -INFINITY ? 0.f : m_run * a.scale_log2;
+        const float mc = m_run == -INFINITY ? 0.f : m_run * a.scale_log2 - kUp<T>;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             sc[e] = __builtin_amdgcn_exp2f(fmaf(sc[e], a.scale_log2, -mc));
@@ -1174,7 +1181,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : HD == 64 ? 3 : 2) void k_att
             if (__any(grow)) {
                 const float alpha = grow ? __builtin_amdgcn_exp2f((m_run - mx) * a.scale_log2) : 1.0f;
                 m_run = grow ? mx : m_run;
-                mc = m_run == -INFINITY ? 0.f : m_run * a.scale_log2;
+                mc = m_run == -INFINITY ? 0.f : m_run * a.scale_log2 - kUp<T>;
                 l_run *= alpha;
 #pragma unroll
                 for (int d = 0; d < DT; ++d) o[d] *= alpha;

@@ -476,6 +476,42 @@ def test_attention_keys_that_are_not_finite(dtype, lens, x):
     assert np.array_equal(got[before], plain[before])
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("fresh", [1, 20])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attention_many_small_weights(dtype, fresh, hd):
+    """A few keys that outweigh all others, with values of zero, before tens of thousands of weights of 2^-25 (in fp16 half of its
+    smallest step) whose values alone make the result: none may be lost to the type's underflow. So many requests over the
+    same pages that a workgroup has whole contexts."""
+    page, blocks, R, d = 64, 1000, 600 // fresh, DT[dtype]
+    n = blocks * page
+    k, v = np.zeros((n, hd)), np.full((n, hd), 1000.0)
+    top = 25.4 * np.log(2)
+    k[:512:32], v[:512:32] = 2.0, 0.0  # (every wave's first keys)
+    q = np.full((R * fresh, hd), 0.5)
+    sc = top / hd  # the score of the large keys is hd * sc, of the others 0
+    kb, vb = O.to_bits(d, k.reshape(blocks, 1, page, hd)), O.to_bits(d, v.reshape(blocks, 1, page // 8, 8, hd).swapaxes(3, 4))
+    u = lambda a: (U32, np.shape(a), 0, np.asarray(a, np.uint32))  # noqa: E731
+    s = Session({"q": (d, q.shape, RO, O.to_bits(d, q)), "k_cache": (d, kb.shape, RO, kb), "v_cache": (d, _rank4(vb), RO, vb),
+                 "table": u(np.tile(np.arange(blocks), (R, 1))), "starts": u(np.arange(R + 1) * fresh),
+                 "context": u(np.full(R, n)), "y": (d, q.shape, 0, None),
+                 "workspace": u(np.zeros(attention_paged_workspace_words(R, R * fresh, 1, 1, hd)))})
+    try:
+        y = O.from_bits(d, s.run("attention_paged", ["y"], **{m: m for m in s.spec}, requests=R, tokens=R * fresh,
+                                 max_fresh=fresh, q_heads=1, kv_heads=1, head_dim=hd, blocks=blocks, page=page, pages=blocks,
+                                 scale=sc)["y"])
+    finally:
+        s.close()
+    seen = n - fresh + 1 + np.tile(np.arange(fresh), R)
+    small = np.exp(-hd * float(np.float32(sc)))
+    want = (1000 * (seen - 16) * small / (16 + (seen - 16) * small))[:, None]
+    # a score's float32 error (its product, the scale, the reference), a weight's rounding and the result's to the type, the float32
+    # sums over the keys, and the weights that may still fall below the type's smallest step: in fp16 2^-32 of the largest each
+    rel = 2 * O.EPS_HALF[d] + 2 * (hd + 8) * O.U24 * top + (n + 16) * O.U24
+    tiny = 1000 * n * 2.0 ** -32 / 16 if d == F16 else 0.0
+    assert np.all(np.abs(y - want) <= rel * want + tiny), (np.abs(y - want).max(), want.max())
+
+
 def test_attention_replayed_with_other_lengths():
     """One recorded list, replayed as the lengths, the table and the queries on the device change, with the shorter and the
     longer in either order: a launch leaves nothing in the workspace that the next could take for its own."""
