@@ -481,8 +481,9 @@ uint64_t Device::submit(CommandList* l, uint32_t repeat) {
     if (repeat < 1) contract_fail("a submission runs its list at least once");
     if (repeat > 1 && !l->reusable_) contract_fail("only a reusable list can be replayed");
     HIPC(hipSetDevice(index_));
-    const bool few = uint64_t(l->cmds_.size()) * repeat <= kDirectLaunches;
-    if (marked_ < next_fence_ - 1 && (!few || host_ns() - marked_ns_ >= kMarkNs)) mark(next_fence_ - 1);
+    const int64_t now = host_ns();
+    const bool burst = uint64_t(l->cmds_.size()) * repeat <= kDirectLaunches && now - submitted_ns_ < kBurstNs;
+    if (marked_ < next_fence_ - 1 && (!burst || now - marked_ns_ >= kMarkNs)) mark(next_fence_ - 1);
     Pending pend{};
     pend.dispatches = l->dispatches_ * int(repeat);
     if (!l->reusable_) {
@@ -567,7 +568,8 @@ uint64_t Device::submit(CommandList* l, uint32_t repeat) {
     }
     uint64_t fence = next_fence_++;
     pending_[fence] = std::move(pend);
-    if (!few || host_ns() - marked_ns_ >= kMarkNs) mark(fence);
+    if (!burst) mark(fence);
+    submitted_ns_ = host_ns();
     return fence;
 }
 

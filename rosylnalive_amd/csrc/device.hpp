@@ -253,20 +253,21 @@ class Device {
     std::map<uint64_t, Pending> pending_;
     // Completion of submissions: events on the stream, each for every submission up to its own, oldest first. Recording one
     // costs 4 us of host time on MI355X, more than a kernel's launch (2.6 us), so submissions of up to kDirectLaunches
-    // commands that follow each other within kMarkNs share one. Before anything else is launched behind a submission without
-    // an event (more commands, or kMarkNs later) it gets one, so no wait ever covers that later work; a wait for a submission
-    // that has none behind it yet records one then.
+    // commands that follow the one before them within kBurstNs have none of their own: the next event, at most kMarkNs
+    // later, is theirs. It is recorded before anything else is launched behind them (more commands, or after a pause), so
+    // no wait ever covers that later work, and by a wait that comes before. (A submission after a pause has its event behind
+    // its launch, where recording it costs no latency: 8 us in front of it.)
     struct Mark {
         uint64_t fence;
         hipEvent_t event;
     };
-    static constexpr int64_t kMarkNs = 50000;
+    static constexpr int64_t kMarkNs = 50000, kBurstNs = 25000;
     void mark(uint64_t fence);
     void reach(uint64_t fence);  // waits until every submission up to `fence` has completed
     std::deque<Mark> marks_;
     std::vector<hipEvent_t> spare_events_;
     uint64_t marked_ = 0;         // the last submission that was marked, and the host clock then
-    int64_t marked_ns_ = 0;
+    int64_t marked_ns_ = 0, submitted_ns_ = 0;  // (and when the last submission had been made)
     uint64_t reached_ = 0;        // submissions up to this one have completed
     std::map<uint64_t, Completion> done_;  // the last kKeptCompletions waited on, by fence
 
