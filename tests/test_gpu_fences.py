@@ -1,11 +1,13 @@
 """Submissions that share a completion event: short lists made right behind each other, waited for in any order; and replays of
 short reusable lists, which are launched again rather than captured, next to captured ones."""
+import ctypes as C
 import time
 
 import numpy as np
 import pytest
 
 from gpu_session import Session
+from rosylnalive_amd import _native
 from rosylnalive_amd.gpu_core import DType, GpuContractException
 
 pytestmark = pytest.mark.gpu
@@ -147,3 +149,45 @@ def test_a_wait_does_not_cover_long_work_submitted_later(long, form, pause):
     assert good >= 4  # (the host may be held up once)
     short.release()
     late.release()
+
+
+@pytest.mark.parametrize("order", ["first to last", "last to first", "every third", "shuffled"])
+@pytest.mark.parametrize("launches", [5, 6, 40])
+def test_results_are_there_when_a_wait_returns(launches, order):
+    """Submissions that take the GPU much longer than the host, right behind each other (those of up to six launches share events,
+    longer ones have their own), each with a result of its own as its last launch: when a wait returns, a copy that nothing
+    orders behind the device's stream (the null stream's, from the tensor's address) finds the result, and those of all
+    submissions before it."""
+    n, count = 1 << 25, 12
+    x = np.arange(1, N + 1, dtype=np.float32)
+    s = Session({"big": (F32, (n,), 0, np.zeros(n, np.float32)), "x": (F32, (N,), 0, x),
+                 **{f"out{i}": (F32, (N,), 0, None) for i in range(count)}})
+    copy = C.CDLL(_native.LIB_PATH).hipMemcpy  # of the runtime that the library runs on
+    copy.argtypes = [C.c_void_p, C.c_void_p, C.c_size_t, C.c_int]
+    lists = []
+    for i in range(count):
+        cl = s.backend.begin(reusable=i % 2 == 1)
+        for _ in range(launches - 1):
+            cl.dispatch("scale_f32", s.fields("scale_f32", x="big", y="big", n=n, a=1.0))
+        _scale(s, cl, float(i + 2), dst=f"out{i}")
+        lists.append(cl)
+    turn = list(range(count))
+    if order == "last to first":
+        turn.reverse()
+    elif order == "every third":
+        turn = turn[2::3] + turn[0::3] + turn[1::3]
+    elif order == "shuffled":
+        np.random.default_rng(6).shuffle(turn)
+    at = [s.heap.view(s.tok[f"out{i}"]).address for i in range(count)]
+    got = np.empty(N, np.float32)
+    try:
+        fences = [s.backend.submit(cl) for cl in lists]
+        for i in turn:
+            assert s.backend.wait(fences[i]).dispatches == launches
+            for j in range(i + 1):
+                assert copy(got.ctypes.data, at[j], got.nbytes, 2) == 0
+                assert np.array_equal(got, x * np.float32(j + 2)), (i, j)
+    finally:
+        for cl in lists:
+            cl.release()
+        s.close()
