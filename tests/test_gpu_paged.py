@@ -186,6 +186,54 @@ def test_append_rows_without_a_slot():
         _append_case(dtype, F32, 4, 2, 128, 16, rows, 1, seed=9)
 
 
+@pytest.mark.parametrize("T", [4095, 4096, 4097])
+@pytest.mark.parametrize("dtype,qkv,qh,kvh,hd", [("f16", "f32", 16, 8, 128), ("bf16", "bf16", 14, 2, 64), ("f16", "f16", 1, 1, 64)])
+def test_append_thousands_of_rows(T, dtype, qkv, qh, kvh, hd):
+    """On both sides of the rows from which a wave takes a row's heads whole."""
+    rows = _rows((0, 256, 2000), (5, 256 * 9 + 3, 1001), (0, 256 * 14, 256), (40, 256 * 16 + 77, 800))
+    rows += [(i, 1 + 7 * i) for i in range(T - 3 - len(rows))]
+    assert len({slot for _, slot in rows}) == len(rows)
+    _append_case(DT[dtype], F32 if qkv == "f32" else DT[qkv], qh, kvh, hd, 256, rows, 3, seed=T, max_pos=2100)
+
+
+def test_append_more_workgroups_than_a_grid_row():
+    """240,001 rows take 67,502 workgroups, more than the 65,535 of a grid's row."""
+    r = np.random.default_rng(40)
+    T, hd, page, pages, MP = 240001, 64, 256, 940, 512
+    qkv = r.standard_normal((T, 3 * hd)).astype(np.float16)
+    ang = np.arange(MP)[:, None] * 1e4 ** (-np.arange(0, hd, 2) / hd)[None]
+    cos, sin = np.cos(ang).astype(np.float32), np.sin(ang).astype(np.float32)
+    qn, kn = (O.to_bits(BF16, 1 + 0.2 * r.standard_normal(hd)) for _ in range(2))
+    slots, positions = np.arange(T) + 7, np.arange(T) % MP
+    slots[100000:] = np.concatenate([r.permutation(slots[100000:150000]), slots[150000:]])
+    kc, vc = (np.full(n, POISON_16, np.uint16) for n in ((pages, 1, page, hd), (pages, 1, page // 8, hd, 8)))
+    u = lambda a: (U32, np.shape(a), 0, np.asarray(a, np.uint32))  # noqa: E731
+    s = Session({"qkv": (F16, qkv.shape, RO, qkv), "q_norm": (BF16, (hd,), RO, qn), "k_norm": (BF16, (hd,), RO, kn),
+                 "cos_table": (F32, cos.shape, RO, cos), "sin_table": (F32, sin.shape, RO, sin), "starts": u([0, T - 2]),
+                 "positions": u(positions), "slots": u(slots), "q": (F16, (T, hd), 0, None), "k_cache": (F16, kc.shape, 0, kc),
+                 "v_cache": (F16, _rank4(vc), 0, vc)})
+    try:
+        got = s.run("qk_norm_rope_append_paged", ["q"], **{n: n for n in s.spec}, requests=1, tokens=T, q_heads=1, kv_heads=1,
+                    head_dim=hd, max_pos=MP, page=page, pages=pages, eps=1e-6)
+        gk, gv = s.read("k_cache").reshape(-1, hd), s.read("v_cache").reshape(-1, hd, 8)
+    finally:
+        s.close()
+    x = qkv.astype(np.float64).reshape(T, 3, hd)
+    w = np.stack([O.from_bits(BF16, qn), O.from_bits(BF16, kn)])
+    h = w * x[:, :2] / np.sqrt((x[:, :2] ** 2).mean(2, keepdims=True) + 1e-6)
+    a, b, c, d = h[..., :hd // 2], h[..., hd // 2:], cos[positions][:, None], sin[positions][:, None]
+    want = np.concatenate([a * c - b * d, b * c + a * d], 2)
+    # (the bound of paged_oracle.append, half a step of fp16 and its smallest)
+    bound = np.tile(np.abs(a) + np.abs(b), 2) * 16 * O.U24 + 2.0 ** -11 * np.abs(want) + 2.0 ** -25
+    mine, at = np.arange(T) < T - 2, slots[:T - 2]
+    f = O.from_bits
+    assert np.all(np.abs(f(F16, got["q"]) - want[:, 0])[mine] <= bound[:, 0][mine]) and np.all(got["q"][~mine] == POISON_16)
+    assert np.all(np.abs(f(F16, gk[at]) - want[mine, 1]) <= bound[mine, 1])
+    assert np.array_equal(gv[at // 8, :, at % 8], qkv.view(np.uint16).reshape(T, 3, hd)[mine, 2])
+    rest = np.setdiff1d(np.arange(pages * page), at)
+    assert np.all(gk[rest] == POISON_16) and np.all(gv[rest // 8, :, rest % 8] == POISON_16)
+
+
 def test_append_no_rows():
     for pad in (1, 70):
         _append_case(F16, F32, 4, 2, 128, 16, [], pad, seed=10)
@@ -331,6 +379,20 @@ def test_attention_many_items(dtype, qh, kvh, hd):
     r = np.random.default_rng(13)
     lens = [(int(x), int(f)) for x, f in zip(r.integers(0, 700, 90), r.choice([0, 1, 1, 1, 2, 20], 90))] + [(300, 150), (1400, 40)]
     _attn_case(DT[dtype], qh, kvh, hd, 32, lens, pad=2)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("qh,kvh,hd", [(16, 8, 128), (32, 8, 128), (4, 4, 64)])
+@pytest.mark.parametrize("batch", ["own", "uneven", "many"])
+def test_attention_mixed_batches_in_wide_tables(dtype, qh, kvh, hd, batch):
+    """Batches of at least 16 requests that bring few rows each, in tables of more than 2048 positions (a launch of its own joins
+    the split items): workgroups of their own per item, too few of them for the long ones, and more items than workgroups."""
+    r = np.random.default_rng(14)
+    single = lambda n, top: [(int(x), 1) for x in r.integers(0, top, n)]  # noqa: E731
+    lens = {"own": single(17, 1500) + [(2200, 40), (0, 70), (1000, 5)],
+            "uneven": single(57, 60) + [(4000, 30), (2900, 17), (3100, 2)],
+            "many": single(40, 500) + [(30, 0), (2300, 33)] + single(40, 300) + [(0, 0), (70, 90)]}[batch]
+    _attn_case(DT[dtype], qh, kvh, hd, 32, lens, pad=4)
 
 
 @pytest.mark.parametrize("qh,kvh,hd", [(256, 1, 64), (100, 1, 128), (34, 2, 64), (17, 1, 128)])
