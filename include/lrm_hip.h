@@ -176,7 +176,7 @@ int lrm_attention_paged_workspace(uint32_t requests, uint32_t tokens, uint32_t q
  * its first submission or, for a list of a few dispatches, launch by launch; it may not hold timers. One-shot lists are
  * closed by Submit. lrm_hip_wait returns once the submission has completed; one of up to six commands (a list's times
  * `repeat`) may share its completion with others of up to six made right behind it, each less than 25 us after the one before
- * and the last less than 50 us after it, and never with more or later work. */
+ * and the last less than 75 us after it, and never with more or later work. */
 typedef struct lrm_hip_list lrm_hip_list;
 int lrm_hip_begin(lrm_hip_device *d, int reusable, lrm_hip_list **out);
 int lrm_hip_dispatch(lrm_hip_list *l, uint32_t kernel, const uint32_t words[32]);

@@ -481,9 +481,8 @@ uint64_t Device::submit(CommandList* l, uint32_t repeat) {
     if (repeat < 1) contract_fail("a submission runs its list at least once");
     if (repeat > 1 && !l->reusable_) contract_fail("only a reusable list can be replayed");
     HIPC(hipSetDevice(index_));
-    const int64_t now = host_ns();
-    const bool burst = uint64_t(l->cmds_.size()) * repeat <= kDirectLaunches && now - submitted_ns_ < kBurstNs;
-    if (marked_ < next_fence_ - 1 && (!burst || now - marked_ns_ >= kMarkNs)) mark(next_fence_ - 1);
+    const bool burst = uint64_t(l->cmds_.size()) * repeat <= kDirectLaunches && host_ns() - submitted_ns_ < kBurstNs;
+    if (!burst && marked_ < next_fence_ - 1) mark(next_fence_ - 1);
     Pending pend{};
     pend.dispatches = l->dispatches_ * int(repeat);
     if (!l->reusable_) {
@@ -568,8 +567,8 @@ uint64_t Device::submit(CommandList* l, uint32_t repeat) {
     }
     uint64_t fence = next_fence_++;
     pending_[fence] = std::move(pend);
-    if (!burst) mark(fence);
     submitted_ns_ = host_ns();
+    if (!burst || submitted_ns_ - marked_ns_ >= kMarkNs) mark(fence);
     return fence;
 }
 

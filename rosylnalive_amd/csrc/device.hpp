@@ -253,10 +253,10 @@ class Device {
     std::map<uint64_t, Pending> pending_;
     // Completion of submissions: events on the stream, each for every submission up to its own, oldest first. Recording one
     // costs 4 us of host time on MI355X, more than a kernel's launch (2.6 us), so submissions of up to kDirectLaunches
-    // commands that follow the one before them within kBurstNs have none of their own: the next event, at most kMarkNs
-    // later, is theirs. It is recorded before anything else is launched behind them (more commands, or after a pause), so
-    // no wait ever covers that later work, and by a wait that comes before. (A submission after a pause has its event behind
-    // its launch, where recording it costs no latency: 8 us in front of it.)
+    // commands that follow the one before them within kBurstNs share one, kMarkNs after the last. It is recorded behind its
+    // submission's launch, where it costs no latency (in front of one 8 us), but for submissions that have none yet when
+    // anything else follows, more commands or after a pause: then in front of that, so no wait ever covers such later work. A
+    // wait for a submission without an event behind it records one.
     struct Mark {
         uint64_t fence;
         hipEvent_t event;
