@@ -158,14 +158,20 @@ int lrm_hip_denormal_probe(lrm_hip_device *d, int *mode, uint32_t results[7]);
  *   [head_dim], cos_table and sin_table [max_pos][head_dim / 2]: per head x w / sqrt(mean x^2 + eps), rotated by the row's
  *   position, q [tokens][q_heads head_dim] and the caches' entries at the row's slot; values as they are. Rows of the batch
  *   are the first starts[requests]. A row whose position is not below max_pos gives zeros and appends nothing; one without a
- *   slot gives q and appends nothing. Slots are distinct: where two rows name one, it is not said whose parts stay.
+ *   slot gives q and appends nothing. Slots are distinct: where two rows name one, it is not said whose parts stay. Float32
+ *   until the one rounding to the cache's type; in fp16 what is past 65,504 is stored as an infinity, and no call reports it
+ *   (LRM_E_RANGE speaks of the executor's own kernels).
  * 49 attention_paged: y = softmax(scale q k^T) v of the new rows, causal (row i of a request sees context - new + i + 1
  *   positions; positions whose page is none are left out; a row that sees none gives zeros), any number of rows per request in
  *   one dispatch. max_fresh: 0, or the most rows of a request: with max_fresh * q_heads / kv_heads <= 16 the form for single
  *   tokens runs (rows past max_fresh are left as they were). q_heads / kv_heads is at most 256. The same lengths give the same
- *   bits. What a row gives does not depend on the tokens behind it, whatever they hold.
+ *   bits. What a row gives does not depend on the tokens behind it, whatever they hold. Scores, maxima, sums and products are
+ *   float32; for the product with v the weights are rounded to the cache's type (bf16 keeps 8 bits of them, fp16 11 and
+ *   those down to 2^-32 of the largest that came before), their sum is of the unrounded ones: on normally distributed
+ *   inputs results are about 1.4 times as far from exact ones as their own rounding to the type would leave them.
  *
- * u32 words of attention_paged's workspace for dispatches of up to that many requests and tokens. The workspace's words must
+ * u32 words of attention_paged's workspace for dispatches of up to that many requests and tokens (68 MB for heads of 128 and
+ * 34 for heads of 64, whatever the batch; 8.5 and 4.3 where tokens * q_heads / kv_heads <= 16). The workspace's words must
  * be zero before the first launch (a new heap's are); every launch leaves the ones that it counts in at zero, so lists with
  * other lengths, tokens or max_fresh may share it one after the other. Dispatches that may overlap need a workspace each. */
 int lrm_attention_paged_workspace(uint32_t requests, uint32_t tokens, uint32_t q_heads, uint32_t kv_heads,

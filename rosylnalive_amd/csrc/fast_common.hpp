@@ -173,8 +173,9 @@ __device__ __forceinline__ float wave_max(float v) { return cross_rows_max(row_m
 
 // ---------------------------------------------------------------- the fp16 range monitor
 // The fast path narrows some activations and the K/V cache to fp16, whose range ends at 65,504: a value the float32
-// reference keeps (a SwiGLU outlier, a large projection) becomes inf there. Every kernel that stores such a value ORs
-// the bit of its site into a sticky device word when a half it stores is inf or NaN; the executor reads and clears the
+// reference keeps (a SwiGLU outlier, a large projection) becomes inf there. Every kernel of the executor's paths that
+// stores such a value (not the paged cache's, which no executor runs: an infinity there would fail another model's next
+// call, whose words these are) ORs the bit of its site into a sticky device word when a half it stores is inf or NaN; the executor reads and clears the
 // word after each forward and decode run and fails the call with the sites named, instead of passing the inf on. The
 // word starts at zero (static storage) and each code object including this header holds its own, one per GPU.
 enum F16Site : uint32_t {

@@ -1,7 +1,8 @@
 // A key/value cache in pages for batches of requests of any lengths (ids 47..49, the fast set): the step's page tables and
 // slots from the request lengths, the append of new keys and values to their slots, and the attention of the new tokens
 // over their requests' pages. Lengths, tables and slots are device memory, so a recorded list replays for new ones; every
-// index that comes from device memory is checked against its tensor before it is used.
+// index that comes from device memory is checked against its tensor, and every sum of lengths against its word, before it
+// is used.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -211,8 +212,9 @@ __device__ __forceinline__ float sum_lanes(float v) {
 // ---------------------------------------------------------------- 48 qk_norm_rope_append_paged
 // n = w x / sqrt(mean x^2 + eps) over a head, (a, b) its halves: (a cos - b sin, b cos + a sin) at the row's position; values
 // as they are. Everything is float32 until the one rounding to the cache's type (nearest even) at the stores.
-// Bound by the projections' bytes (9,200 rows of 32 + 8 + 8 heads of 128 in bf16: 47 us, 5.2 TB/s; 512 rows 5.2 us). Queries and keys: a head is 4 to 16 lanes with 16 bytes of its lower and of its upper
-// half each, so a lane holds the pairs that the rotation turns, the sum of squares is a few DPP adds, and a wave takes 4 to
+// Values past fp16's range become infinities, as its rounding has it. Bound by the projections' bytes (9,200 rows of
+// 32 + 8 + 8 heads of 128 in bf16: 47 us, 5.2 TB/s, back to back; 512 rows 5.2 us, the latency of three loads that wait for each
+// other). Queries and keys: a head is 4 to 16 lanes with 16 bytes of its lower and of its upper half each, so a lane holds the pairs that the rotation turns, the sum of squares is a few DPP adds, and a wave takes 4 to
 // 16 heads of a row at a time; the row's rotation and the norm weights are loaded once per wave. Values: a wave takes the
 // runs of rows that begin in its 8 rows, a run being rows whose slots follow each other in one tile of 8 positions; a
 // whole run's 8 rows of a dim are one 16-byte store, and shorter runs (a single token, the ends of a chunk) store each value
@@ -449,8 +451,9 @@ __device__ __forceinline__ float add_odd(float o, float count) {
 // Bound by the cache's bytes, so every wave streams its own keys straight into the registers that the matrix
 // instruction reads (no LDS, no barrier), two units in flight, and the four waves of a workgroup meet once per item. All
 // units are shared out evenly over 512 workgroups, so a long context spreads over the GPU and a batch of uneven ones leaves no
-// CU behind; the last part of an item to arrive joins its partials. Measured: 200 requests of up to 4000 positions 262 us, 16
-// of 8192 88 us (both 6.1 TB/s), one of 65,701 47 us (5.7 TB/s), one of 700 8.6 us alone.
+// CU behind; the last part of an item to arrive joins its partials. Measured, calls back to back on three streams: 200
+// requests of up to 4000 positions 262 us, 16 of 8192 88 us (both 6.1 TB/s), one of 65,701 47 us (5.7 TB/s); single dispatches
+// after a pause, at lower clocks: 287, 101 and 65 us, one of 700 8.6.
 //
 // A unit is 128 keys of an item, 32 per wave. S^T = K Q^T on 16 x 16 x 32 tiles: the two tiles' rows i hold the keys
 // 8 (i / 4) + 4 tile + i % 4, so that lane group g = lane / 16 gets the scores of the eight keys 8 g .. 8 g + 7 of its column:
@@ -890,9 +893,9 @@ __device__ __forceinline__ void join_item(const AttnArgs& a, const Split& p, int
 // under the maxima of block n + 1. The rows of S^T's tiles hold the keys in the order in which P^T wants them (bits 2 and 3
 // of the row exchanged), so weights never cross lanes. They are rounded to the cache's type for the product, as its values
 // are, at most 2^8 above the reference maximum; scores, sums and products are float32.
-// Measured: 4096 rows on 28,672 positions (16 / 8 heads of 128, fp16) 938 us, 1100 TFLOP/s: the card's power limit, at which
-// a library product of 8192^3 reaches 1159; matrix cores busy 55 % of the cycles. A prompt of 2048 30 us (570 TFLOP/s): 4 us
-// to start, 11 blocks of 1.9 us, 2 to store, 8 for the join.
+// Measured, calls back to back: 4096 rows on 28,672 positions (16 / 8 heads of 128, fp16) 936 to 989 us by card, 1100 to 1040
+// TFLOP/s: the card's power limit, at which a library product of 8192^3 reaches 1159; matrix cores busy 55 % of the cycles. A
+// prompt of 2048 30 us (570 TFLOP/s): 4 us to start, 11 blocks of 1.9 us, 2 to store, 8 for the join.
 template <typename T, int HD, int NW>
 __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : HD == 64 ? 3 : 2) void k_attn_tiles(AttnArgs a, uint32_t bytes) {
     using M = Mfma<T>;
@@ -1067,11 +1070,11 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : HD == 64 ? 3 : 2) void k_att
 
     const __amdgpu_buffer_rsrc_t k_rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(a.kc), 0, bytes, 0x00020000);
     const __amdgpu_buffer_rsrc_t v_rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(a.vc), 0, bytes, 0x00020000);
-    // this wave moves keys 8 wv .. + 7 of a block, 16 bytes per lane and load: both caches hold them in one piece
+    // this wave moves the WK keys of a block from WK wv on, 16 bytes per lane and load: both caches hold them in one piece
     int kst[LPB];  // where a K chunk goes in its block
 #pragma unroll
     for (int i = 0; i < LPB; ++i) {
-        const int p = 64 * i + lane, row = p / CH, ch = p % CH;  // row of the wave's 8, place in the row
+        const int p = 64 * i + lane, row = p / CH, ch = p % CH;  // row of the wave's WK, place in the row
         kst[i] = (WK * wv + row) * KR + ch * 16;
     }
     // operand reads: K row of matrix row c32 is key 16 (c32 / 16) + 8 (c32 / 4 % 2) + 4 (c32 / 8 % 2) + c32 % 4
@@ -1125,7 +1128,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : HD == 64 ? 3 : 2) void k_att
             const uint32_t off = uint32_t((j0 + j) * KB + WK * wv) & ((1u << a.page_log2) - 1);
             soff = id < a.pages ? int((((id * uint32_t(kvh) + hk) << a.page_log2) + off) * RB) : 0;
         };
-        // the chunks of this wave on their way to LDS: two blocks of each cache
+        // the chunks of this wave on their way to LDS: SETS blocks of each cache
         u32x4 rk[SETS][LPB], rv[SETS][LPB];
         auto load_k = [&](auto set, int i, int soff) __attribute__((always_inline)) {
             rk[decltype(set)::value % SETS][i] = __builtin_amdgcn_raw_buffer_load_b128(k_rsrc, 16 * lane + 1024 * i, soff, 0);
@@ -1256,7 +1259,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : HD == 64 ? 3 : 2) void k_att
 
         // Step n stores K(n + 2) and V(n + 1) under its second half, loaded by step n - 2 (a block that is not in the XCD's L2
         // takes about a step to arrive), and loads K(n + 4) and V(n + 3) into the registers that this frees (behind the last
-        // block: the last one again, never read).
+        // block: the last one again, never read). With one set of registers: loaded by step n - 1, and K(n + 3) and V(n + 2).
         using A0 = std::integral_constant<int, 0>;
         using A1 = std::integral_constant<int, 1>;
         int s1, s2, s3, s4;
@@ -1296,7 +1299,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : HD == 64 ? 3 : 2) void k_att
 #pragma unroll
             for (int i = 0; i < 2; ++i) kp[i] = *reinterpret_cast<const u32x4*>(lds + 32 * KR + kbase + 32 * i);
         }
-        int kslot = 0, n = 0;  // kslot = n % 3
+        int kslot = 0, n = 0;  // kslot = n % KN
         auto none = [](int, int) {};
         // PLAIN: every column sees all of this block and the next, all have pages, and more follow: nothing to ask
         auto step = [&](auto set, auto plain) __attribute__((always_inline)) {

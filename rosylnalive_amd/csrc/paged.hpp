@@ -12,7 +12,6 @@ namespace paged {
 // [head_dim] and the value cache [pages][kv_heads][page / 8][head_dim][8]: position p of a page at (p / 8) 8 head_dim +
 // dim 8 + p % 8 of its head's part. The values' product reads 8 positions of one dim per lane, so with 8 positions
 // innermost every such read is 16 bytes, 16 lanes read 256 contiguous ones, and the layout is the same for every page size.
-constexpr int kVTile = 8;
 
 // No page, no slot.
 constexpr uint32_t kNone = 0xFFFFFFFFu;
@@ -29,10 +28,10 @@ inline bool page_ok(uint32_t page) { return page >= 16 && page <= 256 && (page &
 // the part of the one that it begins and does not end. Before them stand kGroups words, in which the items count their parts
 // in where the last one to arrive joins them (word w for the one that w begins; zero between launches), and for the tiles what
 // a join in a launch of its own has to know, eight words per workgroup.
-constexpr uint32_t kGroups = 512;  // the most workgroups of a launch
+constexpr uint32_t kGroups = 512;  // the most workgroups that share out the work
 // Items of few columns (a request's rows x the heads of a group up to 16): two workgroups per CU, units of 128 keys.
 constexpr uint32_t kRowsGroups = 512, kRowsKeys = 128, kRowsCols = 16;
-// Items of many columns: tiles of 32 columns per wave, units of 64 keys, 2048 waves in all: workgroups of eight, one per CU, or of
+// Items of many columns: tiles of 32 columns per wave, units of 64 keys, 2048 waves in all (times of calls back to back): workgroups of eight, one per CU, or of
 // four, two per CU, so that one's start, end and barriers run beside the other's products, and a single token among the
 // chunks holds half as much. Four for heads of 64 (40 mixed requests 31.6 us against 37.8, 3621 rows on 2581 positions 78.5 and
 // 80.8), and for heads of 128, whose blocks then have a place less in LDS, where most requests bring few rows (29 requests
@@ -58,7 +57,8 @@ constexpr uint32_t tile_slots(uint32_t waves) { return kGroups + 8 * tile_groups
 constexpr uint64_t slot_words(uint64_t cols, uint64_t head_dim) { return cols * (2 + head_dim); }
 
 // u32 words of attention_paged's workspace. The lengths of a launch come from the device, so any launch of a batch may
-// split; one whose requests could not together have more than 16 columns on a KV head never takes the tiles.
+// split between all its workgroups, however many requests it has: 68 MB for heads of 128 and 34 for heads of 64; one whose
+// requests could not together have more than 16 columns on a KV head never takes the tiles, 8.5 and 4.3 MB.
 inline uint64_t workspace_words(uint64_t requests, uint64_t tokens, uint64_t q_heads, uint64_t kv_heads,
                                 uint64_t head_dim) {
     (void)requests;
