@@ -182,6 +182,18 @@ __device__ __forceinline__ uint32_t pack(float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2){a, b}, t2));
 }
 
+// Two results of the attention to a pair of the type. A result is a mean of the values, but its weights' rounding may put it up
+// to 2^-11 past them, and next to fp16's end past that: it ends there too (an infinity comes from the values and stays).
+template <typename T>
+__device__ __forceinline__ uint32_t pack_mean(float a, float b) {
+    if constexpr (std::is_same_v<T, _Float16>) {
+        constexpr float end = 65504.f;
+        a = fabsf(a) < INFINITY ? __builtin_amdgcn_fmed3f(a, -end, end) : a;
+        b = fabsf(b) < INFINITY ? __builtin_amdgcn_fmed3f(b, -end, end) : b;
+    }
+    return pack<T>(a, b);
+}
+
 // N consecutive elements as floats, in one load
 template <typename T, int N>
 __device__ __forceinline__ void load_n(const T* p, float (&v)[N]) {
@@ -686,7 +698,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(AttnArgs a, uint32_t k_byt
                 const float inv = sum != 0.f ? 1.0f / sum : 0.f;  // no key at all: zeros
                 const int row = p.row0 + c / group, head = p.h * group + c % group;
                 T* y = static_cast<T*>(a.y) + (size_t(row) * a.qh + head) * HD + d;
-                *reinterpret_cast<uint2*>(y) = make_uint2(pack<T>(v[0] * inv, v[1] * inv), pack<T>(v[2] * inv, v[3] * inv));
+                *reinterpret_cast<uint2*>(y) = make_uint2(pack_mean<T>(v[0] * inv, v[1] * inv), pack_mean<T>(v[2] * inv, v[3] * inv));
             } else {
                 store_part(ws, mine + 2 * int(paged::kRowsCols) + c * HD + d, v);
                 if (d == 0) store_part2(ws, mine + 2 * c, m, sum);
@@ -742,7 +754,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_rows(AttnArgs a, uint32_t k_byt
                         const int row = p.row0 + c / group, head = p.h * group + c % group;
                         T* y = static_cast<T*>(a.y) + (size_t(row) * a.qh + head) * HD + d;
                         *reinterpret_cast<uint2*>(y) =
-                            make_uint2(pack<T>(v[0] * inv, v[1] * inv), pack<T>(v[2] * inv, v[3] * inv));
+                            make_uint2(pack_mean<T>(v[0] * inv, v[1] * inv), pack_mean<T>(v[2] * inv, v[3] * inv));
                     }
                 }
                 if (t == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -878,7 +890,7 @@ __device__ __forceinline__ void join_item(const AttnArgs& a, const Split& p, int
     for (int j = 0; j < N; ++j) {
         const int i = part_d * N + j;  // dims 32 (i / 4) + 8 (i % 4) + 4 h ..
         *reinterpret_cast<uint2*>(y + 32 * (i >> 2) + 8 * (i & 3)) =
-            make_uint2(pack<T>(sum[4 * j] * inv, sum[4 * j + 1] * inv), pack<T>(sum[4 * j + 2] * inv, sum[4 * j + 3] * inv));
+            make_uint2(pack_mean<T>(sum[4 * j] * inv, sum[4 * j + 1] * inv), pack_mean<T>(sum[4 * j + 2] * inv, sum[4 * j + 3] * inv));
     }
 }
 
@@ -1399,8 +1411,8 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : HD == 64 ? 3 : 2) void k_att
 #pragma unroll
                     for (int e = 0; e < 4; ++e)  // dims 32 d + 8 e + 4 h ..
                         *reinterpret_cast<uint2*>(y + 32 * d + 8 * e) =
-                            make_uint2(pack<T>(o[d][4 * e] * inv, o[d][4 * e + 1] * inv),
-                                       pack<T>(o[d][4 * e + 2] * inv, o[d][4 * e + 3] * inv));
+                            make_uint2(pack_mean<T>(o[d][4 * e] * inv, o[d][4 * e + 1] * inv),
+                                       pack_mean<T>(o[d][4 * e + 2] * inv, o[d][4 * e + 3] * inv));
             }
         };
         // the item's parts: part i in slot base + i stride (+ 1 for the first, which its workgroup begins)

@@ -574,6 +574,36 @@ def test_attention_many_small_weights(dtype, fresh, hd):
     assert np.all(np.abs(y - want) <= rel * want + tiny), (np.abs(y - want).max(), want.max())
 
 
+@pytest.mark.parametrize("fresh,blocks", [(1, 4), (1, 40), (2, 40), (9, 40), (40, 30)])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attention_values_at_the_end_of_fp16(hd, fresh, blocks):
+    """Values of +-65,504 at every key: the result is that value whatever the weights, never an infinity, though the rounded
+    weights may be 2^-11 more than their sum (half of that passes fp16's last step). The first keys score less, so that the
+    reference stays at theirs and the other weights are no powers of two."""
+    page, R, group = 64, 1200 if fresh < 9 else 300, 16
+    n, r = blocks * page, np.random.default_rng(31)
+    k = np.full((n, hd), 4.0 / hd)
+    k[:128] = 0.0
+    end = np.where(np.arange(hd) % 3 == 0, -65504.0, 65504.0)
+    q = np.abs(r.standard_normal((R * fresh, group * hd))) * 1.2  # (scores of 3 to 5 in the exponent's powers of two)
+    b = lambda a: O.to_bits(F16, a)  # noqa: E731
+    kb, vb = b(k.reshape(blocks, 1, page, hd)), b(np.tile(end[None, None, None, :, None], (blocks, 1, page // 8, 1, 8)))
+    u = lambda a: (U32, np.shape(a), 0, np.asarray(a, np.uint32))  # noqa: E731
+    s = Session({"q": (F16, q.shape, RO, b(q)), "k_cache": (F16, kb.shape, RO, kb), "v_cache": (F16, _rank4(vb), RO, vb),
+                 "table": u(np.tile(np.arange(blocks), (R, 1))), "starts": u(np.arange(R + 1) * fresh),
+                 "context": u(np.full(R, n)), "y": (F16, q.shape, 0, None),
+                 "workspace": u(np.zeros(attention_paged_workspace_words(R, R * fresh, group, 1, hd)))})
+    try:
+        y = O.from_bits(F16, s.run("attention_paged", ["y"], **{m: m for m in s.spec}, requests=R, tokens=R * fresh,
+                                   max_fresh=fresh, q_heads=group, kv_heads=1, head_dim=hd, blocks=blocks, page=page,
+                                   pages=blocks, scale=1.0)["y"])
+    finally:
+        s.close()
+    # a weight's rounding, the float32 sums over the keys, the result's rounding to a step of 32
+    bound = 65504 * (2.0 ** -11 + 2 * (n + 16) * O.U24) + 16
+    assert np.all(np.abs(y - np.tile(end, group)) <= bound), np.unique(y)
+
+
 def test_attention_replayed_with_other_lengths():
     """One recorded list, replayed as the lengths, the table and the queries on the device change, with the shorter and the
     longer in either order: a launch leaves nothing in the workspace that the next could take for its own."""
