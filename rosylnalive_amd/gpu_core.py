@@ -387,8 +387,9 @@ class _Results(threading.local):
     own; they are made once, since a step has a call of each."""
 
     def __init__(self):
-        self.fence, self.dispatches, self.timers = C.c_uint64(), C.c_int(), C.c_int()
-        self.refs = C.byref(self.fence), C.byref(self.dispatches), C.byref(self.timers)
+        fence, dispatches, timers = C.c_uint64(), C.c_int(), C.c_int()
+        self.submit = fence, C.byref(fence)
+        self.wait = dispatches, timers, C.byref(dispatches), C.byref(timers)
 
 
 _results = _Results()
@@ -454,18 +455,18 @@ class HipBackend:
         return HipCommandList(self, l, reusable)
 
     def submit(self, commands: "HipCommandList", repeat: int = 1) -> Submission:
-        r = _results
-        rc = lib().lrm_hip_submit(self._h, commands._h, repeat, r.refs[0])
+        fence, ref = _results.submit
+        rc = lib().lrm_hip_submit(self._h, commands._h, repeat, ref)
         if rc:
             check(rc)
-        return Submission(r.fence.value)
+        return Submission(fence.value)
 
     def wait(self, submission: int) -> Completion:
-        r = _results
-        rc = lib().lrm_hip_wait(self._h, int(submission), r.refs[1], r.refs[2])
+        nd, nt, nd_ref, nt_ref = _results.wait
+        rc = lib().lrm_hip_wait(self._h, int(submission), nd_ref, nt_ref)
         if rc:
             check(rc)
-        dispatches, n = r.dispatches.value, r.timers.value
+        dispatches, n = nd.value, nt.value
         timers = []
         for i in range(n):
             name = C.create_string_buffer(128)
